@@ -1,0 +1,58 @@
+"""Low-rank adapters of many requests beside a shared projection, on torch CUDA tensors."""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import lib as L
+from .ops import _DTYPE, _need_cuda, _scratch, _stream
+
+_widths: dict = {}
+
+
+def _section_array(sections, n):
+    """The HOST array of section widths; one per tuple of widths (it holds nothing else)."""
+    key = tuple(sections) if sections is not None else (n,)
+    array = _widths.get(key)
+    if array is None:
+        array = _widths[key] = (C.c_int64 * len(key))(*key)
+    return array
+
+
+def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor, adapter_ids: torch.Tensor, sections=None,
+             workspace: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """out[t] = y[t] + scaling[l] * b[l] @ (a[l] @ x[t]) with l = adapter_ids[t]; rows whose id lies outside [0, L) keep y[t].
+
+    y [T, N] is a linear's output for x [T, K]; a [L, R, K] (or [L, S, R, K] for a projection of S linears side by side whose widths are
+    `sections`), b [L, N, R], scaling f32 [L], adapter_ids int32 [T].  `out` may be y."""
+    _need_cuda(y, x, a, b, scaling, adapter_ids, out)
+    t, k = x.shape
+    n = y.shape[1]
+    adapters, s, r = a.shape[0], (a.shape[1] if a.dim() == 4 else 1), a.shape[-2]
+    if a.dim() not in (3, 4) or a.shape[-1] != k or tuple(b.shape) != (adapters, n, r) or y.shape[0] != t:
+        raise ValueError(f"lora_add: y {tuple(y.shape)}, x {tuple(x.shape)}, a {tuple(a.shape)}, b {tuple(b.shape)} do not fit")
+    if scaling.shape != (adapters,) or adapter_ids.shape != (t,) or scaling.dtype != torch.float32 or adapter_ids.dtype != torch.int32:
+        raise ValueError("lora_add: scaling is f32 with one value per adapter, adapter_ids int32 with one per row")
+    dtype = x.dtype
+    if dtype not in (torch.float16, torch.bfloat16) or y.dtype != dtype or a.dtype != dtype or b.dtype != dtype:
+        raise ValueError(f"lora_add: y, x, a and b share one 16-bit dtype, got {y.dtype}, {x.dtype}, {a.dtype}, {b.dtype}")
+    if (len(sections) if sections is not None else 1) != s:
+        raise ValueError(f"lora_add: a holds {s} sections, sections are {sections}")
+    if out is None:
+        out = torch.empty_like(y)
+    elif out.shape != y.shape or out.dtype != dtype:
+        raise ValueError(f"lora_add: out {tuple(out.shape)} {out.dtype} does not fit y {tuple(y.shape)} {dtype}")
+    lib = L.load()
+    ws = workspace
+    if ws is None and t > 256:
+        ws = _scratch(lib.eq_lora_workspace_bytes(t, adapters), x.device)
+    L.check(
+        lib.eq_lora_add(
+            y.data_ptr(), x.data_ptr(), a.data_ptr(), b.data_ptr(), scaling.data_ptr(), adapter_ids.data_ptr(), t, k, n, r, adapters, s,
+            C.addressof(_section_array(sections, n)), _DTYPE[dtype], out.data_ptr(), ws.data_ptr() if ws is not None else None,
+            ws.numel() if ws is not None else 0, _stream(),
+        )
+    )
+    return out

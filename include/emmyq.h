@@ -308,6 +308,25 @@ int eq_moe_w4a16(const void* wq_gate_up, const void* wq_down, int scale_dtype, i
 /* Synchronizes the stream; EQ_ERR_BAD_ARG if the last call met an expert id outside [0, E) (such rows are dropped). */
 int eq_moe_status(const void* workspace, int64_t T, int64_t E, int64_t topk, int64_t H, int64_t I, void* stream);
 
+/* ------------------------------------------------------------------ low-rank adapters beside a shared projection */
+
+/* out[t] = y[t] + scaling[l] * B_l (A_l x[t]) with l = adapter_ids[t]: the adapters of many requests in one call, beside any of the
+ * linears above (y is the linear's output for the same rows of x).  A row whose id lies outside [0, L) (-1 by convention) has no
+ * adapter: out[t] = y[t].  Ids come in any order; rows of one adapter share its weights wherever they stand.  (The reference serves
+ * adapters through its host's graph, emmy/serving/lora.py.)
+ *   y, out [T, N], x [T, K], a [L, S, R, K], b [L, N, R], all act_dtype (EQ_F16 or EQ_BF16); scaling f32 [L]; adapter_ids int32 [T].
+ *   A projection that holds S linears side by side (q | k | v, gate | up) has one A per linear; section_widths (HOST int64 [S], may be
+ *   NULL where S is 1) are their columns: columns of linear s read A_l[s].
+ *   Adapters of a smaller rank than R are stored with zeros behind it (zero rows of A, zero columns of B).
+ * Products and sums in f32 (A x enters the second product as two 16-bit numbers that hold 16 to 22 bits of it); one rounding, of the
+ * result.  out may be y, and overlaps nothing else.  K, N, R and the widths are multiples of 8, S * R <= 1024, S <= 8, L <= 4096;
+ * y, x, a, b and out 16-byte aligned.  The workspace is needed above 256 rows only (256-byte aligned, written before it is read); nothing
+ * is kept between calls. */
+size_t eq_lora_workspace_bytes(int64_t T, int64_t L);
+int eq_lora_add(const void* y, const void* x, const void* a, const void* b, const float* scaling, const int32_t* adapter_ids, int64_t T, int64_t K, int64_t N,
+                int64_t R, int64_t L, int64_t S, const int64_t* section_widths, int act_dtype, void* out, void* workspace, size_t workspace_bytes,
+                void* stream);
+
 /* ------------------------------------------------------------------ expert-parallel MoE over peer memory */
 
 /* Experts sharded E_local per rank over `world` GPUs of one node.  The token exchange of the reference's expert
