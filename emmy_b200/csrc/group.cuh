@@ -1,0 +1,25 @@
+// Rows grouped by a key on the device: the blocks of rows of one adapter (lora.cu) or of one expert (moe_w8.cu).
+#pragma once
+#include "common.cuh"
+
+namespace eq {
+
+struct GroupBlock {
+    int32_t key;    // -1: rows whose id is no key
+    int32_t first;  // in the list of rows
+    int32_t count;  // 1 to block_rows
+};
+
+// Most blocks that T rows of `keys` keys can make (rows whose id is no key count as one more).
+inline int64_t group_max_blocks(int64_t T, int64_t keys, int64_t block_rows) {
+    const int64_t kinds = keys + 1 < T ? keys + 1 : T;  // every kind has at most one block that is not full
+    const int64_t most = kinds + T / block_rows;
+    return most < T ? most : T;
+}
+
+// rows[0, ..): the indices 0 .. T - 1 in order of their ids (those outside [0, keys) last, or left out unless keep_rest); blocks: each at
+// most block_rows rows of one key; n_blocks: how many.  The rows of a key stay in their order.  One launch, a programmatic dependent.
+constexpr int kGroupMaxKeys = 4096;
+int group_rows_launch(const int32_t* ids, int T, int keys, bool keep_rest, int block_rows, GroupBlock* blocks, int32_t* n_blocks, int32_t* rows, cudaStream_t stream);
+
+}  // namespace eq

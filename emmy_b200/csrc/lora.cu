@@ -5,7 +5,7 @@
 //
 // One launch up to 256 rows.  A unit is a block of at most 16 (64 above 256 rows) rows of one adapter; a cluster of CTAs works on it:
 //   rows     which rows share an adapter is worked out by every CTA from the ids alone (up to 256 of them: a row's rank among the rows of
-//            its adapter, the rows whose rank is a multiple of 16 open a block).  Above, lora_plan_kernel lists the blocks first.
+//            its adapter, the rows whose rank is a multiple of 16 open a block).  Above, group.cu lists the blocks first.
 //   shrink   h = A_l x by mma.sync m16n8k16 (rows as M, ranks as N), K cut over all warps of the cluster: every byte of x and A_l is
 //            read by one warp, straight into the fragment's registers (16 bytes a lane: a lane's eight K values are the K indices
 //            {2j, 2j+1, 2j+8, 2j+9} of two steps, in both operands alike).  The warps' sums meet in shared memory in warp order, the
@@ -15,9 +15,8 @@
 // h is kept in f32 and enters the second product as two 16-bit numbers, value and remainder (bf16: 16 bits of fraction, f16: 22, after
 // the row is brought to the top of f16's range by a power of two): the result is rounded once, as it is stored.
 // mma.sync and not tcgen05: a decode batch is bound by the bytes of A and B, a prompt by those of x and y.
-#include <type_traits>
-
-#include "common.cuh"
+#include "group.cuh"
+#include "mma_sync.cuh"
 
 namespace eq {
 
@@ -27,14 +26,8 @@ constexpr int kLoraSelfPlan = kLoraThreads;  // rows up to which a CTA works out
 constexpr int kLoraMaxSections = 8;
 constexpr int kLoraMaxRanks = 1024;          // S * R
 constexpr int kLoraWideRanks = 256;          // S * R up to which blocks have 64 rows above kLoraSelfPlan rows
-constexpr int kLoraMaxAdapters = 4096;
+constexpr int kLoraMaxAdapters = kGroupMaxKeys;
 constexpr int kLoraPass = 32;                // ranks of a shrink pass
-
-struct LoraBlock {
-    int32_t adapter;  // -1: rows without one, copied
-    int32_t first;    // in the list of rows
-    int32_t count;
-};
 
 struct LoraParams {
     const void* x;        // [T][K]
@@ -44,7 +37,7 @@ struct LoraParams {
     const float* scaling; // [L]
     const int32_t* ids;   // [T]
     void* out;            // [T][N], may be y
-    const LoraBlock* blocks;  // above kLoraSelfPlan rows
+    const GroupBlock* blocks;  // above kLoraSelfPlan rows
     const int32_t* n_blocks;
     const int32_t* rows;
     int T, K, N, R, S, L;
@@ -53,21 +46,6 @@ struct LoraParams {
     int ends[kLoraMaxSections];         // columns before the end of section s
     int group_ends[kLoraMaxSections];   // 32-column groups before the end of section s
 };
-
-template <typename T>
-__device__ __forceinline__ void lora_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void lora_mma<__half>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void lora_mma<__nv_bfloat16>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 
 __device__ __forceinline__ void lora_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void lora_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -92,14 +70,6 @@ __device__ __forceinline__ float lora_peer_load(const float* mine, uint32_t rank
 __device__ __forceinline__ int lora_adapter(const LoraParams& p, int t) {
     const int id = p.ids[t];
     return id >= 0 && id < p.L ? id : -1;
-}
-
-// Value and remainder of h in 16 bits.  A value that is not finite has no remainder.
-template <typename T>
-__device__ __forceinline__ void lora_split(float h, T& hi, T& lo) {
-    hi = from_float<T>(h);
-    const float back = to_float(hi);
-    lo = from_float<T>(fabsf(back) <= 3.0e38f ? h - back : 0.f);
 }
 
 template <typename T, int MT>
@@ -151,8 +121,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const __grid_cons
         count = __syncthreads_count(in);
     } else {
         if (unit >= *p.n_blocks) return;
-        const LoraBlock blk = p.blocks[unit];
-        adapter = blk.adapter;
+        const GroupBlock blk = p.blocks[unit];
+        adapter = blk.key;
         count = blk.count;
         if (tid < count) rows_s[tid] = p.rows[blk.first + tid];
         __syncthreads();
@@ -212,8 +182,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const __grid_cons
                 if (m < tiles_m) {
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
-                        lora_mma<T>(acc[m][n], xv[m][0].x, xv[m][1].x, xv[m][0].y, xv[m][1].y, wv[n].x, wv[n].y);
-                        lora_mma<T>(acc[m][n], xv[m][0].z, xv[m][1].z, xv[m][0].w, xv[m][1].w, wv[n].z, wv[n].w);
+                        mma_16816<T>(acc[m][n], xv[m][0].x, xv[m][1].x, xv[m][0].y, xv[m][1].y, wv[n].x, wv[n].y);
+                        mma_16816<T>(acc[m][n], xv[m][0].z, xv[m][1].z, xv[m][0].w, xv[m][1].w, wv[n].z, wv[n].w);
                     }
                 }
             }
@@ -271,7 +241,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const __grid_cons
 #pragma unroll
         for (int i = 0; i < kKeep; ++i) {
             const int n = lane + 32 * i;
-            if (n < ranks) lora_split<T>(h[i] * up, hi_s[r * p.h_stride + n], lo_s[r * p.h_stride + n]);
+            if (n < ranks) split16<T>(h[i] * up, hi_s[r * p.h_stride + n], lo_s[r * p.h_stride + n]);
         }
     }
     lora_cluster_arrive();  // this CTA is done with the others' shared memory
@@ -318,7 +288,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const __grid_cons
                             bottom = *reinterpret_cast<const uint2*>(at + 8 * p.h_stride);
                         }
 #pragma unroll
-                        for (int t = 0; t < 4; ++t) lora_mma<T>(acc[m][t], top.x, bottom.x, top.y, bottom.y, wv[t].x, wv[t].y);
+                        for (int t = 0; t < 4; ++t) mma_16816<T>(acc[m][t], top.x, bottom.x, top.y, bottom.y, wv[t].x, wv[t].y);
                     }
                 }
             }
@@ -345,73 +315,6 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const __grid_cons
         }
     }
     lora_cluster_wait();  // no CTA leaves while another may read its sums
-}
-
-// One CTA: rows in adapter order (those without an adapter last; left out where out is y) and the list of blocks of at most `block_rows`
-// rows.  The order of an adapter's rows is the order of the atomics; no row's result depends on it.
-__global__ void __launch_bounds__(1024) lora_plan_kernel(const __grid_constant__ LoraParams p, LoraBlock* __restrict__ blocks, int32_t* __restrict__ n_blocks,
-                                                         int32_t* __restrict__ rows, int block_rows) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    extern __shared__ int32_t counts[];  // [L + 1] rows, then cursors
-    __shared__ int32_t warp_rows[32], warp_blocks[32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kinds = p.L + 1;
-    for (int i = tid; i < kinds; i += 1024) counts[i] = 0;
-    __syncthreads();
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int tokens = (p.T + 31) & ~31;
-    for (int t = tid; t < tokens; t += 1024) {  // whole warps
-        int kind = -1;
-        if (t < p.T) kind = lora_adapter(p, t);
-        if (kind < 0) kind = t < p.T && !p.in_place ? p.L : -1;
-        const uint32_t same = __match_any_sync(0xFFFFFFFFu, kind);
-        if (kind >= 0 && __ffs(same) - 1 == lane) atomicAdd(counts + kind, __popc(same));
-    }
-    __syncthreads();
-    // exclusive scans over the kinds, `per` neighbouring ones a thread
-    const int per = (kinds + 1023) / 1024, from = min(tid * per, kinds), to = min(from + per, kinds);
-    int sum = 0, bsum = 0;
-    for (int i = from; i < to; ++i) sum += counts[i], bsum += (counts[i] + block_rows - 1) / block_rows;
-    int si = sum, bi = bsum;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const int su = __shfl_up_sync(0xFFFFFFFFu, si, d), bu = __shfl_up_sync(0xFFFFFFFFu, bi, d);
-        if (lane >= d) si += su, bi += bu;
-    }
-    if (lane == 31) warp_rows[warp] = si, warp_blocks[warp] = bi;
-    __syncthreads();
-    int at = si - sum, bat = bi - bsum;
-    for (int w = 0; w < warp; ++w) at += warp_rows[w], bat += warp_blocks[w];
-    for (int i = from; i < to; ++i) {
-        const int c = counts[i];
-        for (int r = 0; r < c; r += block_rows, ++bat) {
-            LoraBlock blk;
-            blk.adapter = i < p.L ? i : -1;
-            blk.first = at + r;
-            blk.count = min(block_rows, c - r);
-            blocks[bat] = blk;
-        }
-        counts[i] = at;
-        at += c;
-    }
-    if (tid == 1023) *n_blocks = bat;
-    __syncthreads();
-    for (int t = tid; t < tokens; t += 1024) {
-        int kind = -1;
-        if (t < p.T) kind = lora_adapter(p, t);
-        if (kind < 0) kind = t < p.T && !p.in_place ? p.L : -1;
-        const uint32_t same = __match_any_sync(0xFFFFFFFFu, kind);
-        const int leader = __ffs(same) - 1;
-        int base = 0;
-        if (kind >= 0 && leader == lane) base = atomicAdd(counts + kind, __popc(same));
-        base = __shfl_sync(0xFFFFFFFFu, base, leader);
-        if (kind >= 0) rows[base + __popc(same & ((1u << lane) - 1))] = t;
-    }
-}
-
-static int64_t lora_max_blocks(int64_t T, int64_t L, int64_t block_rows) {
-    const int64_t kinds = L + 1 < T ? L + 1 : T;  // every kind of rows has at most one block that is not full
-    const int64_t most = kinds + T / block_rows;
-    return most < T ? most : T;
 }
 
 template <typename T, int MT>
@@ -456,7 +359,7 @@ using namespace eq;
 
 extern "C" size_t eq_lora_workspace_bytes(int64_t T, int64_t L) {
     if (T <= kLoraSelfPlan || L <= 0) return 0;
-    return lora_align(256 + static_cast<size_t>(lora_max_blocks(T, L, 16)) * sizeof(LoraBlock)) + lora_align(static_cast<size_t>(T) * sizeof(int32_t));
+    return lora_align(256 + static_cast<size_t>(group_max_blocks(T, L, 16)) * sizeof(GroupBlock)) + lora_align(static_cast<size_t>(T) * sizeof(int32_t));
 }
 
 extern "C" int eq_lora_add(const void* y, const void* x, const void* a, const void* b, const float* scaling, const int32_t* adapter_ids, int64_t T, int64_t K,
@@ -508,29 +411,20 @@ extern "C" int eq_lora_add(const void* y, const void* x, const void* a, const vo
     p.in_place = out == y;
     p.h_stride = static_cast<int>(ceil_div(S * R, 64) * 64 + 16);  // rows 32 bytes apart modulo 128: a half-warp's 8-byte reads meet every bank once
     if (T <= kLoraSelfPlan) {
-        const int64_t units = lora_max_blocks(T, L, 16);
+        const int64_t units = group_max_blocks(T, L, 16);
         return act_dtype == EQ_F16 ? lora_launch<__half, 1>(p, units, stream) : lora_launch<__nv_bfloat16, 1>(p, units, stream);
     }
     const int block_rows = S * R <= kLoraWideRanks ? 64 : 16;
     unsigned char* base = static_cast<unsigned char*>(workspace);
     int32_t* n_blocks = reinterpret_cast<int32_t*>(base);
-    LoraBlock* blocks = reinterpret_cast<LoraBlock*>(base + 256);
-    int32_t* rows = reinterpret_cast<int32_t*>(base + lora_align(256 + static_cast<size_t>(lora_max_blocks(T, L, 16)) * sizeof(LoraBlock)));
+    GroupBlock* blocks = reinterpret_cast<GroupBlock*>(base + 256);
+    int32_t* rows = reinterpret_cast<int32_t*>(base + lora_align(256 + static_cast<size_t>(group_max_blocks(T, L, 16)) * sizeof(GroupBlock)));
     p.blocks = blocks;
     p.n_blocks = n_blocks;
     p.rows = rows;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(1);
-    cfg.blockDim = dim3(1024);
-    cfg.dynamicSmemBytes = (static_cast<size_t>(L) + 1) * sizeof(int32_t);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    EQ_CUDA_OK(cudaLaunchKernelEx(&cfg, lora_plan_kernel, p, blocks, n_blocks, rows, block_rows));
-    const int64_t units = lora_max_blocks(T, L, block_rows);
+    const int st = group_rows_launch(adapter_ids, p.T, p.L, !p.in_place, block_rows, blocks, n_blocks, rows, stream);
+    if (st != EQ_OK) return st;
+    const int64_t units = group_max_blocks(T, L, block_rows);
     if (block_rows == 16) return act_dtype == EQ_F16 ? lora_launch<__half, 1>(p, units, stream) : lora_launch<__nv_bfloat16, 1>(p, units, stream);
     return act_dtype == EQ_F16 ? lora_launch<__half, 4>(p, units, stream) : lora_launch<__nv_bfloat16, 4>(p, units, stream);
 }

@@ -1,4 +1,4 @@
-"""Mixture-of-experts operator calls on torch CUDA tensors (W4A16 experts)."""
+"""Mixture-of-experts operator calls on torch CUDA tensors (W4A16 experts; FP8 experts for a few tokens)."""
 
 from __future__ import annotations
 
@@ -110,3 +110,37 @@ def moe_forward(x, router_logits, w: MoEWeights, topk: int, workspace=None, out=
 
 def moe_status(workspace, t: int, w: MoEWeights, topk: int) -> None:
     L.check(L.load().eq_moe_status(_ptr(workspace), t, w.experts, topk, w.hidden, w.inter, _stream()))
+
+
+def moe_w8a16(x, router_logits, gate_up, gate_up_scale, down, down_scale, topk: int, workspace=None, out=None):
+    """One routed MoE layer of a few tokens on FP8 experts: y[T, H] from x[T, H] and f32 router logits [T, E].
+
+    gate_up e4m3 bits [E, 2I, H] (uint8; gate rows, then up rows), down [E, H, I]; scales f32, per output channel ([E, 2I] and [E, H]) or
+    per 128 x 128 block ([E, 2I / 128, H / 128] and [E, H / 128, I / 128])."""
+    _need_cuda(x, router_logits, gate_up, gate_up_scale, down, down_scale, workspace, out)
+    t, h = x.shape
+    e, n2, k = gate_up.shape
+    i = down.shape[2]
+    if k != h or n2 != 2 * i or tuple(down.shape) != (e, h, i) or tuple(router_logits.shape) != (t, e):
+        raise ValueError(f"moe_w8a16: x {tuple(x.shape)}, router_logits {tuple(router_logits.shape)}, gate_up {tuple(gate_up.shape)}, down {tuple(down.shape)} do not fit")
+    block = gate_up_scale.dim() == 3
+    want = ((e, n2 // 128, h // 128), (e, h // 128, i // 128)) if block else ((e, n2), (e, h))
+    if (tuple(gate_up_scale.shape), tuple(down_scale.shape)) != want:
+        raise ValueError(f"moe_w8a16: scales {tuple(gate_up_scale.shape)} and {tuple(down_scale.shape)} do not fit the weights")
+    if gate_up.dtype != torch.uint8 or down.dtype != torch.uint8 or any(v.dtype != torch.float32 for v in (router_logits, gate_up_scale, down_scale)):
+        raise ValueError("moe_w8a16: weights are e4m3 bits in uint8, scales and router logits f32")
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"moe_w8a16: activations are f16 or bf16, got {x.dtype}")
+    if out is None:
+        out = torch.empty_like(x)
+    elif out.shape != x.shape or out.dtype != x.dtype:
+        raise ValueError(f"moe_w8a16: out {tuple(out.shape)} {out.dtype} does not fit x {tuple(x.shape)} {x.dtype}")
+    lib = L.load()
+    ws = workspace if workspace is not None else _scratch(lib.eq_moe_w8a16_workspace_bytes(t, e, topk, h, i), x.device)
+    L.check(
+        lib.eq_moe_w8a16(
+            gate_up.data_ptr(), gate_up_scale.data_ptr(), down.data_ptr(), down_scale.data_ptr(), int(block), e, topk, h, i, x.data_ptr(),
+            router_logits.data_ptr(), t, _DTYPE[x.dtype], out.data_ptr(), ws.data_ptr(), ws.numel(), _stream(),
+        )
+    )
+    return out
