@@ -3,15 +3,18 @@
 // A projection that holds several linears side by side (q, k and v; gate and up) has one A per linear: section s of the columns reads
 // A_l[s], B_l is [N, R] over all of them.
 //
-// One launch up to 256 rows.  A unit is a block of at most 16 (64 above 256 rows) rows of one adapter; a cluster of CTAs works on it:
-//   rows     which rows share an adapter is worked out by every CTA from the ids alone (up to 256 of them: a row's rank among the rows of
-//            its adapter, the rows whose rank is a multiple of 16 open a block).  Above, group.cu lists the blocks first.
+// Up to 256 rows one launch, lora_rows_kernel.  A unit is a block of at most 16 rows of one adapter; a cluster of CTAs works on it:
+//   rows     which rows share an adapter is worked out by every CTA from the ids alone (a row's rank among the rows of its adapter; the rows
+//            whose rank is a multiple of 16 open a block).
 //   shrink   h = A_l x by mma.sync m16n8k16 (rows as M, ranks as N), K cut over all warps of the cluster: every byte of x and A_l is
 //            read by one warp, straight into the fragment's registers (16 bytes a lane: a lane's eight K values are the K indices
 //            {2j, 2j+1, 2j+8, 2j+9} of two steps, in both operands alike).  The warps' sums meet in shared memory in warp order, the
 //            CTAs' in distributed shared memory in rank order: no atomics, no workspace.
 //   expand   every CTA takes a share of the columns in groups of 32: rows as M, columns as N, R as K.  The columns of a group are dealt
-//            to the four MMA tiles so that a lane ends with eight neighbouring ones: y is read and written 16 bytes at a time.
+//            to the four MMA tiles so that a lane ends with eight neighbouring ones: y is read and written 16 bytes at a time.  The
+//            next group's B and y are on their way while a group is multiplied, the first one's before the CTAs have met.
+// Above, three: group.cu lists blocks of at most 64 rows, lora_shrink_kernel writes h, lora_expand_kernel adds B h to y in tiles of 64 rows x
+// 256 columns, B in shared memory by cp.async one tile ahead.
 // h is kept in f32 and enters the second product as two 16-bit numbers, value and remainder (bf16: 16 bits of fraction, f16: 22, after
 // the row is brought to the top of f16's range by a power of two): the result is rounded once, as it is stored.
 // mma.sync and not tcgen05: a decode batch is bound by the bytes of A and B, a prompt by those of x and y.
@@ -28,6 +31,8 @@ constexpr int kLoraMaxRanks = 1024;          // S * R
 constexpr int kLoraWideRanks = 256;          // S * R up to which blocks have 64 rows above kLoraSelfPlan rows
 constexpr int kLoraMaxAdapters = kGroupMaxKeys;
 constexpr int kLoraPass = 32;                // ranks of a shrink pass
+constexpr int kLoraTile = 256;               // columns of an expand tile
+constexpr int kLoraRun = 4;                  // neighbouring tiles that a CTA takes at a time
 
 struct LoraParams {
     const void* x;        // [T][K]
@@ -40,11 +45,15 @@ struct LoraParams {
     const GroupBlock* blocks;  // above kLoraSelfPlan rows
     const int32_t* n_blocks;
     const int32_t* rows;
+    void* hi;             // [T][S R] h of the rows in their order of `rows`, value and remainder
+    void* lo;
+    float* mul;           // [T] what the products of a row are multiplied by
     int T, K, N, R, S, L;
     int in_place;
-    int h_stride;                       // 16-bit elements of a row of h
+    int h_stride;                       // 16-bit elements of a row of h in shared memory
     int ends[kLoraMaxSections];         // columns before the end of section s
     int group_ends[kLoraMaxSections];   // 32-column groups before the end of section s
+    int tile_ends[kLoraMaxSections];    // 256-column tiles before the end of section s
 };
 
 __device__ __forceinline__ void lora_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -72,13 +81,147 @@ __device__ __forceinline__ int lora_adapter(const LoraParams& p, int t) {
     return id >= 0 && id < p.L ? id : -1;
 }
 
+// A_l x of the block's rows, this warp's slice of K, all warps' sums added: part[r][n] is this CTA's share.  Ends behind a barrier of the CTA.
 template <typename T, int MT>
-__global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const __grid_constant__ LoraParams p) {
+__device__ __forceinline__ void lora_shrink(const LoraParams& p, int adapter, int count, const int32_t* rows_s, float* part, float* red, int slice, int slices) {
     constexpr int kRows = 16 * MT;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int g = lane >> 2, j = lane & 3;
+    const int ranks = p.S * p.R;
+    const int tiles_m = (count + 15) >> 4;
+    const T* x = static_cast<const T*>(p.x);
+    const T* a = static_cast<const T*>(p.a) + static_cast<size_t>(adapter) * ranks * p.K;
+    const int chunks = (p.K + 31) / 32;
+    const int c0 = static_cast<int>(static_cast<int64_t>(chunks) * slice / slices), c1 = static_cast<int>(static_cast<int64_t>(chunks) * (slice + 1) / slices);
+    const T* xr[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = 16 * m + 8 * h + g;
+            xr[m][h] = r < count ? x + static_cast<size_t>(rows_s[r]) * p.K : nullptr;
+        }
+    for (int col = 0; col < ranks; col += kLoraPass) {
+        float acc[MT][4][4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
+#pragma unroll (MT == 1 ? 4 : 1)
+        for (int c = c0; c < c1; ++c) {
+            const int k = 32 * c + 8 * j;
+            const bool in = k < p.K;  // K is a multiple of 8
+            uint4 wv[4], xv[MT][2];
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+                wv[n] = in && col + 8 * n < ranks ? __ldg(reinterpret_cast<const uint4*>(a + static_cast<size_t>(col + 8 * n + g) * p.K + k)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    xv[m][h] = in && xr[m][h] ? __ldg(reinterpret_cast<const uint4*>(xr[m][h] + k)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                if (m < tiles_m) {
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        mma_16816<T>(acc[m][n], xv[m][0].x, xv[m][1].x, xv[m][0].y, xv[m][1].y, wv[n].x, wv[n].y);
+                        mma_16816<T>(acc[m][n], xv[m][0].z, xv[m][1].z, xv[m][0].w, xv[m][1].w, wv[n].z, wv[n].w);
+                    }
+                }
+            }
+        }
+        // [row][kLoraPass + 8]: rows a quarter of the banks apart
+        constexpr int kPitch = kLoraPass + 8;
+        float* mine = red + warp * kRows * kPitch;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+            if (m < tiles_m) {
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        *reinterpret_cast<float2*>(mine + (16 * m + 8 * h + g) * kPitch + 8 * n + 2 * j) = make_float2(acc[m][n][2 * h], acc[m][n][2 * h + 1]);
+            }
+        __syncthreads();
+        const int width = min(kLoraPass, ranks - col);
+        for (int i = tid; i < count * kLoraPass; i += kLoraThreads) {
+            const int r = i / kLoraPass, n = i % kLoraPass;
+            if (n >= width) continue;
+            float s = 0.f;
+#pragma unroll
+            for (int w = 0; w < kLoraWarps; ++w) s += red[(w * kRows + r) * kPitch + n];
+            part[r * ranks + col + n] = s;
+        }
+        __syncthreads();
+    }
+}
+
+// Row r of h over the cluster's shares, scaled, by one warp: put(n, value, remainder) for every rank; the row's factor is returned.
+template <typename T, int RANKS, typename Put>
+__device__ __forceinline__ float lora_join(const float* part, int r, int ranks, uint32_t ctas, float scaling, Put&& put) {
+    const int lane = threadIdx.x & 31;
+    float h[RANKS / 32];
+    float big = 0.f;
+#pragma unroll
+    for (int i = 0; i < RANKS / 32; ++i) {
+        const int n = lane + 32 * i;
+        h[i] = 0.f;
+        if (32 * i < ranks) {  // the whole warp
+            const float* at = part + r * ranks + min(n, ranks - 1);
+            float v[8];
+#pragma unroll
+            for (uint32_t c = 0; c < 8; ++c) v[c] = c < ctas ? lora_peer_load(at, c) : 0.f;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) h[i] += v[c];
+            h[i] = n < ranks ? h[i] * scaling : 0.f;
+            big = fmaxf(big, fabsf(h[i]));
+        }
+    }
+    float up = 1.f, down = 1.f;  // powers of two that bring the row's largest value to [2^13, 2^14) in f16, and back
+    if (std::is_same<T, __half>::value) {
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, off));
+        if (big > 0.f && big < INFINITY) {
+            const int e = min(13 + 127 - static_cast<int>(__float_as_uint(big) >> 23), 120);
+            up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+            down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RANKS / 32; ++i) {
+        const int n = lane + 32 * i;
+        if (n < ranks) {
+            T hi, lo;
+            split16<T>(h[i] * up, hi, lo);
+            put(n, hi, lo);
+        }
+    }
+    return down;
+}
+
+// y + delta of eight neighbouring columns of a row: acc's columns as the four tiles of a group hold them (first of the lane's two rows, or second).
+template <typename T>
+__device__ __forceinline__ uint4 lora_add8(uint4 v, const float (&acc)[4][4], int second, float mul) {
+    T* e = reinterpret_cast<T*>(&v);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) e[2 * t + i] = from_float<T>(fmaf(second ? acc[t][2 + i] : acc[t][i], mul, to_float(e[2 * t + i])));
+    return v;
+}
+
+// ------------------------------------------------------------------------------------------------ up to 256 rows (or more than 256 ranks): blocks of 16 rows
+template <typename T>
+__global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid_constant__ LoraParams p) {
+    constexpr int kRows = 16;
+    constexpr int kChunks = 2;  // of 32 ranks: what a lane asks for at a time
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    extern __shared__ __align__(16) unsigned char smem[];
+    extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int32_t rows_s[kRows];
-    __shared__ __align__(16) int32_t ids_s[MT == 1 ? kLoraSelfPlan : 4];
+    __shared__ __align__(16) int32_t ids_s[kLoraSelfPlan];
     __shared__ int32_t lead_s[kLoraWarps];
     __shared__ int32_t block_s[3];
     __shared__ float mul_s[kRows];
@@ -91,7 +234,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const __grid_cons
     asm volatile("griddepcontrol.wait;" ::: "memory");  // everything read below may come from the kernel before
     // ---- the unit's adapter and rows (the same for all CTAs of the cluster)
     int adapter = -1, count = 0;
-    if (MT == 1 && !p.blocks) {
+    if (!p.blocks) {
         int mine = -2, rank = 0;
         if (tid < p.T) mine = lora_adapter(p, tid);
         ids_s[tid] = mine;
@@ -139,203 +282,340 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const __grid_cons
         }
         return;
     }
-    const int tiles_m = (count + 15) >> 4;
+    const float scaling = __ldg(p.scaling + adapter);
+    float* part = reinterpret_cast<float*>(smem);  // [kRows][ranks]: this CTA's share of K
+    float* red = part + kRows * ranks;             // [warps][kRows][kLoraPass + 8]; the split h lies here afterwards
+    lora_shrink<T, 1>(p, adapter, count, rows_s, part, red, cta * kLoraWarps + warp, ctas * kLoraWarps);
+    lora_cluster_arrive();
 
-    // ---- shrink
-    float* part = reinterpret_cast<float*>(smem);            // [kRows][ranks]: this CTA's share of K
-    float* red = part + kRows * ranks;                       // [warps][kRows][kLoraPass]; the split h lies here afterwards
-    const T* x = static_cast<const T*>(p.x);
-    const T* a = static_cast<const T*>(p.a) + static_cast<size_t>(adapter) * ranks * p.K;
-    const int chunks = (p.K + 31) / 32, slices = ctas * kLoraWarps, slice = cta * kLoraWarps + warp;
-    const int c0 = static_cast<int>(static_cast<int64_t>(chunks) * slice / slices), c1 = static_cast<int>(static_cast<int64_t>(chunks) * (slice + 1) / slices);
-    const T* xr[MT][2];
+    // ---- expand: this warp's groups of 32 columns, each in steps of 64 ranks; a step's B and its group's y are asked for one step ahead
+    const T* b = static_cast<const T*>(p.b) + static_cast<size_t>(adapter) * p.N * p.R;
+    const int groups = p.group_ends[p.S - 1];
+    const int g0 = static_cast<int>(static_cast<int64_t>(groups) * cta / ctas), g1 = static_cast<int>(static_cast<int64_t>(groups) * (cta + 1) / ctas);
+    const bool has0 = g < count, has1 = g + 8 < count;
+    const size_t y0 = static_cast<size_t>(rows_s[has0 ? g : 0]) * p.N, y1 = static_cast<size_t>(rows_s[has1 ? g + 8 : 0]) * p.N;
+    struct Group {
+        int section, first, end;  // columns
+    };
+    auto group = [&](int gi) {
+        Group v;
+        v.section = 0;
+        while (gi >= p.group_ends[v.section]) ++v.section;
+        const int s = v.section;
+        v.first = (s ? p.ends[s - 1] : 0) + 32 * (gi - (s ? p.group_ends[s - 1] : 0));
+        v.end = p.ends[s];
+        return v;
+    };
+    uint4 next_w[4][kChunks], next_y[2];
+    auto ask_w = [&](const Group& v, int k0) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+        for (int t = 0; t < 4; ++t) {
+            const int n = v.first + 8 * (g >> 1) + 2 * t + (g & 1);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = 16 * m + 8 * h + g;
-            xr[m][h] = r < count ? x + static_cast<size_t>(rows_s[r]) * p.K : nullptr;
-        }
-    for (int col = 0; col < ranks; col += kLoraPass) {
-        float acc[MT][4][4];
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int n = 0; n < 4; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
-#pragma unroll (MT == 1 ? 2 : 1)
-        for (int c = c0; c < c1; ++c) {
-            const int k = 32 * c + 8 * j;
-            const bool in = k < p.K;  // K is a multiple of 8
-            uint4 wv[4], xv[MT][2];
-#pragma unroll
-            for (int n = 0; n < 4; ++n)
-                wv[n] = in && col + 8 * n < ranks ? __ldg(reinterpret_cast<const uint4*>(a + static_cast<size_t>(col + 8 * n + g) * p.K + k)) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    xv[m][h] = in && xr[m][h] ? __ldg(reinterpret_cast<const uint4*>(xr[m][h] + k)) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                if (m < tiles_m) {
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        mma_16816<T>(acc[m][n], xv[m][0].x, xv[m][1].x, xv[m][0].y, xv[m][1].y, wv[n].x, wv[n].y);
-                        mma_16816<T>(acc[m][n], xv[m][0].z, xv[m][1].z, xv[m][0].w, xv[m][1].w, wv[n].z, wv[n].w);
-                    }
-                }
+            for (int c = 0; c < kChunks; ++c) {
+                const int k = k0 + 32 * c + 8 * j;
+                next_w[t][c] = n < v.end && k < p.R ? ld_stream_v4(b + static_cast<size_t>(n) * p.R + k) : make_uint4(0, 0, 0, 0);
             }
         }
-        float* mine = red + warp * kRows * kLoraPass;
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int n = 0; n < 4; ++n)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    *reinterpret_cast<float2*>(mine + (16 * m + 8 * h + g) * kLoraPass + 8 * n + 2 * j) = make_float2(acc[m][n][2 * h], acc[m][n][2 * h + 1]);
-        __syncthreads();
-        const int width = min(kLoraPass, ranks - col);
-        for (int i = tid; i < kRows * kLoraPass; i += kLoraThreads) {
-            const int r = i / kLoraPass, n = i % kLoraPass;
-            if (n >= width) continue;
-            float s = 0.f;
-#pragma unroll
-            for (int w = 0; w < kLoraWarps; ++w) s += red[w * kRows * kLoraPass + i];
-            part[r * ranks + col + n] = s;
-        }
-        __syncthreads();
+    };
+    auto ask_y = [&](const Group& v) {
+        const int n = v.first + 8 * j;
+        next_y[0] = has0 && n < v.end ? *reinterpret_cast<const uint4*>(yin + y0 + n) : make_uint4(0, 0, 0, 0);
+        next_y[1] = has1 && n < v.end ? *reinterpret_cast<const uint4*>(yin + y1 + n) : make_uint4(0, 0, 0, 0);
+    };
+    int gi = g0 + warp;
+    Group now = {}, ahead = {};
+    if (gi < g1) {
+        ahead = group(gi);
+        ask_w(ahead, 0);
+        ask_y(ahead);
     }
-    lora_cluster_arrive();
-    lora_cluster_wait();
 
     // ---- h of the whole K, scaled and split; a warp takes a row
+    lora_cluster_wait();
     T* hi_s = reinterpret_cast<T*>(red);
     T* lo_s = hi_s + kRows * p.h_stride;
-    const float scaling = p.scaling[adapter];
-    constexpr int kKeep = (MT == 1 ? kLoraMaxRanks : kLoraWideRanks) / 32;
-    for (int r = warp; r < kRows; r += kLoraWarps) {
-        float h[kKeep];
-        float big = 0.f;
-#pragma unroll
-        for (int i = 0; i < kKeep; ++i) {
-            const int n = lane + 32 * i;
-            h[i] = 0.f;
-            if (n < ranks) {
-                for (uint32_t c = 0; c < ctas; ++c) h[i] += lora_peer_load(part + r * ranks + n, c);
-                h[i] *= scaling;
-                big = fmaxf(big, fabsf(h[i]));
-            }
-        }
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, off));
-        float up = 1.f, down = 1.f;  // powers of two that bring the row's largest value to [2^13, 2^14) in f16, and back
-        if (std::is_same<T, __half>::value && big > 0.f && big < INFINITY) {
-            const int e = min(13 - ilogbf(big), 120);
-            up = ldexpf(1.f, e);
-            down = ldexpf(1.f, -e);
-        }
-        if (lane == 0) mul_s[r] = down;
-#pragma unroll
-        for (int i = 0; i < kKeep; ++i) {
-            const int n = lane + 32 * i;
-            if (n < ranks) split16<T>(h[i] * up, hi_s[r * p.h_stride + n], lo_s[r * p.h_stride + n]);
-        }
+    for (int r = warp; r < count; r += kLoraWarps) {
+        auto put = [&](int n, T hi, T lo) {
+            hi_s[r * p.h_stride + n] = hi;
+            lo_s[r * p.h_stride + n] = lo;
+        };
+        float mul;
+        if (ranks <= 128) mul = lora_join<T, 128>(part, r, ranks, ctas, scaling, put);
+        else mul = lora_join<T, kLoraMaxRanks>(part, r, ranks, ctas, scaling, put);
+        if (lane == 0) mul_s[r] = mul;
     }
     lora_cluster_arrive();  // this CTA is done with the others' shared memory
     __syncthreads();
 
-    // ---- expand
-    const T* b = static_cast<const T*>(p.b) + static_cast<size_t>(adapter) * p.N * p.R;
-    const int groups = p.group_ends[p.S - 1];
-    const int g0 = static_cast<int>(static_cast<int64_t>(groups) * cta / ctas), g1 = static_cast<int>(static_cast<int64_t>(groups) * (cta + 1) / ctas);
-    for (int gi = g0 + warp; gi < g1; gi += kLoraWarps) {
-        int s = 0;
-        while (gi >= p.group_ends[s]) ++s;
-        const int n0 = (s ? p.ends[s - 1] : 0) + 32 * (gi - (s ? p.group_ends[s - 1] : 0)), n_end = p.ends[s];
-        const T* wrow[4];
+    const float mul0 = mul_s[has0 ? g : 0], mul1 = mul_s[has1 ? g + 8 : 0];
+    const int lo_at = kRows * p.h_stride;
+    for (; gi < g1; gi += kLoraWarps) {
+        now = ahead;
+        float acc[4][4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int n = n0 + 8 * (g >> 1) + 2 * t + (g & 1);
-            wrow[t] = n < n_end ? b + static_cast<size_t>(n) * p.R + 4 * j : nullptr;
-        }
-        float acc[MT][4][4];
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+            for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
+        uint4 yv[2];
+        const T* h_row = hi_s + g * p.h_stride + now.section * p.R + 8 * j;
+        for (int k0 = 0; k0 < p.R; k0 += 32 * kChunks) {
+            uint4 wv[4][kChunks];
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[m][t][e] = 0.f;
-        const T* h_row = hi_s + g * p.h_stride + s * p.R + 4 * j;
-        const size_t lo_at = static_cast<size_t>(kRows) * p.h_stride;
-#pragma unroll (MT == 1 ? 2 : 1)
-        for (int k = 0; k < p.R; k += 16) {
-            const bool in = k + 4 * j < p.R;  // R is a multiple of 8
-            uint2 wv[4];
+                for (int c = 0; c < kChunks; ++c) wv[t][c] = next_w[t][c];
+            if (k0 == 0) {
+                yv[0] = next_y[0];
+                yv[1] = next_y[1];
+            }
+            if (k0 + 32 * kChunks < p.R) {
+                ask_w(now, k0 + 32 * kChunks);
+            } else if (gi + kLoraWarps < g1) {
+                ahead = group(gi + kLoraWarps);
+                ask_w(ahead, 0);
+                ask_y(ahead);
+            }
 #pragma unroll
-            for (int t = 0; t < 4; ++t) wv[t] = in && wrow[t] ? __ldg(reinterpret_cast<const uint2*>(wrow[t] + k)) : make_uint2(0, 0);
+            for (int c = 0; c < kChunks; ++c) {
+                const int k = k0 + 32 * c;
+                if (k >= p.R) break;
+                const bool in = k + 8 * j < p.R;  // R is a multiple of 8
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                if (m < tiles_m) {
+                for (int half = 0; half < 2; ++half) {
+                    uint4 top = make_uint4(0, 0, 0, 0), bottom = make_uint4(0, 0, 0, 0);
+                    if (in && has0) top = *reinterpret_cast<const uint4*>(h_row + k + half * lo_at);
+                    if (in && has1) bottom = *reinterpret_cast<const uint4*>(h_row + k + half * lo_at + 8 * p.h_stride);
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const T* at = h_row + 16 * m * p.h_stride + k + half * lo_at;
-                        uint2 top = make_uint2(0, 0), bottom = make_uint2(0, 0);
-                        if (in) {
-                            top = *reinterpret_cast<const uint2*>(at);
-                            bottom = *reinterpret_cast<const uint2*>(at + 8 * p.h_stride);
-                        }
-#pragma unroll
-                        for (int t = 0; t < 4; ++t) mma_16816<T>(acc[m][t], top.x, bottom.x, top.y, bottom.y, wv[t].x, wv[t].y);
+                    for (int t = 0; t < 4; ++t) {
+                        mma_16816<T>(acc[t], top.x, bottom.x, top.y, bottom.y, wv[t][c].x, wv[t][c].y);
+                        mma_16816<T>(acc[t], top.z, bottom.z, top.w, bottom.w, wv[t][c].z, wv[t][c].w);
                     }
                 }
             }
         }
-        const int n = n0 + 8 * j;
-        if (n < n_end) {
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int r = 16 * m + 8 * h + g;
-                    if (r < count) {
-                        const size_t at = static_cast<size_t>(rows_s[r]) * p.N + n;
-                        const float mul = mul_s[r];
-                        uint4 v = *reinterpret_cast<const uint4*>(yin + at);
-                        T* e = reinterpret_cast<T*>(&v);
-#pragma unroll
-                        for (int t = 0; t < 4; ++t)
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) e[2 * t + i] = from_float<T>(fmaf(acc[m][t][2 * h + i], mul, to_float(e[2 * t + i])));
-                        *reinterpret_cast<uint4*>(out + at) = v;
-                    }
-                }
+        const int n = now.first + 8 * j;
+        if (n < now.end) {
+            if (has0) *reinterpret_cast<uint4*>(out + y0 + n) = lora_add8<T>(yv[0], acc, 0, mul0);
+            if (has1) *reinterpret_cast<uint4*>(out + y1 + n) = lora_add8<T>(yv[1], acc, 1, mul1);
         }
     }
     lora_cluster_wait();  // no CTA leaves while another may read its sums
 }
 
-template <typename T, int MT>
-static int lora_launch(const LoraParams& p, int64_t units, cudaStream_t stream) {
-    auto kernel = lora_kernel<T, MT>;
-    constexpr int kRows = 16 * MT;
+// ------------------------------------------------------------------------------------------------ more rows: blocks of 64, h through memory
+template <typename T>
+__global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ int32_t rows_s[64];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ranks = p.S * p.R;
-    const size_t red = static_cast<size_t>(kLoraWarps) * kRows * kLoraPass * sizeof(float);
-    const size_t split = 2 * static_cast<size_t>(kRows) * p.h_stride * 2;
-    const size_t smem = static_cast<size_t>(kRows) * ranks * sizeof(float) + (red > split ? red : split);
-    static bool configured[64] = {};
-    int dev = 0;
-    EQ_CUDA_OK(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 64 || !configured[dev]) {
-        EQ_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024));
-        if (dev >= 0 && dev < 64) configured[dev] = true;
+    const uint32_t cta = lora_cluster_rank(), ctas = lora_cluster_size();
+    const int unit = blockIdx.x / ctas;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (unit >= *p.n_blocks) return;
+    const GroupBlock blk = p.blocks[unit];
+    if (blk.key < 0) return;
+    if (tid < blk.count) rows_s[tid] = p.rows[blk.first + tid];
+    __syncthreads();
+    const float scaling = __ldg(p.scaling + blk.key);
+    float* part = reinterpret_cast<float*>(smem);  // [64][ranks]
+    lora_shrink<T, 4>(p, blk.key, blk.count, rows_s, part, part + 64 * ranks, cta * kLoraWarps + warp, ctas * kLoraWarps);
+    lora_cluster_arrive();
+    lora_cluster_wait();
+    for (int r = cta * kLoraWarps + warp; r < blk.count; r += ctas * kLoraWarps) {
+        T* hi = static_cast<T*>(p.hi) + static_cast<size_t>(blk.first + r) * ranks;
+        T* lo = static_cast<T*>(p.lo) + static_cast<size_t>(blk.first + r) * ranks;
+        const float mul = lora_join<T, kLoraWideRanks>(part, r, ranks, ctas, scaling, [&](int n, T vh, T vl) {
+            hi[n] = vh;
+            lo[n] = vl;
+        });
+        if (lane == 0) p.mul[blk.first + r] = mul;
     }
+    lora_cluster_arrive();
+    lora_cluster_wait();
+}
+
+__device__ __forceinline__ void lora_copy16(uint32_t to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+
+// 16-byte chunk q (0 to 7) of column n's 64 ranks in a stage.  A warp's 16-byte reads go to columns 2t and 2t + 1 at once: their chunks lie in
+// different halves of the banks.
+__device__ __forceinline__ uint32_t lora_stage_at(int n, int q) { return static_cast<uint32_t>(n * 128 + ((q ^ (((n & 1) << 2) | ((n >> 1) & 3))) << 4)); }
+
+// Tiles of 64 rows x 256 columns: warps 2 x 4, a warp 32 x 64.  Steps are 64 ranks of a tile's B (32 KB), two stages.  A CTA takes runs of
+// neighbouring tiles; the runs are dealt over the CTAs, so that blocks of few rows and of many mix.
+template <typename T>
+__global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(const __grid_constant__ LoraParams p) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ int32_t rows_s[64];
+    __shared__ float mul_s[64];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int g = lane >> 2, j = lane & 3;
+    const int wr = warp >> 2, wc = warp & 3;
+    const int ranks = p.S * p.R, steps = (p.R + 63) / 64;
+    T* hi_s = reinterpret_cast<T*>(smem + 2 * kLoraTile * 128);  // [64][h_stride], the section's h
+    T* lo_s = hi_s + 64 * p.h_stride;
+    const uint32_t stage0 = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int n_blocks = *p.n_blocks, tiles = p.tile_ends[p.S - 1];
+    const int64_t units = static_cast<int64_t>(n_blocks) * tiles;
+    const T* yin = static_cast<const T*>(p.y);
+    T* out = static_cast<T*>(p.out);
+
+    // this CTA's units in order: run i is units [(blockIdx.x + i gridDim.x) kLoraRun, + kLoraRun)
+    auto after = [&](int64_t u) {
+        ++u;
+        return u % kLoraRun ? u : u + static_cast<int64_t>(gridDim.x - 1) * kLoraRun;
+    };
+    struct Tile {
+        int block, section, first, end;
+    };
+    auto tile = [&](int64_t u) {
+        Tile v;
+        v.block = static_cast<int>(u / tiles);
+        const int t = static_cast<int>(u - static_cast<int64_t>(v.block) * tiles);
+        v.section = 0;
+        while (t >= p.tile_ends[v.section]) ++v.section;
+        const int s = v.section;
+        v.first = (s ? p.ends[s - 1] : 0) + kLoraTile * (t - (s ? p.tile_ends[s - 1] : 0));
+        v.end = p.ends[s];
+        return v;
+    };
+    // 64 ranks of a tile's columns to a stage
+    auto ask = [&](const Tile& v, int step, int stage) {
+        const int key = p.blocks[v.block].key;
+        if (key >= 0) {
+            const T* b = static_cast<const T*>(p.b) + (static_cast<size_t>(key) * p.N + v.first) * p.R + 64 * step;
+            const int cols = min(kLoraTile, v.end - v.first), chunks = min(8, p.R / 8 - 8 * step);
+#pragma unroll
+            for (int i = 0; i < kLoraTile * 8 / kLoraThreads; ++i) {
+                const int n = (tid + i * kLoraThreads) >> 3, q = tid & 7;
+                if (n < cols && q < chunks) lora_copy16(stage0 + stage * (kLoraTile * 128) + lora_stage_at(n, q), b + static_cast<size_t>(n) * p.R + 8 * q);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
+    int64_t u = static_cast<int64_t>(blockIdx.x) * kLoraRun;
+    int stage = 0, held_block = -1, held_section = -1;
+    if (u < units) ask(tile(u), 0, 0);
+    for (; u < units;) {
+        const Tile now = tile(u);
+        const int64_t u_next = after(u);
+        const GroupBlock blk = p.blocks[now.block];
+        if (held_block != now.block || held_section != now.section) {
+            __syncthreads();  // everyone is done with the rows and the h held so far
+            if (tid < blk.count) rows_s[tid] = p.rows[blk.first + tid];
+            if (blk.key >= 0) {
+                if (tid < blk.count) mul_s[tid] = p.mul[blk.first + tid];
+                const int vecs = p.R / 8;
+                for (int i = tid; i < blk.count * vecs; i += kLoraThreads) {
+                    const int r = i / vecs, v = i - r * vecs;
+                    const size_t from = static_cast<size_t>(blk.first + r) * ranks + now.section * p.R + 8 * v;
+                    *reinterpret_cast<uint4*>(hi_s + r * p.h_stride + 8 * v) = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.hi) + from));
+                    *reinterpret_cast<uint4*>(lo_s + r * p.h_stride + 8 * v) = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.lo) + from));
+                }
+            }
+            __syncthreads();
+            held_block = now.block;
+            held_section = now.section;
+        }
+        const bool active = 32 * wr < blk.count;
+        float acc[2][2][4][4];  // [16 rows][32 columns][tile][..]
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[m][q][t][e] = 0.f;
+        for (int step = 0; step < steps; ++step) {
+            // the next step's B, into the stage that was read last: everyone is past the barrier behind that
+            if (step + 1 < steps) ask(now, step + 1, stage ^ 1);
+            else if (u_next < units) ask(tile(u_next), 0, stage ^ 1);
+            else asm volatile("cp.async.commit_group;" ::: "memory");
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            __syncthreads();
+            if (active && blk.key >= 0) {
+                const unsigned char* base = smem + stage * (kLoraTile * 128);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int k = 64 * step + 32 * c;
+                    if (k >= p.R) break;
+                    const bool in = k + 8 * j < p.R;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        uint4 top[2], bottom[2];
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) {
+                            const T* at = (half ? lo_s : hi_s) + (32 * wr + 16 * m + g) * p.h_stride + k + 8 * j;
+                            top[m] = in ? *reinterpret_cast<const uint4*>(at) : make_uint4(0, 0, 0, 0);
+                            bottom[m] = in ? *reinterpret_cast<const uint4*>(at + 8 * p.h_stride) : make_uint4(0, 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int q = 0; q < 2; ++q)
+#pragma unroll
+                            for (int t = 0; t < 4; ++t) {
+                                const int n = 64 * wc + 32 * q + 8 * (g >> 1) + 2 * t + (g & 1);
+                                const uint4 w = in ? *reinterpret_cast<const uint4*>(base + lora_stage_at(n, 4 * c + j)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                                for (int m = 0; m < 2; ++m) {
+                                    mma_16816<T>(acc[m][q][t], top[m].x, bottom[m].x, top[m].y, bottom[m].y, w.x, w.y);
+                                    mma_16816<T>(acc[m][q][t], top[m].z, bottom[m].z, top[m].w, bottom[m].w, w.z, w.w);
+                                }
+                            }
+                    }
+                }
+            }
+            __syncthreads();
+            stage ^= 1;
+        }
+        if (active) {
+            uint4 yv[2][2][2];
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const int r = 32 * wr + 16 * m + 8 * h + g, n = now.first + 64 * wc + 32 * q + 8 * j;
+                        if (r < blk.count && n < now.end) yv[m][h][q] = *reinterpret_cast<const uint4*>(yin + static_cast<size_t>(rows_s[r]) * p.N + n);
+                    }
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const int r = 32 * wr + 16 * m + 8 * h + g, n = now.first + 64 * wc + 32 * q + 8 * j;
+                        if (r < blk.count && n < now.end)
+                            *reinterpret_cast<uint4*>(out + static_cast<size_t>(rows_s[r]) * p.N + n) =
+                                blk.key >= 0 ? lora_add8<T>(yv[m][h][q], acc[m][q], h, mul_s[r]) : yv[m][h][q];
+                    }
+        }
+        u = u_next;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+static size_t lora_align(size_t v) { return (v + 255) / 256 * 256; }
+
+// CTAs of a cluster: the largest of 8, 4, 2, 1 whose grid stays within `waves` rounds of two CTAs an SM.
+static int lora_cluster(int64_t units, int waves) {
     int ctas = 8;
-    while (ctas > 1 && units * ctas > 2 * sm_count()) ctas /= 2;
+    while (ctas > 1 && units * ctas > 2 * waves * sm_count()) ctas /= 2;
+    return ctas;
+}
+
+static int lora_launch(void (*kernel)(const LoraParams), const LoraParams& p, int64_t grid, int cluster, size_t smem, cudaStream_t stream) {
+    EQ_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(units * ctas));
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
     cfg.blockDim = dim3(kLoraThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -343,7 +623,7 @@ static int lora_launch(const LoraParams& p, int64_t units, cudaStream_t stream) 
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = ctas;
+    attr[1].val.clusterDim.x = cluster;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
@@ -351,15 +631,62 @@ static int lora_launch(const LoraParams& p, int64_t units, cudaStream_t stream) 
     return EQ_OK;
 }
 
-static size_t lora_align(size_t v) { return (v + 255) / 256 * 256; }
+// Shared memory of a shrink over blocks of `rows` rows, with room for the split h behind the sums where it is kept there.
+static size_t lora_smem(int rows, int ranks, int h_stride, bool keep) {
+    const size_t red = static_cast<size_t>(kLoraWarps) * rows * (kLoraPass + 8) * sizeof(float), split = keep ? 2 * static_cast<size_t>(rows) * h_stride * 2 : 0;
+    return static_cast<size_t>(rows) * ranks * sizeof(float) + (red > split ? red : split);
+}
+
+template <typename T>
+static int lora_forward(LoraParams p, int64_t T_, int64_t L, unsigned char* base, cudaStream_t stream) {
+    const int ranks = p.S * p.R;
+    // 16-bit elements of a row of h: rows 64 bytes apart modulo 128, so that the 16-byte reads of two rows meet every bank once
+    auto stride = [](int n) { return (n + 63) / 64 * 64 + 32; };
+    const int block_rows = p.T > kLoraSelfPlan && ranks <= kLoraWideRanks ? 64 : 16;
+    const int64_t units = group_max_blocks(T_, L, block_rows);
+    if (p.T > kLoraSelfPlan) {
+        size_t o = 0;
+        auto take = [&](size_t bytes) {
+            void* at = base + o;
+            o += lora_align(bytes);
+            return at;
+        };
+        int32_t* n_blocks = static_cast<int32_t*>(take(4));
+        GroupBlock* blocks = static_cast<GroupBlock*>(take(static_cast<size_t>(units) * sizeof(GroupBlock)));
+        int32_t* rows = static_cast<int32_t*>(take(static_cast<size_t>(T_) * 4));
+        p.blocks = blocks;
+        p.n_blocks = n_blocks;
+        p.rows = rows;
+        const int st = group_rows_launch(p.ids, p.T, p.L, !p.in_place, block_rows, blocks, n_blocks, rows, stream);
+        if (st != EQ_OK) return st;
+        if (block_rows == 64) {
+            p.mul = static_cast<float*>(take(static_cast<size_t>(T_) * 4));
+            p.hi = take(static_cast<size_t>(T_) * ranks * 2);
+            p.lo = take(static_cast<size_t>(T_) * ranks * 2);
+        }
+    }
+    if (block_rows == 16) {
+        p.h_stride = stride(ranks);
+        const int ctas = lora_cluster(units, 2);
+        return lora_launch(lora_rows_kernel<T>, p, units * ctas, ctas, lora_smem(16, ranks, p.h_stride, true), stream);
+    }
+    const int ctas = lora_cluster(units, 1);
+    const int st = lora_launch(lora_shrink_kernel<T>, p, units * ctas, ctas, lora_smem(64, ranks, 0, false), stream);
+    if (st != EQ_OK) return st;
+    p.h_stride = stride(p.R);
+    const int64_t runs = ceil_div(units * p.tile_ends[p.S - 1], kLoraRun), most = 2 * sm_count();
+    return lora_launch(lora_expand_kernel<T>, p, runs < most ? runs : most, 1, 2 * kLoraTile * 128 + 2 * static_cast<size_t>(64) * p.h_stride * 2, stream);
+}
 
 }  // namespace eq
 
 using namespace eq;
 
-extern "C" size_t eq_lora_workspace_bytes(int64_t T, int64_t L) {
-    if (T <= kLoraSelfPlan || L <= 0) return 0;
-    return lora_align(256 + static_cast<size_t>(group_max_blocks(T, L, 16)) * sizeof(GroupBlock)) + lora_align(static_cast<size_t>(T) * sizeof(int32_t));
+extern "C" size_t eq_lora_workspace_bytes(int64_t T, int64_t L, int64_t S, int64_t R) {
+    if (T <= kLoraSelfPlan || L <= 0 || S <= 0 || R <= 0) return 0;
+    const size_t lists = 256 + lora_align(static_cast<size_t>(group_max_blocks(T, L, 16)) * sizeof(GroupBlock)) + lora_align(static_cast<size_t>(T) * 4);
+    if (S > kLoraWideRanks || R > kLoraWideRanks || S * R > kLoraWideRanks) return lists;
+    return lists + lora_align(static_cast<size_t>(T) * 4) + 2 * lora_align(static_cast<size_t>(T) * S * R * 2);
 }
 
 extern "C" int eq_lora_add(const void* y, const void* x, const void* a, const void* b, const float* scaling, const int32_t* adapter_ids, int64_t T, int64_t K,
@@ -376,15 +703,17 @@ extern "C" int eq_lora_add(const void* y, const void* x, const void* a, const vo
                kLoraMaxRanks, kLoraMaxAdapters, (long long)S, (long long)R, (long long)L);
     EQ_REQUIRE(T < (int64_t(1) << 31) / 64 && K < (int64_t(1) << 28) && N < (int64_t(1) << 28), EQ_ERR_UNSUPPORTED, "eq_lora_add: extents too large");
     LoraParams p = {};
-    int64_t end = 0, groups = 0;
+    int64_t end = 0, groups = 0, tiles = 0;
     for (int64_t s = 0; s < S; ++s) {
         const int64_t width = section_widths ? section_widths[s] : (S == 1 ? N : 0);
         EQ_REQUIRE(width > 0 && width % 8 == 0 && width <= N - end, EQ_ERR_BAD_ARG, "eq_lora_add: section %lld has %lld columns: positive multiples of 8 that add up to N", (long long)s,
                    (long long)width);
         end += width;
         groups += ceil_div(width, 32);
+        tiles += ceil_div(width, kLoraTile);
         p.ends[s] = static_cast<int>(end);
         p.group_ends[s] = static_cast<int>(groups);
+        p.tile_ends[s] = static_cast<int>(tiles);
     }
     EQ_REQUIRE(end == N, EQ_ERR_BAD_ARG, "eq_lora_add: the sections hold %lld of %lld columns", (long long)end, (long long)N);
     if (T == 0) return EQ_OK;
@@ -392,7 +721,7 @@ extern "C" int eq_lora_add(const void* y, const void* x, const void* a, const vo
     EQ_REQUIRE(aligned(y, 16) && aligned(x, 16) && aligned(a, 16) && aligned(b, 16) && aligned(out, 16), EQ_ERR_BAD_ALIGN,
                "eq_lora_add: activations and adapters must be 16-byte aligned");
     EQ_REQUIRE(aligned(scaling, 4) && aligned(adapter_ids, 4), EQ_ERR_BAD_ALIGN, "eq_lora_add: scaling and adapter_ids must be 4-byte aligned");
-    const size_t need = eq_lora_workspace_bytes(T, L);
+    const size_t need = eq_lora_workspace_bytes(T, L, S, R);
     EQ_REQUIRE(need == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= need), EQ_ERR_WORKSPACE,
                "eq_lora_add: workspace of %zu bytes (256-byte aligned) needed, %zu given", need, workspace_bytes);
     p.x = x;
@@ -409,22 +738,6 @@ extern "C" int eq_lora_add(const void* y, const void* x, const void* a, const vo
     p.S = static_cast<int>(S);
     p.L = static_cast<int>(L);
     p.in_place = out == y;
-    p.h_stride = static_cast<int>(ceil_div(S * R, 64) * 64 + 16);  // rows 32 bytes apart modulo 128: a half-warp's 8-byte reads meet every bank once
-    if (T <= kLoraSelfPlan) {
-        const int64_t units = group_max_blocks(T, L, 16);
-        return act_dtype == EQ_F16 ? lora_launch<__half, 1>(p, units, stream) : lora_launch<__nv_bfloat16, 1>(p, units, stream);
-    }
-    const int block_rows = S * R <= kLoraWideRanks ? 64 : 16;
     unsigned char* base = static_cast<unsigned char*>(workspace);
-    int32_t* n_blocks = reinterpret_cast<int32_t*>(base);
-    GroupBlock* blocks = reinterpret_cast<GroupBlock*>(base + 256);
-    int32_t* rows = reinterpret_cast<int32_t*>(base + lora_align(256 + static_cast<size_t>(group_max_blocks(T, L, 16)) * sizeof(GroupBlock)));
-    p.blocks = blocks;
-    p.n_blocks = n_blocks;
-    p.rows = rows;
-    const int st = group_rows_launch(adapter_ids, p.T, p.L, !p.in_place, block_rows, blocks, n_blocks, rows, stream);
-    if (st != EQ_OK) return st;
-    const int64_t units = group_max_blocks(T, L, block_rows);
-    if (block_rows == 16) return act_dtype == EQ_F16 ? lora_launch<__half, 1>(p, units, stream) : lora_launch<__nv_bfloat16, 1>(p, units, stream);
-    return act_dtype == EQ_F16 ? lora_launch<__half, 4>(p, units, stream) : lora_launch<__nv_bfloat16, 4>(p, units, stream);
+    return act_dtype == EQ_F16 ? lora_forward<__half>(p, T, L, base, stream) : lora_forward<__nv_bfloat16>(p, T, L, base, stream);
 }

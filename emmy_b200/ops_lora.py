@@ -47,7 +47,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     lib = L.load()
     ws = workspace
     if ws is None and t > 256:
-        ws = _scratch(lib.eq_lora_workspace_bytes(t, adapters), x.device)
+        ws = _scratch(lib.eq_lora_workspace_bytes(t, adapters, s, r), x.device)
     L.check(
         lib.eq_lora_add(
             y.data_ptr(), x.data_ptr(), a.data_ptr(), b.data_ptr(), scaling.data_ptr(), adapter_ids.data_ptr(), t, k, n, r, adapters, s,

@@ -338,7 +338,7 @@ int eq_moe_w8a16(const uint8_t* gate_up, const float* gate_up_scale, const uint8
  * result.  out may be y, and overlaps nothing else.  K, N, R and the widths are multiples of 8, S * R <= 1024, S <= 8, L <= 4096;
  * y, x, a, b and out 16-byte aligned.  The workspace is needed above 256 rows only (256-byte aligned, written before it is read); nothing
  * is kept between calls. */
-size_t eq_lora_workspace_bytes(int64_t T, int64_t L);
+size_t eq_lora_workspace_bytes(int64_t T, int64_t L, int64_t S, int64_t R);
 int eq_lora_add(const void* y, const void* x, const void* a, const void* b, const float* scaling, const int32_t* adapter_ids, int64_t T, int64_t K, int64_t N,
                 int64_t R, int64_t L, int64_t S, const int64_t* section_widths, int act_dtype, void* out, void* workspace, size_t workspace_bytes,
                 void* stream);

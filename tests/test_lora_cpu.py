@@ -35,10 +35,10 @@ def test_lora_add_validates_before_it_launches(eq):
         assert call(**{name: 4104}) == L.EQ_ERR_BAD_ALIGN
     assert call(ids=4098) == L.EQ_ERR_BAD_ALIGN
     # a workspace above 256 rows only
-    assert eq.eq_lora_workspace_bytes(256, 8) == 0 and eq.eq_lora_workspace_bytes(257, 8) > 257 * 4
+    assert eq.eq_lora_workspace_bytes(256, 8, 1, 8) == 0 and eq.eq_lora_workspace_bytes(257, 8, 1, 8) > 257 * (4 + 4 * 8)
     assert call(t=257) == L.EQ_ERR_WORKSPACE
     assert call(t=257, ws=C.c_void_p(4096 + 128), ws_bytes=1 << 20) == L.EQ_ERR_WORKSPACE
-    assert call(t=257, ws=one, ws_bytes=eq.eq_lora_workspace_bytes(257, 3) - 1) == L.EQ_ERR_WORKSPACE
+    assert call(t=257, ws=one, ws_bytes=eq.eq_lora_workspace_bytes(257, 3, 1, 8) - 1) == L.EQ_ERR_WORKSPACE
 
 
 def test_ops_refuse_cpu_tensors():
