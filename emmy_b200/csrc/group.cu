@@ -11,7 +11,7 @@ constexpr int kGroupManyWarps = 8;
 
 __global__ void __launch_bounds__(32 * kGroupWarps) group_rows_kernel(const int32_t* __restrict__ ids, int T, int keys, int keep_rest, int block_rows,
                                                                       GroupBlock* __restrict__ blocks, int32_t* __restrict__ n_blocks,
-                                                                      int32_t* __restrict__ rows) {
+                                                                      int32_t* __restrict__ rows, int* __restrict__ status) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ int32_t counts[];  // [warps][keys + 1] rows, then where the warp's next row of the key goes
     __shared__ int32_t warp_rows[kGroupWarps], warp_blocks[kGroupWarps];
@@ -22,16 +22,22 @@ __global__ void __launch_bounds__(32 * kGroupWarps) group_rows_kernel(const int3
     const int run = (T + 32 * warps - 1) / (32 * warps) * 32;  // rows of a warp
     const int t0 = min(static_cast<int64_t>(run) * warp, static_cast<int64_t>(T)), t1 = min(t0 + run, T);
     int32_t* mine = counts + warp * kinds;
+    constexpr int kAhead = 4;  // ids in flight
     auto kind_of = [&](int t) {
         if (t >= t1) return -1;
         const int id = ids[t];
         return id >= 0 && id < keys ? id : keep_rest ? keys : -1;
     };
-    for (int t = t0; t < t1; t += 32) {
-        const int kind = kind_of(t + lane);
-        const uint32_t same = __match_any_sync(0xFFFFFFFFu, kind);
-        if (kind >= 0 && __ffs(same) - 1 == lane) mine[kind] += __popc(same);
-        __syncwarp();
+    for (int t = t0; t < t1; t += 32 * kAhead) {
+        int kind[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) kind[a] = kind_of(t + 32 * a + lane);
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const uint32_t same = __match_any_sync(0xFFFFFFFFu, kind[a]);
+            if (kind[a] >= 0 && __ffs(same) - 1 == lane) mine[kind[a]] += __popc(same);
+            __syncwarp();
+        }
     }
     __syncthreads();
     // exclusive scans over the kinds, `per` neighbouring ones a thread
@@ -77,20 +83,28 @@ __global__ void __launch_bounds__(32 * kGroupWarps) group_rows_kernel(const int3
             blocks[bat] = blk;
         }
     }
-    if (tid == threads - 1) *n_blocks = bat;
+    if (tid == threads - 1) {
+        *n_blocks = bat;
+        if (status) *status = 0;
+    }
     __syncthreads();
-    for (int t = t0; t < t1; t += 32) {
-        const int kind = kind_of(t + lane);
-        const uint32_t same = __match_any_sync(0xFFFFFFFFu, kind);
-        if (kind >= 0) rows[mine[kind] + __popc(same & ((1u << lane) - 1))] = t + lane;
-        __syncwarp();
-        if (kind >= 0 && __ffs(same) - 1 == lane) mine[kind] += __popc(same);
-        __syncwarp();
+    for (int t = t0; t < t1; t += 32 * kAhead) {
+        int kind[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) kind[a] = kind_of(t + 32 * a + lane);
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const uint32_t same = __match_any_sync(0xFFFFFFFFu, kind[a]);
+            if (kind[a] >= 0) rows[mine[kind[a]] + __popc(same & ((1u << lane) - 1))] = t + 32 * a + lane;
+            __syncwarp();
+            if (kind[a] >= 0 && __ffs(same) - 1 == lane) mine[kind[a]] += __popc(same);
+            __syncwarp();
+        }
     }
 }
 
 int group_rows_launch(const int32_t* ids, int T, int keys, bool keep_rest, int block_rows, GroupBlock* blocks, int32_t* n_blocks, int32_t* rows,
-                      cudaStream_t stream) {
+                      int* status, cudaStream_t stream) {
     static_assert((kGroupFew + 1) * kGroupWarps * 4 <= 160 * 1024 && (kGroupMaxKeys + 1) * kGroupManyWarps * 4 <= 160 * 1024, "the counters");
     EQ_REQUIRE(keys <= kGroupMaxKeys, EQ_ERR_UNSUPPORTED, "at most %d keys", kGroupMaxKeys);
     EQ_CUDA_OK(cudaFuncSetAttribute(group_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
@@ -105,7 +119,7 @@ int group_rows_launch(const int32_t* ids, int T, int keys, bool keep_rest, int b
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    EQ_CUDA_OK(cudaLaunchKernelEx(&cfg, group_rows_kernel, ids, T, keys, static_cast<int>(keep_rest), block_rows, blocks, n_blocks, rows));
+    EQ_CUDA_OK(cudaLaunchKernelEx(&cfg, group_rows_kernel, ids, T, keys, static_cast<int>(keep_rest), block_rows, blocks, n_blocks, rows, status));
     return EQ_OK;
 }
 

@@ -18,8 +18,9 @@ inline int64_t group_max_blocks(int64_t T, int64_t keys, int64_t block_rows) {
 }
 
 // rows[0, ..): the indices 0 .. T - 1 in order of their ids (those outside [0, keys) last, or left out unless keep_rest); blocks: each at
-// most block_rows rows of one key; n_blocks: how many.  The rows of a key stay in their order.  One launch, a programmatic dependent.
+// most block_rows rows of one key; n_blocks: how many; status (may be null): set to zero.  The rows of a key stay in their order.  One launch, a programmatic dependent.
 constexpr int kGroupMaxKeys = 4096;
-int group_rows_launch(const int32_t* ids, int T, int keys, bool keep_rest, int block_rows, GroupBlock* blocks, int32_t* n_blocks, int32_t* rows, cudaStream_t stream);
+int group_rows_launch(const int32_t* ids, int T, int keys, bool keep_rest, int block_rows, GroupBlock* blocks, int32_t* n_blocks, int32_t* rows, int* status,
+                      cudaStream_t stream);
 
 }  // namespace eq

@@ -13,13 +13,16 @@
 //   expand   every CTA takes a share of the columns in groups of 32: rows as M, columns as N, R as K.  The columns of a group are dealt
 //            to the four MMA tiles so that a lane ends with eight neighbouring ones: y is read and written 16 bytes at a time.  The
 //            next group's B and y are on their way while a group is multiplied, the first one's before the CTAs have met.
-// Above, three: group.cu lists blocks of at most 64 rows, lora_shrink_kernel writes h, lora_expand_kernel adds B h to y in tiles of 64 rows x
-// 256 columns, B in shared memory by cp.async one tile ahead.
+// Above, three: group.cu lists blocks of at most 128 rows, lora_shrink_kernel writes h, lora_expand_kernel adds B h to y in tiles of 128 rows x
+// 128 columns.  Both products run on tcgen05: the rows of a block lie anywhere, so the threads gather them by cp.async into the swizzled tile that
+// the MMA reads, one or two steps ahead; two CTAs an SM, so that the sums of one are turned and added while the other's copies land.
 // h is kept in f32 and enters the second product as two 16-bit numbers, value and remainder (bf16: 16 bits of fraction, f16: 22, after
 // the row is brought to the top of f16's range by a power of two): the result is rounded once, as it is stored.
-// mma.sync and not tcgen05: a decode batch is bound by the bytes of A and B, a prompt by those of x and y.
+// Up to 16 rows a block, mma.sync and not tcgen05: a decode batch is bound by the bytes of A and B and by latency, and fragments need no trip through
+// shared or tensor memory.
 #include "group.cuh"
 #include "mma_sync.cuh"
+#include "tc_common.cuh"
 
 namespace eq {
 
@@ -28,10 +31,14 @@ constexpr int kLoraWarps = kLoraThreads / 32;
 constexpr int kLoraSelfPlan = kLoraThreads;  // rows up to which a CTA works out the blocks itself, one row a thread
 constexpr int kLoraMaxSections = 8;
 constexpr int kLoraMaxRanks = 1024;          // S * R
-constexpr int kLoraWideRanks = 256;          // S * R up to which blocks have 64 rows above kLoraSelfPlan rows
+constexpr int kLoraWideRanks = 256;          // S * R up to which blocks have 128 rows above kLoraSelfPlan rows
 constexpr int kLoraMaxAdapters = kGroupMaxKeys;
 constexpr int kLoraPass = 32;                // ranks of a shrink pass
-constexpr int kLoraTile = 256;               // columns of an expand tile
+constexpr int kLoraRows = 128;               // of a block then
+constexpr int kLoraTile = 128;               // columns of an expand tile
+constexpr int kLoraStages = 3;               // of the shrink
+constexpr int kLoraSub = 128 * 128;          // bytes of 128 rows x 64 elements
+constexpr int kLoraTurn = 32 * 36 * 4;       // a warp's 32 x 32 sums, rows 144 bytes apart
 constexpr int kLoraRun = 4;                  // neighbouring tiles that a CTA takes at a time
 
 struct LoraParams {
@@ -48,12 +55,13 @@ struct LoraParams {
     void* hi;             // [T][S R] h of the rows in their order of `rows`, value and remainder
     void* lo;
     float* mul;           // [T] what the products of a row are multiplied by
+    int* status;          // a bounded wait ran out
     int T, K, N, R, S, L;
     int in_place;
     int h_stride;                       // 16-bit elements of a row of h in shared memory
     int ends[kLoraMaxSections];         // columns before the end of section s
     int group_ends[kLoraMaxSections];   // 32-column groups before the end of section s
-    int tile_ends[kLoraMaxSections];    // 256-column tiles before the end of section s
+    int tile_ends[kLoraMaxSections];    // kLoraTile-column tiles before the end of section s
 };
 
 __device__ __forceinline__ void lora_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -82,69 +90,45 @@ __device__ __forceinline__ int lora_adapter(const LoraParams& p, int t) {
 }
 
 // A_l x of the block's rows, this warp's slice of K, all warps' sums added: part[r][n] is this CTA's share.  Ends behind a barrier of the CTA.
-template <typename T, int MT>
+template <typename T>
 __device__ __forceinline__ void lora_shrink(const LoraParams& p, int adapter, int count, const int32_t* rows_s, float* part, float* red, int slice, int slices) {
-    constexpr int kRows = 16 * MT;
+    constexpr int kRows = 16;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, j = lane & 3;
     const int ranks = p.S * p.R;
-    const int tiles_m = (count + 15) >> 4;
     const T* x = static_cast<const T*>(p.x);
     const T* a = static_cast<const T*>(p.a) + static_cast<size_t>(adapter) * ranks * p.K;
     const int chunks = (p.K + 31) / 32;
     const int c0 = static_cast<int>(static_cast<int64_t>(chunks) * slice / slices), c1 = static_cast<int>(static_cast<int64_t>(chunks) * (slice + 1) / slices);
-    const T* xr[MT][2];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = 16 * m + 8 * h + g;
-            xr[m][h] = r < count ? x + static_cast<size_t>(rows_s[r]) * p.K : nullptr;
-        }
+    const T* x0 = g < count ? x + static_cast<size_t>(rows_s[g]) * p.K : nullptr;
+    const T* x1 = g + 8 < count ? x + static_cast<size_t>(rows_s[g + 8]) * p.K : nullptr;
     for (int col = 0; col < ranks; col += kLoraPass) {
-        float acc[MT][4][4];
+        float acc[4][4];
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int n = 0; n < 4; ++n)
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
-#pragma unroll (MT == 1 ? 4 : 1)
+            for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+#pragma unroll 4
         for (int c = c0; c < c1; ++c) {
             const int k = 32 * c + 8 * j;
             const bool in = k < p.K;  // K is a multiple of 8
-            uint4 wv[4], xv[MT][2];
+            const uint4 zero = make_uint4(0, 0, 0, 0);
+            uint4 wv[4];
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
-                wv[n] = in && col + 8 * n < ranks ? __ldg(reinterpret_cast<const uint4*>(a + static_cast<size_t>(col + 8 * n + g) * p.K + k)) : make_uint4(0, 0, 0, 0);
+            for (int n = 0; n < 4; ++n) wv[n] = in && col + 8 * n < ranks ? __ldg(reinterpret_cast<const uint4*>(a + static_cast<size_t>(col + 8 * n + g) * p.K + k)) : zero;
+            const uint4 top = in && x0 ? __ldg(reinterpret_cast<const uint4*>(x0 + k)) : zero, bottom = in && x1 ? __ldg(reinterpret_cast<const uint4*>(x1 + k)) : zero;
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    xv[m][h] = in && xr[m][h] ? __ldg(reinterpret_cast<const uint4*>(xr[m][h] + k)) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                if (m < tiles_m) {
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        mma_16816<T>(acc[m][n], xv[m][0].x, xv[m][1].x, xv[m][0].y, xv[m][1].y, wv[n].x, wv[n].y);
-                        mma_16816<T>(acc[m][n], xv[m][0].z, xv[m][1].z, xv[m][0].w, xv[m][1].w, wv[n].z, wv[n].w);
-                    }
-                }
+            for (int n = 0; n < 4; ++n) {
+                mma_16816<T>(acc[n], top.x, bottom.x, top.y, bottom.y, wv[n].x, wv[n].y);
+                mma_16816<T>(acc[n], top.z, bottom.z, top.w, bottom.w, wv[n].z, wv[n].w);
             }
         }
-        // [row][kLoraPass + 8]: rows a quarter of the banks apart
-        constexpr int kPitch = kLoraPass + 8;
+        constexpr int kPitch = kLoraPass + 8;  // rows a quarter of the banks apart
         float* mine = red + warp * kRows * kPitch;
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-            if (m < tiles_m) {
+        for (int n = 0; n < 4; ++n)
 #pragma unroll
-                for (int n = 0; n < 4; ++n)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        *reinterpret_cast<float2*>(mine + (16 * m + 8 * h + g) * kPitch + 8 * n + 2 * j) = make_float2(acc[m][n][2 * h], acc[m][n][2 * h + 1]);
-            }
+            for (int h = 0; h < 2; ++h) *reinterpret_cast<float2*>(mine + (8 * h + g) * kPitch + 8 * n + 2 * j) = make_float2(acc[n][2 * h], acc[n][2 * h + 1]);
         __syncthreads();
         const int width = min(kLoraPass, ranks - col);
         for (int i = tid; i < count * kLoraPass; i += kLoraThreads) {
@@ -159,9 +143,10 @@ __device__ __forceinline__ void lora_shrink(const LoraParams& p, int adapter, in
     }
 }
 
-// Row r of h over the cluster's shares, scaled, by one warp: put(n, value, remainder) for every rank; the row's factor is returned.
+// A row of h over the cluster's shares (`part`: the row in this CTA's), scaled, by one warp: put(n, value, remainder) for every rank; the row's
+// factor is returned.
 template <typename T, int RANKS, typename Put>
-__device__ __forceinline__ float lora_join(const float* part, int r, int ranks, uint32_t ctas, float scaling, Put&& put) {
+__device__ __forceinline__ float lora_join(const float* part, int ranks, uint32_t ctas, float scaling, Put&& put) {
     const int lane = threadIdx.x & 31;
     float h[RANKS / 32];
     float big = 0.f;
@@ -170,7 +155,7 @@ __device__ __forceinline__ float lora_join(const float* part, int r, int ranks, 
         const int n = lane + 32 * i;
         h[i] = 0.f;
         if (32 * i < ranks) {  // the whole warp
-            const float* at = part + r * ranks + min(n, ranks - 1);
+            const float* at = part + min(n, ranks - 1);
             float v[8];
 #pragma unroll
             for (uint32_t c = 0; c < 8; ++c) v[c] = c < ctas ? lora_peer_load(at, c) : 0.f;
@@ -285,7 +270,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid
     const float scaling = __ldg(p.scaling + adapter);
     float* part = reinterpret_cast<float*>(smem);  // [kRows][ranks]: this CTA's share of K
     float* red = part + kRows * ranks;             // [warps][kRows][kLoraPass + 8]; the split h lies here afterwards
-    lora_shrink<T, 1>(p, adapter, count, rows_s, part, red, cta * kLoraWarps + warp, ctas * kLoraWarps);
+    lora_shrink<T>(p, adapter, count, rows_s, part, red, cta * kLoraWarps + warp, ctas * kLoraWarps);
     lora_cluster_arrive();
 
     // ---- expand: this warp's groups of 32 columns, each in steps of 64 ranks; a step's B and its group's y are asked for one step ahead
@@ -341,8 +326,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid
             lo_s[r * p.h_stride + n] = lo;
         };
         float mul;
-        if (ranks <= 128) mul = lora_join<T, 128>(part, r, ranks, ctas, scaling, put);
-        else mul = lora_join<T, kLoraMaxRanks>(part, r, ranks, ctas, scaling, put);
+        if (ranks <= 128) mul = lora_join<T, 128>(part + r * ranks, ranks, ctas, scaling, put);
+        else mul = lora_join<T, kLoraMaxRanks>(part + r * ranks, ranks, ctas, scaling, put);
         if (lane == 0) mul_s[r] = mul;
     }
     lora_cluster_arrive();  // this CTA is done with the others' shared memory
@@ -403,31 +388,131 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid
     lora_cluster_wait();  // no CTA leaves while another may read its sums
 }
 
-// ------------------------------------------------------------------------------------------------ more rows: blocks of 64, h through memory
+// ------------------------------------------------------------------------------------------------ more rows: blocks of 128, h through memory
+// 16-byte chunk c of row r of a tile of 64-element rows, as the MMA's 128-byte swizzle has it.
+__device__ __forceinline__ uint32_t lora_sw(int r, int c) { return static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4)); }
+// 16 bytes to shared memory, zeros where `in` is false.
+__device__ __forceinline__ void lora_copy(uint32_t to, const void* from, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void lora_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void lora_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Every thread waits for an MMA's commit.  One that does not come is reported; nothing is waited for after that.
+__device__ __forceinline__ bool lora_mma_done(uint32_t bar, uint32_t parity, bool broken, int* status) {
+    if (broken) return false;
+    if (tc::mbar_wait(bar, parity)) return true;
+    atomicExch(status, 1);
+    return false;
+}
+
+template <typename T>
+constexpr uint32_t lora_fmt() {
+    return std::is_same<T, __half>::value ? 0u : 1u;
+}
+
+// h of a block: 128 rows x all ranks, K in steps of 64 cut over the cluster.
 template <typename T>
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ int32_t rows_s[64];
+    extern __shared__ __align__(128) unsigned char smem_raw[];
+    __shared__ int32_t rows_s[kLoraRows];
+    __shared__ __align__(8) uint64_t bars[kLoraStages];
+    __shared__ uint32_t tmem_slot;
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int ranks = p.S * p.R;
+    const int ranks = p.S * p.R, n_mma = (ranks + 15) & ~15;
     const uint32_t cta = lora_cluster_rank(), ctas = lora_cluster_size();
     const int unit = blockIdx.x / ctas;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (unit >= *p.n_blocks) return;
     const GroupBlock blk = p.blocks[unit];
     if (blk.key < 0) return;
-    if (tid < blk.count) rows_s[tid] = p.rows[blk.first + tid];
+    uint32_t cols = 32;
+    while (cols < static_cast<uint32_t>(n_mma)) cols *= 2;
+    if (tid == 0) {
+        for (int i = 0; i < kLoraStages; ++i) tc::mbar_init(tc::smem_u32(bars + i), 1);
+        tc::mbar_fence_init();
+    }
+    if (warp == 0) tc::tmem_alloc(tc::smem_u32(&tmem_slot), cols);
+    if (tid < kLoraRows) rows_s[tid] = p.rows[blk.first + min(tid, blk.count - 1)];  // rows behind the last one repeat it: nobody reads their sums
+    tc::fence_before_sync();
     __syncthreads();
+    tc::fence_after_sync();
+    // with the TMEM columns in hand: a dependent grid that took them first and then waited for this one would never give them back
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t tmem = tmem_slot;
     const float scaling = __ldg(p.scaling + blk.key);
-    float* part = reinterpret_cast<float*>(smem);  // [64][ranks]
-    lora_shrink<T, 4>(p, blk.key, blk.count, rows_s, part, part + 64 * ranks, cta * kLoraWarps + warp, ctas * kLoraWarps);
+    const T* a = static_cast<const T*>(p.a) + static_cast<size_t>(blk.key) * ranks * p.K;
+    const int all = (p.K + 63) / 64;
+    const int s0 = static_cast<int>(static_cast<int64_t>(all) * cta / ctas), steps = static_cast<int>(static_cast<int64_t>(all) * (cta + 1) / ctas) - s0;
+    const int stage_bytes = kLoraSub + ((n_mma * 128 + 1023) & ~1023);
+    const uint32_t base = tc::smem_u32(smem), bar0 = tc::smem_u32(bars);
+    const int c = tid & 7, r0 = tid >> 3;
+    const T* xr[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) xr[i] = static_cast<const T*>(p.x) + static_cast<size_t>(rows_s[r0 + 32 * i]) * p.K;
+    auto ask = [&](int step) {
+        const uint32_t to = base + (step % kLoraStages) * stage_bytes;
+        const int k = 64 * (s0 + step) + 8 * c;
+        const bool in = k < p.K;
+        const int from = in ? k : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lora_copy(to + lora_sw(r0 + 32 * i, c), xr[i] + from, in);
+        for (int r = r0; r < ranks; r += 32) lora_copy(to + kLoraSub + lora_sw(r, c), a + static_cast<size_t>(r) * p.K + from, in);
+    };
+    for (int i = 0; i < kLoraStages - 1; ++i) {
+        if (i < steps) ask(i);
+        lora_commit();
+    }
+    bool broken = false;
+    const uint32_t idesc = tc::instr_desc(lora_fmt<T>(), lora_fmt<T>(), 128, static_cast<uint32_t>(n_mma));
+    for (int step = 0; step < steps; ++step) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kLoraStages - 2) : "memory");
+        lora_proxy_fence();
+        __syncthreads();
+        if (tid == 0) {
+            const uint32_t at = base + (step % kLoraStages) * stage_bytes;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+                tc::mma_f16(tmem, tc::smem_desc_k_sw128(at + ks * 32), tc::smem_desc_k_sw128(at + kLoraSub + ks * 32), idesc, step > 0 || ks > 0);
+            tc::mma_commit(bar0 + 8 * (step % kLoraStages));
+        }
+        // the stage that the step before this one read is filled again
+        if (step > 0 && !lora_mma_done(bar0 + 8 * ((step - 1) % kLoraStages), ((step - 1) / kLoraStages) & 1, broken, p.status)) broken = true;
+        if (step + kLoraStages - 1 < steps) ask(step + kLoraStages - 1);
+        lora_commit();
+    }
+    if (steps > 0 && !lora_mma_done(bar0 + 8 * ((steps - 1) % kLoraStages), ((steps - 1) / kLoraStages) & 1, broken, p.status)) broken = true;
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    tc::fence_after_sync();
+    // this CTA's share of the sums over the stages: [128][ranks + 4]
+    float* part = reinterpret_cast<float*>(smem);
+    const int pitch = ranks + 4;
+    for (int c0 = 32 * (warp >> 2); c0 < ranks; c0 += 64) {
+        const int row = 32 * (warp & 3) + lane;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            if (c0 + 16 * half >= ranks) continue;  // the whole warp
+            uint32_t v[16];
+            if (steps > 0) tc::tmem_ld_32x16(tmem + ((32u * (warp & 3)) << 16) + c0 + 16 * half, v);
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (c0 + 16 * half + 4 * i < ranks)
+                    *reinterpret_cast<uint4*>(part + row * pitch + c0 + 16 * half + 4 * i) =
+                        steps > 0 ? make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == 0) tc::tmem_dealloc(tmem, cols);
     lora_cluster_arrive();
     lora_cluster_wait();
     for (int r = cta * kLoraWarps + warp; r < blk.count; r += ctas * kLoraWarps) {
         T* hi = static_cast<T*>(p.hi) + static_cast<size_t>(blk.first + r) * ranks;
         T* lo = static_cast<T*>(p.lo) + static_cast<size_t>(blk.first + r) * ranks;
-        const float mul = lora_join<T, kLoraWideRanks>(part, r, ranks, ctas, scaling, [&](int n, T vh, T vl) {
+        const float mul = lora_join<T, kLoraWideRanks>(part + r * pitch, ranks, ctas, scaling, [&](int n, T vh, T vl) {
             hi[n] = vh;
             lo[n] = vl;
         });
@@ -437,47 +522,48 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(const __gr
     lora_cluster_wait();
 }
 
-__device__ __forceinline__ void lora_copy16(uint32_t to, const void* from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-}
-
-// 16-byte chunk q (0 to 7) of column n's 64 ranks in a stage.  A warp's 16-byte reads go to columns 2t and 2t + 1 at once: their chunks lie in
-// different halves of the banks.
-__device__ __forceinline__ uint32_t lora_stage_at(int n, int q) { return static_cast<uint32_t>(n * 128 + ((q ^ (((n & 1) << 2) | ((n >> 1) & 3))) << 4)); }
-
-// Tiles of 64 rows x 256 columns: warps 2 x 4, a warp 32 x 64.  Steps are 64 ranks of a tile's B (32 KB), two stages.  A CTA takes runs of
-// neighbouring tiles; the runs are dealt over the CTAs, so that blocks of few rows and of many mix.
+// Tiles of 128 rows x 128 columns, steps of 64 ranks.  A CTA takes runs of neighbouring tiles; the runs are dealt over the CTAs, so that blocks
+// of few rows and of many mix.
 template <typename T>
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(const __grid_constant__ LoraParams p) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ int32_t rows_s[64];
-    __shared__ float mul_s[64];
+    extern __shared__ __align__(128) unsigned char smem_raw[];
+    __shared__ int32_t rows_s[kLoraRows];
+    __shared__ float mul_s[kLoraRows];
+    __shared__ __align__(8) uint64_t bars[2];
+    __shared__ uint32_t tmem_slot;
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int g = lane >> 2, j = lane & 3;
-    const int wr = warp >> 2, wc = warp & 3;
-    const int ranks = p.S * p.R, steps = (p.R + 63) / 64;
-    T* hi_s = reinterpret_cast<T*>(smem + 2 * kLoraTile * 128);  // [64][h_stride], the section's h
-    T* lo_s = hi_s + 64 * p.h_stride;
-    const uint32_t stage0 = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+    const int ranks = p.S * p.R, steps = (p.R + 63) / 64, vecs = p.R / 8;
+    // [2 stages][128 columns x 64 ranks], h: [steps][value, remainder][128 rows x 64 ranks], [warps] sums being turned
+    unsigned char* h_s = smem + 2 * kLoraSub;
+    float* turn = reinterpret_cast<float*>(h_s + steps * 2 * kLoraSub + warp * kLoraTurn);
+    if (tid == 0) {
+        tc::mbar_init(tc::smem_u32(bars), 1);
+        tc::mbar_init(tc::smem_u32(bars + 1), 1);
+        tc::mbar_fence_init();
+    }
+    if (warp == 0) tc::tmem_alloc(tc::smem_u32(&tmem_slot), kLoraTile);
+    // what no copy writes of the last sixteen ranks is zero, in both operands
+    if (p.R % 16)
+        for (int i = tid; i < (2 + 2 * steps) * kLoraSub / 16; i += kLoraThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // with the TMEM columns in hand
+    const uint32_t tmem = tmem_slot, bar0 = tc::smem_u32(bars), b_at = tc::smem_u32(smem), h_at = b_at + 2 * kLoraSub;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int n_blocks = *p.n_blocks, tiles = p.tile_ends[p.S - 1];
     const int64_t units = static_cast<int64_t>(n_blocks) * tiles;
     const T* yin = static_cast<const T*>(p.y);
     T* out = static_cast<T*>(p.out);
 
-    // this CTA's units in order: run i is units [(blockIdx.x + i gridDim.x) kLoraRun, + kLoraRun)
-    auto after = [&](int64_t u) {
-        ++u;
-        return u % kLoraRun ? u : u + static_cast<int64_t>(gridDim.x - 1) * kLoraRun;
-    };
     struct Tile {
         int block, section, first, end;
     };
-    auto tile = [&](int64_t u) {
+    int64_t u = static_cast<int64_t>(blockIdx.x) * kLoraRun;  // this CTA's units: [(blockIdx.x + i gridDim.x) kLoraRun, + kLoraRun)
+    auto locate = [&](int block, int t) {
         Tile v;
-        v.block = static_cast<int>(u / tiles);
-        const int t = static_cast<int>(u - static_cast<int64_t>(v.block) * tiles);
+        v.block = block;
         v.section = 0;
         while (t >= p.tile_ends[v.section]) ++v.section;
         const int s = v.section;
@@ -485,122 +571,135 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(const __gr
         v.end = p.ends[s];
         return v;
     };
-    // 64 ranks of a tile's columns to a stage
+    auto tile = [&](int64_t at) {
+        const int block = static_cast<int>(at / tiles);
+        return locate(block, static_cast<int>(at - static_cast<int64_t>(block) * tiles));
+    };
+    const int c = tid & 7, r0 = tid >> 3;
     auto ask = [&](const Tile& v, int step, int stage) {
         const int key = p.blocks[v.block].key;
-        if (key >= 0) {
-            const T* b = static_cast<const T*>(p.b) + (static_cast<size_t>(key) * p.N + v.first) * p.R + 64 * step;
-            const int cols = min(kLoraTile, v.end - v.first), chunks = min(8, p.R / 8 - 8 * step);
+        if (key >= 0 && 8 * step + c < vecs) {
+            const T* b = static_cast<const T*>(p.b) + (static_cast<size_t>(key) * p.N + v.first + r0) * p.R + 64 * step + 8 * c;
+            const uint32_t to = b_at + stage * kLoraSub + lora_sw(r0, c);  // rows 32 apart have the same swizzle
 #pragma unroll
-            for (int i = 0; i < kLoraTile * 8 / kLoraThreads; ++i) {
-                const int n = (tid + i * kLoraThreads) >> 3, q = tid & 7;
-                if (n < cols && q < chunks) lora_copy16(stage0 + stage * (kLoraTile * 128) + lora_stage_at(n, q), b + static_cast<size_t>(n) * p.R + 8 * q);
-            }
+            for (int i = 0; i < kLoraTile / 32; ++i)
+                if (v.first + r0 + 32 * i < v.end) lora_copy(to + i * 32 * 128, b + static_cast<size_t>(32 * i) * p.R, true);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        lora_commit();
     };
-
-    int64_t u = static_cast<int64_t>(blockIdx.x) * kLoraRun;
-    int stage = 0, held_block = -1, held_section = -1;
-    if (u < units) ask(tile(u), 0, 0);
-    for (; u < units;) {
-        const Tile now = tile(u);
-        const int64_t u_next = after(u);
+    const uint32_t idesc = tc::instr_desc(lora_fmt<T>(), lora_fmt<T>(), 128, kLoraTile);
+    int n_step = 0;  // MMA steps issued so far
+    bool broken = false;
+    auto step_done = [&](int n) {
+        if (!lora_mma_done(bar0 + 8 * (n & 1), (n >> 1) & 1, broken, p.status)) broken = true;
+    };
+    int held_block = -1, held_section = -1;
+    Tile now = {};
+    if (u < units) {
+        now = tile(u);
+        ask(now, 0, 0);
+    }
+    int stage = 0;
+    const int quarter = warp & 3, row_in = lane >> 2, col_in = 64 * (warp >> 2) + 8 * (lane & 3);
+    while (u < units) {
+        int64_t u_next = u + 1;
+        if (u_next % kLoraRun == 0) u_next += static_cast<int64_t>(gridDim.x - 1) * kLoraRun;
+        const bool more = u_next < units;
+        const Tile next = more ? tile(u_next) : now;
         const GroupBlock blk = p.blocks[now.block];
         if (held_block != now.block || held_section != now.section) {
-            __syncthreads();  // everyone is done with the rows and the h held so far
+            __syncthreads();  // everyone is done with the rows held so far; their MMAs are done
             if (tid < blk.count) rows_s[tid] = p.rows[blk.first + tid];
             if (blk.key >= 0) {
                 if (tid < blk.count) mul_s[tid] = p.mul[blk.first + tid];
-                const int vecs = p.R / 8;
                 for (int i = tid; i < blk.count * vecs; i += kLoraThreads) {
                     const int r = i / vecs, v = i - r * vecs;
                     const size_t from = static_cast<size_t>(blk.first + r) * ranks + now.section * p.R + 8 * v;
-                    *reinterpret_cast<uint4*>(hi_s + r * p.h_stride + 8 * v) = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.hi) + from));
-                    *reinterpret_cast<uint4*>(lo_s + r * p.h_stride + 8 * v) = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.lo) + from));
+                    unsigned char* to = h_s + (v >> 3) * 2 * kLoraSub + lora_sw(r, v & 7);
+                    *reinterpret_cast<uint4*>(to) = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.hi) + from));
+                    *reinterpret_cast<uint4*>(to + kLoraSub) = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.lo) + from));
                 }
             }
-            __syncthreads();
             held_block = now.block;
             held_section = now.section;
         }
-        const bool active = 32 * wr < blk.count;
-        float acc[2][2][4][4];  // [16 rows][32 columns][tile][..]
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[m][q][t][e] = 0.f;
         for (int step = 0; step < steps; ++step) {
-            // the next step's B, into the stage that was read last: everyone is past the barrier behind that
-            if (step + 1 < steps) ask(now, step + 1, stage ^ 1);
-            else if (u_next < units) ask(tile(u_next), 0, stage ^ 1);
-            else asm volatile("cp.async.commit_group;" ::: "memory");
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            lora_proxy_fence();
+            tc::fence_before_sync();  // the sums of the tile before this one have been read
             __syncthreads();
-            if (active && blk.key >= 0) {
-                const unsigned char* base = smem + stage * (kLoraTile * 128);
+            if (tid == 0 && blk.key >= 0) {
+                tc::fence_after_sync();
+                const int k16 = min(4, (p.R - 64 * step + 15) / 16);
+                const uint32_t a_at = h_at + step * 2 * kLoraSub, w_at = b_at + stage * kLoraSub;
+                for (int ks = 0; ks < k16; ++ks) {
+                    const uint64_t w = tc::smem_desc_k_sw128(w_at + ks * 32);
+                    tc::mma_f16(tmem, tc::smem_desc_k_sw128(a_at + ks * 32), w, idesc, step > 0 || ks > 0);
+                    tc::mma_f16(tmem, tc::smem_desc_k_sw128(a_at + kLoraSub + ks * 32), w, idesc, true);
+                }
+                tc::mma_commit(bar0 + 8 * (n_step & 1));
+            }
+            // the other stage is filled again: the MMA that read it is done (it ended a tile, or is waited for here)
+            if (step > 0 && blk.key >= 0) step_done(n_step - 1);
+            if (blk.key >= 0) ++n_step;
+            if (step + 1 < steps) ask(now, step + 1, stage ^ 1);
+            else if (more) ask(next, 0, stage ^ 1);
+            stage ^= 1;
+        }
+        // y of this thread's rows and columns, then the sums
+        uint4 yv[4][2];
+        size_t at[4];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int k = 64 * step + 32 * c;
-                    if (k >= p.R) break;
-                    const bool in = k + 8 * j < p.R;
+        for (int i = 0; i < 4; ++i) {
+            const int r = 32 * quarter + 8 * i + row_in;
+            at[i] = 0;
+            if (r < blk.count) {
+                at[i] = static_cast<size_t>(rows_s[r]) * p.N + now.first + col_in;
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        uint4 top[2], bottom[2];
+                for (int h = 0; h < 2; ++h)
+                    if (now.first + col_in + 32 * h < now.end) yv[i][h] = *reinterpret_cast<const uint4*>(yin + at[i] + 32 * h);
+            }
+        }
+        if (blk.key >= 0) {
+            step_done(n_step - 1);
+            tc::fence_after_sync();
+        }
+        if (32 * quarter < blk.count) {
 #pragma unroll
-                        for (int m = 0; m < 2; ++m) {
-                            const T* at = (half ? lo_s : hi_s) + (32 * wr + 16 * m + g) * p.h_stride + k + 8 * j;
-                            top[m] = in ? *reinterpret_cast<const uint4*>(at) : make_uint4(0, 0, 0, 0);
-                            bottom[m] = in ? *reinterpret_cast<const uint4*>(at + 8 * p.h_stride) : make_uint4(0, 0, 0, 0);
+            for (int h = 0; h < 2; ++h) {
+                if (blk.key >= 0) {
+                    uint32_t v[32];
+                    tc::tmem_ld_32x32(tmem + ((32u * quarter) << 16) + 64 * (warp >> 2) + 32 * h, v);
+                    tc::tmem_ld_wait();
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(turn + lane * 36 + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                    __syncwarp();
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = 8 * i + row_in;
+                    if (32 * quarter + r < blk.count && now.first + col_in + 32 * h < now.end) {
+                        uint4 w = yv[i][h];
+                        if (blk.key >= 0) {
+                            const float mul = mul_s[32 * quarter + r];
+                            const float4 d0 = *reinterpret_cast<const float4*>(turn + r * 36 + 8 * (lane & 3)), d1 = *reinterpret_cast<const float4*>(turn + r * 36 + 8 * (lane & 3) + 4);
+                            const float d[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
+                            T* e = reinterpret_cast<T*>(&w);
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) e[q] = from_float<T>(fmaf(d[q], mul, to_float(e[q])));
                         }
-#pragma unroll
-                        for (int q = 0; q < 2; ++q)
-#pragma unroll
-                            for (int t = 0; t < 4; ++t) {
-                                const int n = 64 * wc + 32 * q + 8 * (g >> 1) + 2 * t + (g & 1);
-                                const uint4 w = in ? *reinterpret_cast<const uint4*>(base + lora_stage_at(n, 4 * c + j)) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                                for (int m = 0; m < 2; ++m) {
-                                    mma_16816<T>(acc[m][q][t], top[m].x, bottom[m].x, top[m].y, bottom[m].y, w.x, w.y);
-                                    mma_16816<T>(acc[m][q][t], top[m].z, bottom[m].z, top[m].w, bottom[m].w, w.z, w.w);
-                                }
-                            }
+                        *reinterpret_cast<uint4*>(out + at[i] + 32 * h) = w;
                     }
                 }
             }
-            __syncthreads();
-            stage ^= 1;
-        }
-        if (active) {
-            uint4 yv[2][2][2];
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const int r = 32 * wr + 16 * m + 8 * h + g, n = now.first + 64 * wc + 32 * q + 8 * j;
-                        if (r < blk.count && n < now.end) yv[m][h][q] = *reinterpret_cast<const uint4*>(yin + static_cast<size_t>(rows_s[r]) * p.N + n);
-                    }
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const int r = 32 * wr + 16 * m + 8 * h + g, n = now.first + 64 * wc + 32 * q + 8 * j;
-                        if (r < blk.count && n < now.end)
-                            *reinterpret_cast<uint4*>(out + static_cast<size_t>(rows_s[r]) * p.N + n) =
-                                blk.key >= 0 ? lora_add8<T>(yv[m][h][q], acc[m][q], h, mul_s[r]) : yv[m][h][q];
-                    }
         }
         u = u_next;
+        now = next;
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == 0) tc::tmem_dealloc(tmem, kLoraTile);
 }
 
 static size_t lora_align(size_t v) { return (v + 255) / 256 * 256; }
@@ -631,51 +730,49 @@ static int lora_launch(void (*kernel)(const LoraParams), const LoraParams& p, in
     return EQ_OK;
 }
 
-// Shared memory of a shrink over blocks of `rows` rows, with room for the split h behind the sums where it is kept there.
-static size_t lora_smem(int rows, int ranks, int h_stride, bool keep) {
-    const size_t red = static_cast<size_t>(kLoraWarps) * rows * (kLoraPass + 8) * sizeof(float), split = keep ? 2 * static_cast<size_t>(rows) * h_stride * 2 : 0;
-    return static_cast<size_t>(rows) * ranks * sizeof(float) + (red > split ? red : split);
-}
+// Bytes of A's rows in a stage of the shrink.
+static size_t lora_stage_rows(int ranks) { return (static_cast<size_t>((ranks + 15) & ~15) * 128 + 1023) & ~size_t(1023); }
 
 template <typename T>
 static int lora_forward(LoraParams p, int64_t T_, int64_t L, unsigned char* base, cudaStream_t stream) {
     const int ranks = p.S * p.R;
-    // 16-bit elements of a row of h: rows 64 bytes apart modulo 128, so that the 16-byte reads of two rows meet every bank once
-    auto stride = [](int n) { return (n + 63) / 64 * 64 + 32; };
-    const int block_rows = p.T > kLoraSelfPlan && ranks <= kLoraWideRanks ? 64 : 16;
+    const int block_rows = p.T > kLoraSelfPlan && ranks <= kLoraWideRanks ? kLoraRows : 16;
     const int64_t units = group_max_blocks(T_, L, block_rows);
     if (p.T > kLoraSelfPlan) {
-        size_t o = 0;
+        size_t o = 256;
         auto take = [&](size_t bytes) {
             void* at = base + o;
             o += lora_align(bytes);
             return at;
         };
-        int32_t* n_blocks = static_cast<int32_t*>(take(4));
+        p.status = reinterpret_cast<int*>(base);
+        int32_t* n_blocks = reinterpret_cast<int32_t*>(base) + 1;
         GroupBlock* blocks = static_cast<GroupBlock*>(take(static_cast<size_t>(units) * sizeof(GroupBlock)));
         int32_t* rows = static_cast<int32_t*>(take(static_cast<size_t>(T_) * 4));
         p.blocks = blocks;
         p.n_blocks = n_blocks;
         p.rows = rows;
-        const int st = group_rows_launch(p.ids, p.T, p.L, !p.in_place, block_rows, blocks, n_blocks, rows, stream);
+        const int st = group_rows_launch(p.ids, p.T, p.L, !p.in_place, block_rows, blocks, n_blocks, rows, p.status, stream);
         if (st != EQ_OK) return st;
-        if (block_rows == 64) {
+        if (block_rows == kLoraRows) {
             p.mul = static_cast<float*>(take(static_cast<size_t>(T_) * 4));
             p.hi = take(static_cast<size_t>(T_) * ranks * 2);
             p.lo = take(static_cast<size_t>(T_) * ranks * 2);
         }
     }
     if (block_rows == 16) {
-        p.h_stride = stride(ranks);
+        p.h_stride = (ranks + 63) / 64 * 64 + 32;  // rows 64 bytes apart modulo 128: the 16-byte reads of two rows meet every bank once
+        const size_t red = static_cast<size_t>(kLoraWarps) * 16 * (kLoraPass + 8) * sizeof(float), split = 2 * static_cast<size_t>(16) * p.h_stride * 2;
         const int ctas = lora_cluster(units, 2);
-        return lora_launch(lora_rows_kernel<T>, p, units * ctas, ctas, lora_smem(16, ranks, p.h_stride, true), stream);
+        return lora_launch(lora_rows_kernel<T>, p, units * ctas, ctas, static_cast<size_t>(16) * ranks * sizeof(float) + (red > split ? red : split), stream);
     }
+    const size_t stages = static_cast<size_t>(kLoraStages) * (kLoraSub + lora_stage_rows(ranks)), sums = static_cast<size_t>(kLoraRows) * (ranks + 4) * sizeof(float);
     const int ctas = lora_cluster(units, 1);
-    const int st = lora_launch(lora_shrink_kernel<T>, p, units * ctas, ctas, lora_smem(64, ranks, 0, false), stream);
+    const int st = lora_launch(lora_shrink_kernel<T>, p, units * ctas, ctas, 1024 + (stages > sums ? stages : sums), stream);
     if (st != EQ_OK) return st;
-    p.h_stride = stride(p.R);
-    const int64_t runs = ceil_div(units * p.tile_ends[p.S - 1], kLoraRun), most = 2 * sm_count();
-    return lora_launch(lora_expand_kernel<T>, p, runs < most ? runs : most, 1, 2 * kLoraTile * 128 + 2 * static_cast<size_t>(64) * p.h_stride * 2, stream);
+    const size_t smem = 1024 + static_cast<size_t>(2 + 2 * ((p.R + 63) / 64)) * kLoraSub + kLoraWarps * kLoraTurn;
+    const int64_t runs = ceil_div(units * p.tile_ends[p.S - 1], kLoraRun), most = (smem <= 113 * 1024 ? 2 : 1) * sm_count();
+    return lora_launch(lora_expand_kernel<T>, p, runs < most ? runs : most, 1, smem, stream);
 }
 
 }  // namespace eq
@@ -740,4 +837,14 @@ extern "C" int eq_lora_add(const void* y, const void* x, const void* a, const vo
     p.in_place = out == y;
     unsigned char* base = static_cast<unsigned char*>(workspace);
     return act_dtype == EQ_F16 ? lora_forward<__half>(p, T, L, base, stream) : lora_forward<__nv_bfloat16>(p, T, L, base, stream);
+}
+
+extern "C" int eq_lora_status(const void* workspace, void* stream_) {
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    EQ_REQUIRE(workspace, EQ_ERR_BAD_ARG, "eq_lora_status: null workspace");
+    int host = 0;
+    EQ_CUDA_OK(cudaMemcpyAsync(&host, workspace, sizeof(int), cudaMemcpyDeviceToHost, stream));
+    EQ_CUDA_OK(cudaStreamSynchronize(stream));
+    EQ_REQUIRE(host == 0, EQ_ERR_TIMEOUT, "eq_lora_status: a bounded pipeline wait ran out (code %d)", host);
+    return EQ_OK;
 }

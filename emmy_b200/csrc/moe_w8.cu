@@ -696,7 +696,7 @@ static int w8_forward(W8Params p, const uint8_t* gate_up, const float* gate_up_s
     }
     int st = eq_moe_route(p.logits, p.T, p.E, p.topk, 1, w.ids, w.scores, stream);
     if (st != EQ_OK) return st;
-    st = group_rows_launch(w.ids, static_cast<int>(R), p.E, false, kW8BlockRows, w.blocks, w.n_blocks, w.rows, stream);
+    st = group_rows_launch(w.ids, static_cast<int>(R), p.E, false, kW8BlockRows, w.blocks, w.n_blocks, w.rows, nullptr, stream);
     if (st != EQ_OK) return st;
     st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, false, false>, 2 * sm_count(), ring + part, stream, p);
     if (st != EQ_OK) return st;

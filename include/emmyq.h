@@ -342,6 +342,8 @@ size_t eq_lora_workspace_bytes(int64_t T, int64_t L, int64_t S, int64_t R);
 int eq_lora_add(const void* y, const void* x, const void* a, const void* b, const float* scaling, const int32_t* adapter_ids, int64_t T, int64_t K, int64_t N,
                 int64_t R, int64_t L, int64_t S, const int64_t* section_widths, int act_dtype, void* out, void* workspace, size_t workspace_bytes,
                 void* stream);
+/* Synchronizes the stream; EQ_ERR_TIMEOUT if a bounded pipeline wait of the last call of more than 256 rows on this workspace ran out. */
+int eq_lora_status(const void* workspace, void* stream);
 
 /* ------------------------------------------------------------------ expert-parallel MoE over peer memory */
 
