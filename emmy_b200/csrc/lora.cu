@@ -13,7 +13,7 @@
 //   expand   every CTA takes a share of the columns in groups of 32: rows as M, columns as N, R as K.  The columns of a group are dealt
 //            to the four MMA tiles so that a lane ends with eight neighbouring ones: y is read and written 16 bytes at a time.  The
 //            next group's B and y are on their way while a group is multiplied, the first one's before the CTAs have met.
-// Above, three: group.cu lists blocks of at most 128 rows, lora_shrink_kernel writes h, lora_expand_kernel adds B h to y in tiles of 128 rows x
+// Above, two, the first of them group.cu's list of the blocks; for larger calls (lora_block_rows) three: blocks of at most 128 rows, lora_shrink_kernel writes h, lora_expand_kernel adds B h to y in tiles of 128 rows x
 // 128 columns.  Both products run on tcgen05: the rows of a block lie anywhere, so the threads gather them by cp.async into the swizzled tile that
 // the MMA reads, one or two steps ahead; two CTAs an SM, so that the sums of one are turned and added while the other's copies land.
 // h is kept in f32 and enters the second product as two 16-bit numbers, value and remainder (bf16: 16 bits of fraction, f16: 22, after
@@ -31,15 +31,14 @@ constexpr int kLoraWarps = kLoraThreads / 32;
 constexpr int kLoraSelfPlan = kLoraThreads;  // rows up to which a CTA works out the blocks itself, one row a thread
 constexpr int kLoraMaxSections = 8;
 constexpr int kLoraMaxRanks = 1024;          // S * R
-constexpr int kLoraWideRanks = 256;          // S * R up to which blocks have 128 rows above kLoraSelfPlan rows
+constexpr int kLoraWideRanks = 256;          // S * R, and
+constexpr int kLoraWideRank = 128;           // R, up to which blocks have 128 rows above kLoraSelfPlan rows
 constexpr int kLoraMaxAdapters = kGroupMaxKeys;
 constexpr int kLoraPass = 32;                // ranks of a shrink pass
 constexpr int kLoraRows = 128;               // of a block then
 constexpr int kLoraTile = 128;               // columns of an expand tile
-constexpr int kLoraStages = 3;               // of the shrink
+constexpr int kLoraStages = 6;               // of the shrink at most
 constexpr int kLoraSub = 128 * 128;          // bytes of 128 rows x 64 elements
-constexpr int kLoraTurn = 32 * 36 * 4;       // a warp's 32 x 32 sums, rows 144 bytes apart
-constexpr int kLoraRun = 4;                  // neighbouring tiles that a CTA takes at a time
 
 struct LoraParams {
     const void* x;        // [T][K]
@@ -49,15 +48,17 @@ struct LoraParams {
     const float* scaling; // [L]
     const int32_t* ids;   // [T]
     void* out;            // [T][N], may be y
-    const GroupBlock* blocks;  // above kLoraSelfPlan rows
+    GroupBlock* blocks;        // above kLoraSelfPlan rows
     const int32_t* n_blocks;
     const int32_t* rows;
-    void* hi;             // [T][S R] h of the rows in their order of `rows`, value and remainder
+    void* hi;             // [T][S x R rounded up to 16] h of the rows in their order of `rows`, value and remainder
     void* lo;
     float* mul;           // [T] what the products of a row are multiplied by
     int* status;          // a bounded wait ran out
     int T, K, N, R, S, L;
     int in_place;
+    int run;                            // neighbouring expand tiles that a CTA takes at a time
+    int stages;                         // of the shrink: 3, or kLoraStages where they fit beside a second CTA
     int h_stride;                       // 16-bit elements of a row of h in shared memory
     int ends[kLoraMaxSections];         // columns before the end of section s
     int group_ends[kLoraMaxSections];   // 32-column groups before the end of section s
@@ -90,7 +91,7 @@ __device__ __forceinline__ int lora_adapter(const LoraParams& p, int t) {
 }
 
 // A_l x of the block's rows, this warp's slice of K, all warps' sums added: part[r][n] is this CTA's share.  Ends behind a barrier of the CTA.
-template <typename T>
+template <typename T, int kUnroll>
 __device__ __forceinline__ void lora_shrink(const LoraParams& p, int adapter, int count, const int32_t* rows_s, float* part, float* red, int slice, int slices) {
     constexpr int kRows = 16;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -108,7 +109,7 @@ __device__ __forceinline__ void lora_shrink(const LoraParams& p, int adapter, in
         for (int n = 0; n < 4; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-#pragma unroll 4
+#pragma unroll kUnroll
         for (int c = c0; c < c1; ++c) {
             const int k = 32 * c + 8 * j;
             const bool in = k < p.K;  // K is a multiple of 8
@@ -199,10 +200,11 @@ __device__ __forceinline__ uint4 lora_add8(uint4 v, const float (&acc)[4][4], in
 }
 
 // ------------------------------------------------------------------------------------------------ up to 256 rows (or more than 256 ranks): blocks of 16 rows
-template <typename T>
+// kChunks: of 32 ranks, what a lane asks for at a time; one where there are no more (K=14336 N=4096, rank 32, 17 rows 8.8 us against 10.2; three CTAs an
+// SM then, of 80 registers, 10.5).
+template <typename T, int kChunks>
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid_constant__ LoraParams p) {
     constexpr int kRows = 16;
-    constexpr int kChunks = 2;  // of 32 ranks: what a lane asks for at a time
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int32_t rows_s[kRows];
@@ -270,7 +272,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid
     const float scaling = __ldg(p.scaling + adapter);
     float* part = reinterpret_cast<float*>(smem);  // [kRows][ranks]: this CTA's share of K
     float* red = part + kRows * ranks;             // [warps][kRows][kLoraPass + 8]; the split h lies here afterwards
-    lora_shrink<T>(p, adapter, count, rows_s, part, red, cta * kLoraWarps + warp, ctas * kLoraWarps);
+    lora_shrink<T, 2 * kChunks>(p, adapter, count, rows_s, part, red, cta * kLoraWarps + warp, ctas * kLoraWarps);
     lora_cluster_arrive();
 
     // ---- expand: this warp's groups of 32 columns, each in steps of 64 ranks; a step's B and its group's y are asked for one step ahead
@@ -327,7 +329,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid
         };
         float mul;
         if (ranks <= 128) mul = lora_join<T, 128>(part + r * ranks, ranks, ctas, scaling, put);
-        else mul = lora_join<T, kLoraMaxRanks>(part + r * ranks, ranks, ctas, scaling, put);
+        else mul = lora_join<T, kChunks == 1 ? 32 * kLoraMaxSections : kLoraMaxRanks>(part + r * ranks, ranks, ctas, scaling, put);
         if (lane == 0) mul_s[r] = mul;
     }
     lora_cluster_arrive();  // this CTA is done with the others' shared memory
@@ -389,6 +391,9 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid
 }
 
 // ------------------------------------------------------------------------------------------------ more rows: blocks of 128, h through memory
+// A block's note: its first row where its rows are neighbours, or a few rows or many that lie apart.
+constexpr int kLoraFew = -1, kLoraApart = -2;
+
 // 16-byte chunk c of row r of a tile of 64-element rows, as the MMA's 128-byte swizzle has it.
 __device__ __forceinline__ uint32_t lora_sw(int r, int c) { return static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4)); }
 // 16 bytes to shared memory, zeros where `in` is false.
@@ -420,12 +425,16 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(const __gr
     __shared__ uint32_t tmem_slot;
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int ranks = p.S * p.R, n_mma = (ranks + 15) & ~15;
+    const int ranks = p.S * p.R, n_mma = (ranks + 15) & ~15, section_ranks = (p.R + 15) & ~15, pad = section_ranks - p.R;
     const uint32_t cta = lora_cluster_rank(), ctas = lora_cluster_size();
     const int unit = blockIdx.x / ctas;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (unit >= *p.n_blocks) return;
     const GroupBlock blk = p.blocks[unit];
+    if (cta == 0 && tid == 0) {  // the rows of a block ascend
+        const int first = p.rows[blk.first], last = p.rows[blk.first + blk.count - 1];
+        p.blocks[unit].note = last - first == blk.count - 1 ? first : blk.count <= 32 ? kLoraFew : kLoraApart;
+    }
     if (blk.key < 0) return;
     uint32_t cols = 32;
     while (cols < static_cast<uint32_t>(n_mma)) cols *= 2;
@@ -434,7 +443,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(const __gr
         tc::mbar_fence_init();
     }
     if (warp == 0) tc::tmem_alloc(tc::smem_u32(&tmem_slot), cols);
-    if (tid < kLoraRows) rows_s[tid] = p.rows[blk.first + min(tid, blk.count - 1)];  // rows behind the last one repeat it: nobody reads their sums
+    if (tid < kLoraRows) rows_s[tid] = tid < blk.count ? p.rows[blk.first + tid] : -1;  // rows behind the last one: nobody reads their sums
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
@@ -450,39 +459,51 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(const __gr
     const int c = tid & 7, r0 = tid >> 3;
     const T* xr[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) xr[i] = static_cast<const T*>(p.x) + static_cast<size_t>(rows_s[r0 + 32 * i]) * p.K;
-    auto ask = [&](int step) {
-        const uint32_t to = base + (step % kLoraStages) * stage_bytes;
+    for (int i = 0; i < 4; ++i) xr[i] = rows_s[r0 + 32 * i] >= 0 ? static_cast<const T*>(p.x) + static_cast<size_t>(rows_s[r0 + 32 * i]) * p.K : nullptr;
+    const int stages = p.stages;
+    auto ask = [&](int step, int stage) {
+        const uint32_t to = base + stage * stage_bytes;
         const int k = 64 * (s0 + step) + 8 * c;
         const bool in = k < p.K;
         const int from = in ? k : 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) lora_copy(to + lora_sw(r0 + 32 * i, c), xr[i] + from, in);
+        for (int i = 0; i < 4; ++i)
+            if (xr[i]) lora_copy(to + lora_sw(r0 + 32 * i, c), xr[i] + from, in);
         for (int r = r0; r < ranks; r += 32) lora_copy(to + kLoraSub + lora_sw(r, c), a + static_cast<size_t>(r) * p.K + from, in);
     };
-    for (int i = 0; i < kLoraStages - 1; ++i) {
-        if (i < steps) ask(i);
+    for (int i = 0; i < stages - 1; ++i) {
+        if (i < steps) ask(i, i);
         lora_commit();
     }
     bool broken = false;
     const uint32_t idesc = tc::instr_desc(lora_fmt<T>(), lora_fmt<T>(), 128, static_cast<uint32_t>(n_mma));
+    int stage = 0, before = 0;      // of this step, of the step before
+    uint32_t phase = 0, phase_before = 0;
     for (int step = 0; step < steps; ++step) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kLoraStages - 2) : "memory");
+        // (the group of this step is the one behind stages - 2 younger ones)
+        if (stages == 3) asm volatile("cp.async.wait_group 1;" ::: "memory");
+        else asm volatile("cp.async.wait_group %0;" ::"n"(kLoraStages - 2) : "memory");
         lora_proxy_fence();
         __syncthreads();
         if (tid == 0) {
-            const uint32_t at = base + (step % kLoraStages) * stage_bytes;
+            const uint32_t at = base + stage * stage_bytes;
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
                 tc::mma_f16(tmem, tc::smem_desc_k_sw128(at + ks * 32), tc::smem_desc_k_sw128(at + kLoraSub + ks * 32), idesc, step > 0 || ks > 0);
-            tc::mma_commit(bar0 + 8 * (step % kLoraStages));
+            tc::mma_commit(bar0 + 8 * stage);
         }
         // the stage that the step before this one read is filled again
-        if (step > 0 && !lora_mma_done(bar0 + 8 * ((step - 1) % kLoraStages), ((step - 1) / kLoraStages) & 1, broken, p.status)) broken = true;
-        if (step + kLoraStages - 1 < steps) ask(step + kLoraStages - 1);
+        if (step > 0 && !lora_mma_done(bar0 + 8 * before, phase_before, broken, p.status)) broken = true;
+        if (step + stages - 1 < steps) ask(step + stages - 1, step > 0 ? before : stages - 1);
         lora_commit();
+        before = stage;
+        phase_before = phase;
+        if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
+        }
     }
-    if (steps > 0 && !lora_mma_done(bar0 + 8 * ((steps - 1) % kLoraStages), ((steps - 1) / kLoraStages) & 1, broken, p.status)) broken = true;
+    if (steps > 0 && !lora_mma_done(bar0 + 8 * before, phase_before, broken, p.status)) broken = true;
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
     tc::fence_after_sync();
@@ -510,204 +531,377 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(const __gr
     lora_cluster_arrive();
     lora_cluster_wait();
     for (int r = cta * kLoraWarps + warp; r < blk.count; r += ctas * kLoraWarps) {
-        T* hi = static_cast<T*>(p.hi) + static_cast<size_t>(blk.first + r) * ranks;
-        T* lo = static_cast<T*>(p.lo) + static_cast<size_t>(blk.first + r) * ranks;
+        T* hi = static_cast<T*>(p.hi) + static_cast<size_t>(blk.first + r) * p.S * section_ranks;
+        T* lo = static_cast<T*>(p.lo) + static_cast<size_t>(blk.first + r) * p.S * section_ranks;
         const float mul = lora_join<T, kLoraWideRanks>(part + r * pitch, ranks, ctas, scaling, [&](int n, T vh, T vl) {
-            hi[n] = vh;
-            lo[n] = vl;
+            const int to = n + n / p.R * pad;
+            hi[to] = vh;
+            lo[to] = vl;
         });
+        if (pad)  // eight ranks behind each section's: zeros, the MMA takes sixteen at a time
+            for (int i = lane; i < 8 * p.S; i += 32) {
+                const int to = (i >> 3) * section_ranks + p.R + (i & 7);
+                hi[to] = lo[to] = from_float<T>(0.f);
+            }
         if (lane == 0) p.mul[blk.first + r] = mul;
     }
     lora_cluster_arrive();
     lora_cluster_wait();
 }
 
-// Tiles of 128 rows x 128 columns, steps of 64 ranks.  A CTA takes runs of neighbouring tiles; the runs are dealt over the CTAs, so that blocks
-// of few rows and of many mix.
+// ---- y + B h in tiles of 128 rows x 128 columns
+constexpr int kLoraExpandThreads = 320;
+constexpr int kLoraTileY = 2 * kLoraSub;             // a y tile: two halves of 64 columns, swizzled
+constexpr int kLoraMostY = 4, kLoraMostB = 3;
+
+// Rings of y tiles, of B tiles (`steps` x 64 ranks), and h (value and remainder), in shared memory.
+struct LoraExpandLayout {
+    int ys, bs, b_bytes, h_bytes;
+    size_t smem;
+};
+__host__ __device__ inline LoraExpandLayout lora_layout(int steps) {
+    LoraExpandLayout v;
+    v.ys = steps == 1 ? 4 : 3;
+    v.bs = steps == 1 ? 3 : 1;
+    v.b_bytes = steps * kLoraSub;
+    v.h_bytes = 2 * steps * kLoraSub;
+    v.smem = 1024 + static_cast<size_t>(v.ys) * kLoraTileY + static_cast<size_t>(v.bs) * v.b_bytes + v.h_bytes;
+    return v;
+}
+
+__device__ __forceinline__ void lora_tma_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(bar),
+                 "r"(c0), "r"(c1), "r"(c2)
+                 : "memory");
+}
+__device__ __forceinline__ void lora_bulk_in(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void lora_tma_store(const CUtensorMap* map, int c0, int c1, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src), "r"(c0), "r"(c1) : "memory");
+}
+
+// The n-th use of a ring of `size` barriers.
+__device__ __forceinline__ bool lora_ring_wait(uint32_t ring, int n, int size) { return tc::mbar_wait(ring + 8 * (n % size), static_cast<uint32_t>((n / size) & 1)); }
+
+// What the copying warp tells the others about a tile.
+struct LoraTile {
+    int32_t live;                    // 0: no more tiles
+    int32_t mma;                     // which of the CTA's products the tile's is; -1: none
+    int32_t first, cols;             // columns
+    int32_t count, note;             // the block's
+    int32_t row[kLoraRows];
+    float mul[kLoraRows];
+};
+struct LoraProduct {
+    int32_t live, new_h, last_h;     // the first and the last one that reads h as it is
+};
+
+// A CTA takes runs of neighbouring tiles; the runs are dealt over the CTAs, so that blocks of few rows and of many mix.
+// Warp 0 brings y, B and (when the run, the block or the section changes) h by TMA and notes what a tile is; warp 1 issues the MMAs, h as two operands
+// against the same B, into one of two accumulators; warps 2 to 9 add the sums to y where it lies (a row a lane, two warps a row quarter) and send the
+// parts out by TMA.  Everything but the additions is asynchronous, so one CTA an SM with two or three tiles on their way is bound by memory.  (A second
+// eight of adding warps gained nothing.)
+// That is for blocks whose rows are neighbours, a prompt's.  A few rows that lie apart, requests that decode, come by a bulk copy each
+// (about 50 cycles a copy: for all rows the same prompt took 532 us); of more, and at ragged ends, a lane reads and writes its row's 128 bytes itself.
+// Waits are bounded.
 template <typename T>
-__global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(const __grid_constant__ LoraParams p) {
+__global__ void __launch_bounds__(kLoraExpandThreads, 1)
+    lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_hi, const __grid_constant__ CUtensorMap map_lo,
+                       const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_out, const __grid_constant__ LoraParams p) {
     extern __shared__ __align__(128) unsigned char smem_raw[];
-    __shared__ int32_t rows_s[kLoraRows];
-    __shared__ float mul_s[kLoraRows];
-    __shared__ __align__(8) uint64_t bars[2];
+    __shared__ LoraTile notes[kLoraMostY];
+    __shared__ LoraProduct products[kLoraMostB];
+    __shared__ __align__(8) uint64_t bars[2 * kLoraMostY + 2 * kLoraMostB + 4 + 2];
     __shared__ uint32_t tmem_slot;
-    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int ranks = p.S * p.R, steps = (p.R + 63) / 64, vecs = p.R / 8;
-    // [2 stages][128 columns x 64 ranks], h: [steps][value, remainder][128 rows x 64 ranks], [warps] sums being turned
-    unsigned char* h_s = smem + 2 * kLoraSub;
-    float* turn = reinterpret_cast<float*>(h_s + steps * 2 * kLoraSub + warp * kLoraTurn);
-    if (tid == 0) {
-        tc::mbar_init(tc::smem_u32(bars), 1);
-        tc::mbar_init(tc::smem_u32(bars + 1), 1);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int steps = (p.R + 63) / 64, section_ranks = (p.R + 15) & ~15;
+    const LoraExpandLayout lay = lora_layout(steps);
+    const uint32_t y_at = (tc::smem_u32(smem_raw) + 1023) & ~1023u, b_at = y_at + lay.ys * kLoraTileY, h_at = b_at + lay.bs * lay.b_bytes;
+    const uint32_t y_full = tc::smem_u32(bars), y_free = y_full + 8 * kLoraMostY, b_full = y_free + 8 * kLoraMostY, b_free = b_full + 8 * kLoraMostB;
+    const uint32_t acc_full = b_free + 8 * kLoraMostB, acc_free = acc_full + 16, h_full = acc_free + 16, h_free = h_full + 8;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kLoraMostY; ++i) {
+            tc::mbar_init(y_full + 8 * i, 1);
+            tc::mbar_init(y_free + 8 * i, 8);
+        }
+        for (int i = 0; i < kLoraMostB; ++i) {
+            tc::mbar_init(b_full + 8 * i, 1);
+            tc::mbar_init(b_free + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(acc_full + 8 * i, 1);
+            tc::mbar_init(acc_free + 8 * i, 8);
+        }
+        tc::mbar_init(h_full, 1);
+        tc::mbar_init(h_free, 1);
         tc::mbar_fence_init();
     }
-    if (warp == 0) tc::tmem_alloc(tc::smem_u32(&tmem_slot), kLoraTile);
-    // what no copy writes of the last sixteen ranks is zero, in both operands
-    if (p.R % 16)
-        for (int i = tid; i < (2 + 2 * steps) * kLoraSub / 16; i += kLoraThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+    if (warp == 1) tc::tmem_alloc(tc::smem_u32(&tmem_slot), 2 * kLoraTile);
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // with the TMEM columns in hand
-    const uint32_t tmem = tmem_slot, bar0 = tc::smem_u32(bars), b_at = tc::smem_u32(smem), h_at = b_at + 2 * kLoraSub;
+    // with the TMEM columns in hand: a dependent grid that took them first and then waited for this one would never give them back
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t tmem = tmem_slot;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int n_blocks = *p.n_blocks, tiles = p.tile_ends[p.S - 1];
-    const int64_t units = static_cast<int64_t>(n_blocks) * tiles;
-    const T* yin = static_cast<const T*>(p.y);
-    T* out = static_cast<T*>(p.out);
-
-    struct Tile {
-        int block, section, first, end;
-    };
-    int64_t u = static_cast<int64_t>(blockIdx.x) * kLoraRun;  // this CTA's units: [(blockIdx.x + i gridDim.x) kLoraRun, + kLoraRun)
-    auto locate = [&](int block, int t) {
-        Tile v;
-        v.block = block;
-        v.section = 0;
-        while (t >= p.tile_ends[v.section]) ++v.section;
-        const int s = v.section;
-        v.first = (s ? p.ends[s - 1] : 0) + kLoraTile * (t - (s ? p.tile_ends[s - 1] : 0));
-        v.end = p.ends[s];
-        return v;
-    };
-    auto tile = [&](int64_t at) {
-        const int block = static_cast<int>(at / tiles);
-        return locate(block, static_cast<int>(at - static_cast<int64_t>(block) * tiles));
-    };
-    const int c = tid & 7, r0 = tid >> 3;
-    auto ask = [&](const Tile& v, int step, int stage) {
-        const int key = p.blocks[v.block].key;
-        if (key >= 0 && 8 * step + c < vecs) {
-            const T* b = static_cast<const T*>(p.b) + (static_cast<size_t>(key) * p.N + v.first + r0) * p.R + 64 * step + 8 * c;
-            const uint32_t to = b_at + stage * kLoraSub + lora_sw(r0, c);  // rows 32 apart have the same swizzle
+    if (warp == 0) {
+        // ---- copies in
+        const int tiles = p.tile_ends[p.S - 1], n_blocks = *p.n_blocks;
+        const int64_t step = static_cast<int64_t>(gridDim.x - 1) * p.run + 1;  // from the last tile of a run to the first of the next
+        const int step_blocks = static_cast<int>(step / tiles), step_tiles = static_cast<int>(step % tiles);
+        int block = static_cast<int>(static_cast<int64_t>(blockIdx.x) * p.run / tiles), t = static_cast<int>(static_cast<int64_t>(blockIdx.x) * p.run % tiles);
+        int left = p.run, section = 0, n = 0, n_b = 0, n_h = 0;  // left: tiles of the run, this one included
+        bool new_block = true, new_h = true;                     // since the tile before
+        GroupBlock blk = {};
+        int row[4] = {};
+        float mul[4] = {};
+        bool ok = true;
+        for (; block < n_blocks; ++n) {
+            while (t >= p.tile_ends[section]) ++section;
+            const int first = (section ? p.ends[section - 1] : 0) + kLoraTile * (t - (section ? p.tile_ends[section - 1] : 0));
+            const int cols = min(kLoraTile, p.ends[section] - first), halves = cols > 64 ? 2 : 1;
+            if (new_block) {
+                blk = p.blocks[block];
+                // neighbouring rows need no list, and a factor is one in bf16
+                if (blk.note < 0 || std::is_same<T, __half>::value) {
 #pragma unroll
-            for (int i = 0; i < kLoraTile / 32; ++i)
-                if (v.first + r0 + 32 * i < v.end) lora_copy(to + i * 32 * 128, b + static_cast<size_t>(32 * i) * p.R, true);
-        }
-        lora_commit();
-    };
-    const uint32_t idesc = tc::instr_desc(lora_fmt<T>(), lora_fmt<T>(), 128, kLoraTile);
-    int n_step = 0;  // MMA steps issued so far
-    bool broken = false;
-    auto step_done = [&](int n) {
-        if (!lora_mma_done(bar0 + 8 * (n & 1), (n >> 1) & 1, broken, p.status)) broken = true;
-    };
-    int held_block = -1, held_section = -1;
-    Tile now = {};
-    if (u < units) {
-        now = tile(u);
-        ask(now, 0, 0);
-    }
-    int stage = 0;
-    const int quarter = warp & 3, row_in = lane >> 2, col_in = 64 * (warp >> 2) + 8 * (lane & 3);
-    while (u < units) {
-        int64_t u_next = u + 1;
-        if (u_next % kLoraRun == 0) u_next += static_cast<int64_t>(gridDim.x - 1) * kLoraRun;
-        const bool more = u_next < units;
-        const Tile next = more ? tile(u_next) : now;
-        const GroupBlock blk = p.blocks[now.block];
-        if (held_block != now.block || held_section != now.section) {
-            __syncthreads();  // everyone is done with the rows held so far; their MMAs are done
-            if (tid < blk.count) rows_s[tid] = p.rows[blk.first + tid];
-            if (blk.key >= 0) {
-                if (tid < blk.count) mul_s[tid] = p.mul[blk.first + tid];
-                for (int i = tid; i < blk.count * vecs; i += kLoraThreads) {
-                    const int r = i / vecs, v = i - r * vecs;
-                    const size_t from = static_cast<size_t>(blk.first + r) * ranks + now.section * p.R + 8 * v;
-                    unsigned char* to = h_s + (v >> 3) * 2 * kLoraSub + lora_sw(r, v & 7);
-                    *reinterpret_cast<uint4*>(to) = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.hi) + from));
-                    *reinterpret_cast<uint4*>(to + kLoraSub) = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.lo) + from));
-                }
-            }
-            held_block = now.block;
-            held_section = now.section;
-        }
-        for (int step = 0; step < steps; ++step) {
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            lora_proxy_fence();
-            tc::fence_before_sync();  // the sums of the tile before this one have been read
-            __syncthreads();
-            if (tid == 0 && blk.key >= 0) {
-                tc::fence_after_sync();
-                const int k16 = min(4, (p.R - 64 * step + 15) / 16);
-                const uint32_t a_at = h_at + step * 2 * kLoraSub, w_at = b_at + stage * kLoraSub;
-                for (int ks = 0; ks < k16; ++ks) {
-                    const uint64_t w = tc::smem_desc_k_sw128(w_at + ks * 32);
-                    tc::mma_f16(tmem, tc::smem_desc_k_sw128(a_at + ks * 32), w, idesc, step > 0 || ks > 0);
-                    tc::mma_f16(tmem, tc::smem_desc_k_sw128(a_at + kLoraSub + ks * 32), w, idesc, true);
-                }
-                tc::mma_commit(bar0 + 8 * (n_step & 1));
-            }
-            // the other stage is filled again: the MMA that read it is done (it ended a tile, or is waited for here)
-            if (step > 0 && blk.key >= 0) step_done(n_step - 1);
-            if (blk.key >= 0) ++n_step;
-            if (step + 1 < steps) ask(now, step + 1, stage ^ 1);
-            else if (more) ask(next, 0, stage ^ 1);
-            stage ^= 1;
-        }
-        // y of this thread's rows and columns, then the sums
-        uint4 yv[4][2];
-        size_t at[4];
+                    for (int q = 0; q < 4; ++q) {
+                        const int r = lane + 32 * q;
+                        row[q] = r < blk.count ? p.rows[blk.first + r] : 0;
+                        mul[q] = r < blk.count && blk.key >= 0 ? p.mul[blk.first + r] : 0.f;
+                    }
+                } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = 32 * quarter + 8 * i + row_in;
-            at[i] = 0;
-            if (r < blk.count) {
-                at[i] = static_cast<size_t>(rows_s[r]) * p.N + now.first + col_in;
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    if (now.first + col_in + 32 * h < now.end) yv[i][h] = *reinterpret_cast<const uint4*>(yin + at[i] + 32 * h);
-            }
-        }
-        if (blk.key >= 0) {
-            step_done(n_step - 1);
-            tc::fence_after_sync();
-        }
-        if (32 * quarter < blk.count) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (blk.key >= 0) {
-                    uint32_t v[32];
-                    tc::tmem_ld_32x32(tmem + ((32u * quarter) << 16) + 64 * (warp >> 2) + 32 * h, v);
-                    tc::tmem_ld_wait();
-                    __syncwarp();
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(turn + lane * 36 + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                    __syncwarp();
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = 8 * i + row_in;
-                    if (32 * quarter + r < blk.count && now.first + col_in + 32 * h < now.end) {
-                        uint4 w = yv[i][h];
-                        if (blk.key >= 0) {
-                            const float mul = mul_s[32 * quarter + r];
-                            const float4 d0 = *reinterpret_cast<const float4*>(turn + r * 36 + 8 * (lane & 3)), d1 = *reinterpret_cast<const float4*>(turn + r * 36 + 8 * (lane & 3) + 4);
-                            const float d[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
-                            T* e = reinterpret_cast<T*>(&w);
-#pragma unroll
-                            for (int q = 0; q < 8; ++q) e[q] = from_float<T>(fmaf(d[q], mul, to_float(e[q])));
-                        }
-                        *reinterpret_cast<uint4*>(out + at[i] + 32 * h) = w;
+                    for (int q = 0; q < 4; ++q) {
+                        row[q] = blk.note + lane + 32 * q;
+                        mul[q] = 1.f;
                     }
                 }
             }
+            const bool adds = blk.key >= 0;
+            // h is asked for anew with every run, block and section, and given back with the last tile before the next: what that is, is known here
+            const bool last_h = left == 1 || t + 1 == p.tile_ends[section];
+            const int sb = n_b % lay.bs, sy = n % lay.ys;
+            if (adds && n_b >= lay.bs) ok = lora_ring_wait(b_free, n_b - lay.bs, lay.bs);
+            if (ok && adds && new_h && n_h > 0) ok = lora_ring_wait(h_free, n_h - 1, 1);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            if (adds) {
+                if (lane == 0) {
+                    products[sb].live = 1;
+                    products[sb].new_h = new_h;
+                    products[sb].last_h = last_h;
+                    tc::mbar_expect_tx(b_full + 8 * sb, lay.b_bytes);
+                    for (int k = 0; k < steps; ++k) lora_tma_3d(b_at + sb * lay.b_bytes + k * kLoraSub, &map_b, 64 * k, first, blk.key, b_full + 8 * sb);
+                    if (new_h) {
+                        tc::mbar_expect_tx(h_full, lay.h_bytes);
+                        for (int k = 0; k < steps; ++k) {
+                            tc::tma_load_2d(h_at + 2 * k * kLoraSub, &map_hi, section * section_ranks + 64 * k, blk.first, h_full);
+                            tc::tma_load_2d(h_at + (2 * k + 1) * kLoraSub, &map_lo, section * section_ranks + 64 * k, blk.first, h_full);
+                        }
+                    }
+                }
+                ++n_b;
+                n_h += new_h;
+            }
+            if (n >= lay.ys) ok = lora_ring_wait(y_free, n - lay.ys, lay.ys);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            LoraTile& note = notes[sy];
+            if (lane == 0) {
+                note.live = 1;
+                note.mma = adds ? n_b - 1 : -1;
+                note.first = first;
+                note.cols = cols;
+                note.count = blk.count;
+                note.note = blk.note;
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                note.row[lane + 32 * q] = row[q];
+                note.mul[lane + 32 * q] = mul[q];
+            }
+            __syncwarp();
+            const uint32_t bar = y_full + 8 * sy, to = y_at + sy * kLoraTileY;
+            if (lane == 0) {
+                tc::mbar_expect_tx(bar, blk.note >= 0 ? halves * kLoraSub : blk.note == kLoraFew ? blk.count * cols * 2 : 0);
+                if (blk.note >= 0)
+                    for (int h = 0; h < halves; ++h) tc::tma_load_2d(to + h * kLoraSub, &map_y, first + 64 * h, blk.note, bar);
+            }
+            if (blk.note == kLoraFew) {
+                __syncwarp();  // behind the bytes that are expected
+                if (lane < blk.count)
+                    for (int h = 0; h < halves; ++h)
+                        lora_bulk_in(to + h * kLoraSub + lane * 128, static_cast<const T*>(p.y) + static_cast<size_t>(row[0]) * p.N + first + 64 * h, 2 * min(64, cols - 64 * h), bar);
+            }
+            // the next tile
+            new_block = false;
+            new_h = last_h;
+            if (--left == 0) {
+                left = p.run;
+                block += step_blocks;
+                t += step_tiles;
+                section = 0;
+                new_block = step_blocks > 0;
+            } else {
+                ++t;
+            }
+            if (t >= tiles) {
+                t -= tiles;
+                ++block;
+                section = 0;
+                new_block = true;
+            }
         }
-        u = u_next;
-        now = next;
+        // the end
+        if (ok && n_b >= lay.bs) ok = lora_ring_wait(b_free, n_b - lay.bs, lay.bs);
+        if (ok && lane == 0) {
+            products[n_b % lay.bs].live = 0;
+            tc::mbar_arrive(b_full + 8 * (n_b % lay.bs));
+        }
+        if (ok && n >= lay.ys) ok = lora_ring_wait(y_free, n - lay.ys, lay.ys);
+        if (ok && lane == 0) {
+            notes[n % lay.ys].live = 0;
+            tc::mbar_arrive(y_full + 8 * (n % lay.ys));
+        }
+        if (!ok && lane == 0) {  // nothing may land behind the CTA's end
+            atomicExch(p.status, 1);
+            for (int i = n < lay.ys ? 0 : n - lay.ys; i < n; ++i) lora_ring_wait(y_full, i, lay.ys);
+            for (int i = n_b < lay.bs ? 0 : n_b - lay.bs; i < n_b; ++i) lora_ring_wait(b_full, i, lay.bs);
+            if (n_h > 0) lora_ring_wait(h_full, n_h - 1, 1);
+        }
+    } else if (warp == 1) {
+        // ---- MMAs
+        if (lane == 0) {
+            const uint32_t idesc = tc::instr_desc(lora_fmt<T>(), lora_fmt<T>(), 128, kLoraTile);
+            int n_h = 0, n = 0;
+            for (;; ++n) {
+                const int s = n % lay.bs;
+                bool ok = lora_ring_wait(b_full, n, lay.bs);
+                if (ok && !products[s].live) break;
+                const bool last_h = ok && products[s].last_h;
+                if (ok && products[s].new_h) ok = lora_ring_wait(h_full, n_h++, 1);
+                if (ok && n >= 2) ok = lora_ring_wait(acc_free, n - 2, 2);
+                if (!ok) {
+                    atomicExch(p.status, 2);
+                    break;
+                }
+                tc::fence_after_sync();
+                const uint32_t d = tmem + kLoraTile * (n & 1), w_at = b_at + s * lay.b_bytes;
+                for (int k = 0; k < section_ranks / 16; ++k) {
+                    const uint32_t a = h_at + (k >> 2) * 2 * kLoraSub + (k & 3) * 32;
+                    const uint64_t w = tc::smem_desc_k_sw128(w_at + (k >> 2) * kLoraSub + (k & 3) * 32);
+                    tc::mma_f16(d, tc::smem_desc_k_sw128(a), w, idesc, k > 0);
+                    tc::mma_f16(d, tc::smem_desc_k_sw128(a + kLoraSub), w, idesc, true);
+                }
+                if (last_h) tc::mma_commit(h_free);
+                tc::mma_commit(b_free + 8 * s);
+                tc::mma_commit(acc_full + 8 * (n & 1));
+            }
+            if (n > 0) lora_ring_wait(acc_full, n - 1, 2);  // nothing in flight when the columns are given back
+        }
+    } else {
+        // ---- sums, a row a lane
+        const int quarter = warp & 3, half = (warp - 2) >> 2, r = 32 * quarter + lane;
+        for (int n = 0;; ++n) {
+            const int s = n % lay.ys;
+            if (!__all_sync(0xFFFFFFFFu, lora_ring_wait(y_full, n, lay.ys))) {
+                if (lane == 0) atomicExch(p.status, 3);
+                break;
+            }
+            const LoraTile& note = notes[s];
+            if (!note.live) break;
+            const int mma = note.mma, count = note.count, where = note.note, first = note.first + 64 * half;
+            const int bytes = min(128, 2 * note.cols - 128 * half);  // of this warp's columns
+            const bool has = r < count, here = where != kLoraApart, whole = where >= 0 && bytes == 128 && 32 * quarter + 32 <= count;
+            const bool mine = 32 * quarter < count && bytes > 0;  // of the whole warp
+            const int turn = where >= 0 ? r & 7 : 0;  // TMA has swizzled the tile, bulk copies of rows have not
+            const uint32_t part = y_at + s * kLoraTileY + half * kLoraSub, at = part + r * 128;
+            const size_t to = static_cast<size_t>(note.row[r]) * p.N + first;
+            const float mul = note.mul[r];
+            uint4 y[8];
+            if (mine) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    if (here)
+                        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(y[c].x), "=r"(y[c].y), "=r"(y[c].z), "=r"(y[c].w) : "r"(at + ((c ^ turn) << 4)) : "memory");
+                    else if (has && 16 * c < bytes)
+                        y[c] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.y) + to + 8 * c);
+                }
+            }
+            if (mma >= 0) {
+                if (!lora_ring_wait(acc_full, mma, 2)) atomicExch(p.status, 3);
+                __syncwarp();
+                if (mine) {
+                    tc::fence_after_sync();
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t v[32];
+                        tc::tmem_ld_32x32(tmem + ((32u * quarter) << 16) + kLoraTile * (mma & 1) + 64 * half + 32 * h, v);
+                        tc::tmem_ld_wait();
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            T* e = reinterpret_cast<T*>(&y[4 * h + c]);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) e[i] = from_float<T>(fmaf(__uint_as_float(v[8 * c + i]), mul, to_float(e[i])));
+                        }
+                    }
+                }
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(acc_free + 8 * (mma & 1));
+            }
+            if (mine && whole) {
+                if (mma >= 0) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        asm volatile("st.shared.v4.u32 [%4], {%0,%1,%2,%3};" ::"r"(y[c].x), "r"(y[c].y), "r"(y[c].z), "r"(y[c].w), "r"(at + ((c ^ turn) << 4)) : "memory");
+                    lora_proxy_fence();
+                    __syncwarp();
+                }
+                if (lane == 0) {
+                    lora_tma_store(&map_out, first, where + 32 * quarter, part + 32 * quarter * 128);
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                }
+            } else if (mine && has) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    if (16 * c < bytes) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + to + 8 * c) = y[c];
+            }
+            // the slot is free once its rows have been read, by the lanes and by the copy out
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(y_free + 8 * s);
+        }
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     tc::fence_before_sync();
     __syncthreads();
-    if (warp == 0) tc::tmem_dealloc(tmem, kLoraTile);
+    if (warp == 1) tc::tmem_dealloc(tmem, 2 * kLoraTile);
 }
 
 static size_t lora_align(size_t v) { return (v + 255) / 256 * 256; }
 
-// CTAs of a cluster: the largest of 8, 4, 2, 1 whose grid stays within `waves` rounds of two CTAs an SM.
-static int lora_cluster(int64_t units, int waves) {
+static bool lora_wide(int64_t S, int64_t R) { return R <= kLoraWideRank && S <= kLoraMaxSections && S * R <= kLoraWideRanks; }
+
+// Rows of a block.  Above kLoraSelfPlan rows, 16 (lora_rows_kernel reads a block's A and B from L2 again for every 16 rows, and has one launch behind the list) up to
+// T (K + 2 N) max(R, 32) = 10^9, 128 from there on.  Both forced, 16 : 128, us, prompts of 3 adapters | with 100 rows that decode, of 16 adapters:
+//   K=N=4096, rank 16         600 rows 20 : 25 | 20 : 34, 1200 25 : 26 | 27 : 34, 2400 43 : 34 | 44 : 42, 4800 73 : 48 | 73 : 52
+//   K=4096 N=28672, rank 16   300 rows 29 : 30 | 30 : 73, 600 53 : 38 | 53 : 82, 1200 88 : 50 | 88 : 87, 4800 307 : 121 | 303 : 161
+//   K=14336 N=4096, rank 16   600 rows 25 : 35 | 26 : 45, 1200 40 : 37 | 41 : 46, 2400 67 : 46 | 67 : 64
+//   K=N=4096, rank 64         300 rows 19 : 24 | 19 : 31, 600 30 : 26 | 31 : 36, 1200 39 : 27 | 46 : 36; rank 128  300 rows 27 : 27 | 28 : 35, 600 45 : 29 | 47 : 41
+static int lora_block_rows(int64_t T, int64_t K, int64_t N, int64_t S, int64_t R) {
+    if (T <= kLoraSelfPlan || !lora_wide(S, R)) return 16;
+    return static_cast<double>(T) * (K + 2 * N) * (R < 32 ? 32 : R) < 1e9 ? 16 : kLoraRows;
+}
+static int64_t lora_units(int64_t T, int64_t L, int block_rows) { return group_max_blocks(T, L, block_rows, block_rows == kLoraRows); }
+
+// CTAs of a cluster: the largest of 8, 4, 2, 1 whose grid stays within `most` CTAs an SM.  (The grid is sized for the most blocks that the rows can
+// make: usually there are fewer.)
+static int lora_cluster(int64_t units, int most) {
     int ctas = 8;
-    while (ctas > 1 && units * ctas > 2 * waves * sm_count()) ctas /= 2;
+    while (ctas > 1 && units * ctas > most * sm_count()) ctas /= 2;
     return ctas;
 }
 
@@ -735,9 +929,9 @@ static size_t lora_stage_rows(int ranks) { return (static_cast<size_t>((ranks + 
 
 template <typename T>
 static int lora_forward(LoraParams p, int64_t T_, int64_t L, unsigned char* base, cudaStream_t stream) {
-    const int ranks = p.S * p.R;
-    const int block_rows = p.T > kLoraSelfPlan && ranks <= kLoraWideRanks ? kLoraRows : 16;
-    const int64_t units = group_max_blocks(T_, L, block_rows);
+    const int ranks = p.S * p.R, section_ranks = (p.R + 15) & ~15;
+    const int block_rows = lora_block_rows(p.T, p.K, p.N, p.S, p.R);
+    const int64_t units = lora_units(T_, L, block_rows);
     if (p.T > kLoraSelfPlan) {
         size_t o = 256;
         auto take = [&](size_t bytes) {
@@ -752,27 +946,53 @@ static int lora_forward(LoraParams p, int64_t T_, int64_t L, unsigned char* base
         p.blocks = blocks;
         p.n_blocks = n_blocks;
         p.rows = rows;
-        const int st = group_rows_launch(p.ids, p.T, p.L, !p.in_place, block_rows, blocks, n_blocks, rows, p.status, stream);
+        const int st = group_rows_launch(p.ids, p.T, p.L, !p.in_place, block_rows, block_rows == kLoraRows, blocks, n_blocks, rows, p.status, stream);
         if (st != EQ_OK) return st;
         if (block_rows == kLoraRows) {
             p.mul = static_cast<float*>(take(static_cast<size_t>(T_) * 4));
-            p.hi = take(static_cast<size_t>(T_) * ranks * 2);
-            p.lo = take(static_cast<size_t>(T_) * ranks * 2);
+            p.hi = take(static_cast<size_t>(T_) * p.S * section_ranks * 2);
+            p.lo = take(static_cast<size_t>(T_) * p.S * section_ranks * 2);
         }
     }
     if (block_rows == 16) {
         p.h_stride = (ranks + 63) / 64 * 64 + 32;  // rows 64 bytes apart modulo 128: the 16-byte reads of two rows meet every bank once
         const size_t red = static_cast<size_t>(kLoraWarps) * 16 * (kLoraPass + 8) * sizeof(float), split = 2 * static_cast<size_t>(16) * p.h_stride * 2;
-        const int ctas = lora_cluster(units, 2);
-        return lora_launch(lora_rows_kernel<T>, p, units * ctas, ctas, static_cast<size_t>(16) * ranks * sizeof(float) + (red > split ? red : split), stream);
+        const int ctas = lora_cluster(units, 4);
+        return lora_launch(p.R <= 32 ? lora_rows_kernel<T, 1> : lora_rows_kernel<T, 2>, p, units * ctas, ctas, static_cast<size_t>(16) * ranks * sizeof(float) + (red > split ? red : split), stream);
     }
-    const size_t stages = static_cast<size_t>(kLoraStages) * (kLoraSub + lora_stage_rows(ranks)), sums = static_cast<size_t>(kLoraRows) * (ranks + 4) * sizeof(float);
-    const int ctas = lora_cluster(units, 1);
+    // 64 steps of 5120 x 16 ranks, us: three stages .. six ..
+    p.stages = kLoraStages * (kLoraSub + lora_stage_rows(ranks)) <= 110 * 1024 ? kLoraStages : 3;
+    const size_t stages = p.stages * (kLoraSub + lora_stage_rows(ranks)), sums = static_cast<size_t>(kLoraRows) * (ranks + 4) * sizeof(float);
+    const int ctas = lora_cluster(units, 3);
     const int st = lora_launch(lora_shrink_kernel<T>, p, units * ctas, ctas, 1024 + (stages > sums ? stages : sums), stream);
     if (st != EQ_OK) return st;
-    const size_t smem = 1024 + static_cast<size_t>(2 + 2 * ((p.R + 63) / 64)) * kLoraSub + kLoraWarps * kLoraTurn;
-    const int64_t runs = ceil_div(units * p.tile_ends[p.S - 1], kLoraRun), most = (smem <= 113 * 1024 ? 2 : 1) * sm_count();
-    return lora_launch(lora_expand_kernel<T>, p, runs < most ? runs : most, 1, smem, stream);
+    const CUtensorMapDataType elem = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    CUtensorMap map_b, map_hi, map_lo, map_y, map_out;
+    int mt = make_tensor_map_3d(&map_b, p.b, elem, 2, p.L, p.N, p.R, kLoraTile, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+    const uint64_t h_cols = static_cast<uint64_t>(p.S) * section_ranks;
+    if (mt == EQ_OK) mt = make_tensor_map_2d(&map_hi, p.hi, elem, 2, p.T, h_cols, h_cols * 2, kLoraRows, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (mt == EQ_OK) mt = make_tensor_map_2d(&map_lo, p.lo, elem, 2, p.T, h_cols, h_cols * 2, kLoraRows, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (mt == EQ_OK) mt = make_tensor_map_2d(&map_y, p.y, elem, 2, p.T, p.N, static_cast<uint64_t>(p.N) * 2, kLoraRows, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (mt == EQ_OK) mt = make_tensor_map_2d(&map_out, p.out, elem, 2, p.T, p.N, static_cast<uint64_t>(p.N) * 2, 32, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (mt != EQ_OK) return mt;
+    const LoraExpandLayout lay = lora_layout((p.R + 63) / 64);
+    // a CTA's tiles: runs of four where that leaves at least two runs a CTA, fewer where there are few tiles
+    const int64_t all_tiles = units * p.tile_ends[p.S - 1];
+    p.run = static_cast<int>(all_tiles / (2 * sm_count()) < 1 ? 1 : all_tiles / (2 * sm_count()) > 4 ? 4 : all_tiles / (2 * sm_count()));
+    const int64_t runs = ceil_div(all_tiles, p.run);
+    EQ_CUDA_OK(cudaFuncSetAttribute(lora_expand_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lay.smem)));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(runs < sm_count() ? runs : sm_count()));
+    cfg.blockDim = dim3(kLoraExpandThreads);
+    cfg.dynamicSmemBytes = lay.smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    EQ_CUDA_OK(cudaLaunchKernelEx(&cfg, lora_expand_kernel<T>, map_b, map_hi, map_lo, map_y, map_out, static_cast<const LoraParams&>(p)));
+    return EQ_OK;
 }
 
 }  // namespace eq
@@ -781,9 +1001,9 @@ using namespace eq;
 
 extern "C" size_t eq_lora_workspace_bytes(int64_t T, int64_t L, int64_t S, int64_t R) {
     if (T <= kLoraSelfPlan || L <= 0 || S <= 0 || R <= 0) return 0;
-    const size_t lists = 256 + lora_align(static_cast<size_t>(group_max_blocks(T, L, 16)) * sizeof(GroupBlock)) + lora_align(static_cast<size_t>(T) * 4);
-    if (S > kLoraWideRanks || R > kLoraWideRanks || S * R > kLoraWideRanks) return lists;
-    return lists + lora_align(static_cast<size_t>(T) * 4) + 2 * lora_align(static_cast<size_t>(T) * S * R * 2);
+    const int64_t few = lora_units(T, L, 16), many = lora_units(T, L, kLoraRows);
+    const size_t lists = 256 + lora_align(static_cast<size_t>(few > many ? few : many) * sizeof(GroupBlock)) + lora_align(static_cast<size_t>(T) * 4);
+    return !lora_wide(S, R) ? lists : lists + lora_align(static_cast<size_t>(T) * 4) + 2 * lora_align(static_cast<size_t>(T) * S * ((R + 15) / 16 * 16) * 2);
 }
 
 extern "C" int eq_lora_add(const void* y, const void* x, const void* a, const void* b, const float* scaling, const int32_t* adapter_ids, int64_t T, int64_t K,

@@ -654,7 +654,7 @@ static W8Workspace w8_carve(void* base, int64_t T, int64_t E, int64_t topk, int6
         w.scores = static_cast<float*>(take(R * 4));
         w.rows = static_cast<int32_t*>(take(R * 4));
         w.n_blocks = static_cast<int32_t*>(take(4));
-        w.blocks = static_cast<GroupBlock*>(take(static_cast<size_t>(group_max_blocks(R, E, kW8BlockRows)) * sizeof(GroupBlock)));
+        w.blocks = static_cast<GroupBlock*>(take(static_cast<size_t>(group_max_blocks(R, E, kW8BlockRows, false)) * sizeof(GroupBlock)));
         w.rows_out = static_cast<float*>(take(static_cast<size_t>(R) * H * 4));
     }
     w.bytes = o;
@@ -696,7 +696,7 @@ static int w8_forward(W8Params p, const uint8_t* gate_up, const float* gate_up_s
     }
     int st = eq_moe_route(p.logits, p.T, p.E, p.topk, 1, w.ids, w.scores, stream);
     if (st != EQ_OK) return st;
-    st = group_rows_launch(w.ids, static_cast<int>(R), p.E, false, kW8BlockRows, w.blocks, w.n_blocks, w.rows, nullptr, stream);
+    st = group_rows_launch(w.ids, static_cast<int>(R), p.E, false, kW8BlockRows, false, w.blocks, w.n_blocks, w.rows, nullptr, stream);
     if (st != EQ_OK) return st;
     st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, false, false>, 2 * sm_count(), ring + part, stream, p);
     if (st != EQ_OK) return st;

@@ -219,5 +219,8 @@ __host__ __device__ constexpr uint32_t instr_desc_nvfp4(uint32_t m, uint32_t n, 
 // box of box_cols x box_rows elements and the 128-byte swizzle.  elem: CU_TENSOR_MAP_DATA_TYPE_*.
 int make_tensor_map_2d(CUtensorMap* map, const void* base, CUtensorMapDataType elem, size_t elem_bytes, uint64_t rows,
                        uint64_t cols, uint64_t pitch, uint32_t box_rows, uint32_t box_cols, CUtensorMapSwizzle swizzle);
+// The same for a contiguous [planes][rows][cols] array and boxes of one plane.
+int make_tensor_map_3d(CUtensorMap* map, const void* base, CUtensorMapDataType elem, size_t elem_bytes, uint64_t planes, uint64_t rows, uint64_t cols,
+                       uint32_t box_rows, uint32_t box_cols, CUtensorMapSwizzle swizzle);
 
 }  // namespace eq

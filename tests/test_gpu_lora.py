@@ -51,8 +51,7 @@ def close(got, y, x, a, b, scaling, ids, sections):
     limit = (torch.finfo(dtype).eps / 2) * (ref.abs() + chain * size) + chain * size + tiny
     off = (got.double() - ref).abs()
     assert torch.isfinite(got).all()
-    worst = (off / limit).max().item()
-    assert worst <= 1, f"{worst:.2f} of the limit"
+    assert (off <= limit).all(), f"{(off - limit).max().item():.3g} over a limit of {limit.max().item():.3g}"
     none = ~((ids >= 0) & (ids < len(a)))
     assert torch.equal(got[none], y[none])
 
@@ -82,6 +81,12 @@ def call(args, sections, **kw):
         (321, 512, [256, 256], 256, 7),  # 512 ranks in all: blocks of 16 rows above 256 rows too
         (1000, 2048, [1032], 32, 4),
         (64, 256, [128] * 8, 128, 3),  # eight sections, 1024 ranks
+        # prompts: ranks around the steps of 64, columns around the tiles of 128, more tiles than CTAs
+        (700, 256, [8200], 128, 5),
+        (600, 72, [9000, 3000, 64], 72, 2),
+        (900, 640, [4096, 136], 128, 3),
+        (513, 4096, [2048], 40, 1),
+        (3000, 128, [1000, 24, 5000], 64, 2),
     ],
 )
 def test_matches_the_formula(t, k, sections, r, adapters, dtype):
@@ -148,6 +153,30 @@ def test_scaling_of_zero_and_below():
     args = make(20, 64, [64], 8, 3, BF16, seed=6)
     args[4][:] = torch.tensor([0.0, -1.5, 1.0])
     close(call(args, [64]), *args, [64])
+
+
+@pytest.mark.parametrize("r", [8, 64, 72, 128])
+@pytest.mark.parametrize("order", ["prompts", "decode and prompts", "interleaved", "reversed"])
+def test_where_the_rows_of_a_block_lie(order, r):
+    """Neighbouring rows, few and many rows apart, ragged last quarters, blocks without an adapter; in place and not; the waits' word stays clear."""
+    from emmy_b200 import lib as L
+
+    t, adapters, n = 1111, 7, 4104
+    i = torch.arange(t)
+    ids = {
+        "prompts": i * 5 // t - 1,
+        "decode and prompts": torch.where(i < 60, i * 5 % 8 - 1, (i - 60) * 3 // t * 2),
+        "interleaved": i % 3 - 1,
+        "reversed": 6 - i * 7 // t,
+    }[order]
+    args = make(t, 264, [n], r, adapters, BF16, seed=r, ids=ids)
+    ws = torch.full((L.load().eq_lora_workspace_bytes(t, adapters, 1, r),), 255, dtype=torch.uint8, device="cuda")
+    got = call(args, [n], workspace=ws)
+    L.check(L.load().eq_lora_status(ws.data_ptr(), None))
+    close(got, *args, [n])
+    y = args[0].clone()
+    call([y, *args[1:]], [n], out=y)
+    assert torch.equal(y, got)
 
 
 def test_empty_calls():
