@@ -980,6 +980,7 @@ static int lora_forward(LoraParams p, int64_t T_, int64_t L, unsigned char* base
     const int64_t all_tiles = units * p.tile_ends[p.S - 1];
     p.run = static_cast<int>(all_tiles / (2 * sm_count()) < 1 ? 1 : all_tiles / (2 * sm_count()) > 4 ? 4 : all_tiles / (2 * sm_count()));
     const int64_t runs = ceil_div(all_tiles, p.run);
+    EQ_CUDA_OK(cudaFuncSetAttribute(lora_expand_kernel<T>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     EQ_CUDA_OK(cudaFuncSetAttribute(lora_expand_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lay.smem)));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(runs < sm_count() ? runs : sm_count()));

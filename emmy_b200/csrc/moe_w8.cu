@@ -1,26 +1,34 @@
 // Routed MoE layer of a few tokens on FP8 (e4m3) experts, weights as the checkpoint stores them:
 //     y[t] = sum_j p[t, j] W_down[e] (silu(W_gate[e] x[t]) * (W_up[e] x[t])),  e = id[t, j],
 // id the topk experts of largest router logit (ties to the lowest id), p their softmax, renormalised over the picks.
-// Activations keep their 16 bits (a decode batch is bound by the weights' bytes: quantizing them would cost accuracy and buy nothing);
-// a weight is bits x scale, the scale per output channel or per 128 x 128 block, applied to f32 sums.  The products of a 128-element block of K are
-// summed by mma.sync in f32, the blocks added in f32.  silu(gate) * up is kept as two 16-bit numbers (value and remainder), so that the
-// layer rounds once, as y is stored.
 //
-// Up to 32 tokens and 256 experts, two launches:
+// A weight is bits x scale, the scale per output channel or per 128 x 128 block, applied to f32 sums.  e4m3 is a part of f16, so a weight is expanded
+// to f16 by one conversion a pair, exactly, whatever the activations' type, and these are brought to f16 without loss: a row of bf16 is multiplied by a power of
+// two that takes its largest value to [2^14, 2^15) (its eight bits are exact in f16 down to 2^-31 of that, and off by 2^-39 of it below); a row of silu(gate) * up,
+// in f32, the same way, as two numbers, value and remainder (2^-22 of itself, 2^-39 of the largest).  Products are mma.sync m16n8k16 with f32 sums.  The layer
+// rounds once, as y is stored.  (bf16 MMAs want two conversions and a packing more a pair: 264 instructions per 2 KB of weights where this takes ..., beside the
+// 89 cycles that HBM needs for them; 16 tokens of 128 experts of 2048 x 768 123 us a layer.  m16n8k32 on e4m3 parts of the activations converts both operands
+// inside every MMA: 189 us.)
+//
+// Up to 32 tokens and 256 experts:
 //   gate_up  Every CTA routes the tokens and groups the picks by expert itself: a block is at most eight rows (picks) of one expert, so
 //            an expert that several tokens picked is read once.  The blocks' tiles of eight gate and the same eight up rows (one MMA
-//            A operand of sixteen rows, the block's rows as the N = 8 columns) are one stream, cut into equal spans over the CTAs and
-//            in a CTA into equal shares of 128-element items over its warps.  A tile's silu and product happen in the registers of whoever
-//            has its sums; tiles that several warps share meet in shared memory in warp order.
-//   down     The second launch has routed the tokens and asked for its first weights before the first one ends.  A CTA has sixteen
-//            output channels of ALL the blocks: the picks of a token meet inside it (f32, a fixed order), y is written once, and nothing is
-//            combined across CTAs: no atomics, no counters, no rows in memory.
+//            A operand of sixteen rows) are one stream, cut into equal spans over the CTAs and in a CTA into equal shares of 128-element items over its
+//            warps.  A tile's silu and product happen in the registers of whoever has its sums; tiles that several warps share meet in shared
+//            memory in warp order.
+//   down     A cluster of CTAs has sixteen output channels of ALL the blocks: the picks of a token meet inside it (f32, a fixed order), y is written
+//            once, and nothing is combined in memory: no atomics, no counters.  It has routed the tokens and asked for its first weights before
+//            the launch ahead of it ends.
+// Where the activations are small (kW8Own bytes) each CTA brings them to f16 for itself, and these two launches are the layer; else
+// w8_parts_kernel does it, for x (of bf16) ahead of the first and for silu * up between the two.
 // Above, route + group.cu list the blocks, and both products run as streams of tiles; the down rows go to memory in f32 and
 // moe_w8_combine_kernel adds them.
 //
 // Weights reach a lane through a ring in shared memory that the lane fills by cp.async for itself (16 bytes of a row: K indices 16 j .. 16 j + 15
 // of each half of the item, in both operands alike), so no warp waits for another.  mma.sync and not tcgen05: with at most eight rows the weights'
-// bytes bound the layer; an item of 2 KB is 8 MMAs (17 cycles of an SM's 2.1 each) beside the 89 cycles that HBM needs for it.
+// bytes bound the layer.
+#include <type_traits>
+
 #include "group.cuh"
 #include "mma_sync.cuh"
 
@@ -28,21 +36,25 @@ namespace eq {
 
 constexpr int kW8Threads = 256;
 constexpr int kW8Warps = kW8Threads / 32;
-constexpr int kW8Depth = 5;             // items of a warp's ring
-constexpr int kW8Item = 2048;           // sixteen rows x 128 elements
+// A warp's items are MW x 16 rows x 128 elements, in a ring of w8_depth(MW).
+constexpr int w8_depth(int mw) { return mw == 1 ? 3 : 2; }
+constexpr int w8_ring(int mw) { return w8_depth(mw) * mw * 2048; }
 constexpr int kW8SelfTokens = 32;       // tokens up to which the CTAs route and group themselves (one bit each of a word)
 constexpr int kW8SelfExperts = 256;
 constexpr int kW8MaxTopK = 16;
 constexpr int kW8SelfPicks = kW8SelfTokens * kW8MaxTopK;
 constexpr int kW8BlockRows = 8;
+constexpr int kW8PartsH = 2;            // value and remainder of silu(gate) * up
+constexpr int kW8Own = 32 * 1024;       // bytes of f16 activations that a CTA makes for itself
 
 struct W8Params {
     const uint8_t* w;         // this phase's weights: gate_up [E][2I][H] or down [E][H][I]
     const float* scale;       // [E][2I] / [E][H], or [E][2I / 128][H / 128] / [E][H / 128][I / 128]
     const float* logits;      // [T][E]
     const void* x;            // [T][H]
-    void* hi;                 // [picks][I] silu(gate) * up, value
-    void* lo;                 //            and remainder
+    const __half* parts;      // this phase's activations: [T][H] or [picks][2][I], where the CTAs do not make them
+    const float* part_scale;  // [T] or [picks]: what brings them back; null: nothing does
+    float* h;                 // [picks][I] silu(gate) * up, in expert order
     void* y;                  // [T][H]
     float* rows_out;          // [picks][H], general form
     const GroupBlock* blocks; // general form
@@ -51,6 +63,7 @@ struct W8Params {
     int T, E, topk, H, I;
 };
 
+// ------------------------------------------------------------------------------------------------ routing and grouping
 // The picks in expert order, worked out by a CTA for itself.
 struct W8Plan {
     uint32_t tokens[kW8SelfExperts];      // tokens that picked an expert
@@ -170,40 +183,122 @@ __device__ __forceinline__ void w8_plan(const W8Params& p, W8Plan& plan) {
     __syncthreads();
 }
 
-// Two e4m3 values (the low or the high half of a word) as a pair of the activations' type.
-template <typename T>
-__device__ __forceinline__ uint32_t w8_pair(uint32_t two) {
-    uint32_t h;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(two)));
-    if (std::is_same<T, __half>::value) return h;
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-    const __nv_bfloat162 r = __floats2bfloat162_rn(f.x, f.y);  // exact: e4m3 has four significant bits
-    return *reinterpret_cast<const uint32_t*>(&r);
+// ------------------------------------------------------------------------------------------------ activations in f16
+// The power of two that brings a largest value of `big` to [2^14, 2^15); 1 for zero.
+__device__ __forceinline__ float w8_up(float big) {
+    const int e = static_cast<int>(__float_as_uint(big) >> 23);  // biased; big >= 0
+    return big > 0.f ? __uint_as_float(static_cast<uint32_t>(min(254, 127 + 14 - (e - 127))) << 23) : 1.f;
+}
+// Value and, where P is 2, remainder of two neighbouring values.  What is not finite has no remainder.
+template <int P>
+__device__ __forceinline__ void w8_split(float v0, float v1, uint32_t (&out)[P]) {
+    const __half2 hi = __floats2half2_rn(v0, v1);
+    out[0] = *reinterpret_cast<const uint32_t*>(&hi);
+    if (P == 2) {
+        const float2 back = __half22float2(hi);
+        const __half2 lo = __floats2half2_rn(fabsf(v0) < INFINITY ? v0 - back.x : 0.f, fabsf(v1) < INFINITY ? v1 - back.y : 0.f);
+        out[P - 1] = *reinterpret_cast<const uint32_t*>(&lo);
+    }
+}
+// Four neighbouring values of a row.
+template <typename InT>
+__device__ __forceinline__ float4 w8_load4(const InT* p) {
+    if constexpr (std::is_same<InT, float>::value) {
+        return __ldcg(reinterpret_cast<const float4*>(p));
+    } else {
+        const uint2 raw = __ldcg(reinterpret_cast<const uint2*>(p));
+        const InT* e = reinterpret_cast<const InT*>(&raw);
+        return make_float4(to_float(e[0]), to_float(e[1]), to_float(e[2]), to_float(e[3]));
+    }
+}
+// A row of n values (a multiple of 128) by `threads` threads of which this one is `at`: parts to put(part, index, four f16).  `widest` reduces the
+// threads' largest finite value.  Returns the power of two that brings the parts back.
+template <int P, typename InT, typename Widest, typename Put>
+__device__ __forceinline__ float w8_row_parts(const InT* row, int n, int at, int threads, Widest&& widest, Put&& put) {
+    float big = 0.f;
+    for (int i = 4 * at; i < n; i += 4 * threads) {
+        const float4 v = w8_load4(row + i);
+        const float a[4] = {fabsf(v.x), fabsf(v.y), fabsf(v.z), fabsf(v.w)};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) big = a[q] < INFINITY ? fmaxf(big, a[q]) : big;
+    }
+    const float up = w8_up(widest(big));
+    for (int i = 4 * at; i < n; i += 4 * threads) {
+        const float4 v = w8_load4(row + i);
+        uint32_t first[P], second[P];
+        w8_split<P>(v.x * up, v.y * up, first);
+        w8_split<P>(v.z * up, v.w * up, second);
+#pragma unroll
+        for (int p = 0; p < P; ++p) put(p, i, make_uint2(first[p], second[p]));
+    }
+    return 1.f / up;  // of a power of two: exact
+}
+__device__ __forceinline__ float w8_warp_max(float v) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, off));
+    return v;
 }
 
+// A CTA a row.
+template <int P, typename InT>
+__global__ void __launch_bounds__(kW8Threads) w8_parts_kernel(const InT* __restrict__ rows, int n, __half* __restrict__ parts, float* __restrict__ scale) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // behind the wait: what follows may read this launch's inputs early
+    __shared__ float warps[kW8Warps];
+    auto widest = [&](float v) {
+        v = w8_warp_max(v);
+        if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = v;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kW8Warps; ++w) v = fmaxf(v, warps[w]);
+        return v;
+    };
+    __half* to = parts + static_cast<size_t>(blockIdx.x) * P * n;
+    const float down = w8_row_parts<P>(rows + static_cast<size_t>(blockIdx.x) * n, n, threadIdx.x, kW8Threads, widest,
+                                       [&](int p, int i, uint2 four) { *reinterpret_cast<uint2*>(to + static_cast<size_t>(p) * n + i) = four; });
+    if (threadIdx.x == 0) scale[blockIdx.x] = down;
+}
+
+// ------------------------------------------------------------------------------------------------ the stream of weights
 __device__ __forceinline__ uint4 w8_lds(uint32_t at) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
     return v;
 }
-
-// One item: acc[16 rows][8 columns] += W x over 128 elements.  slot: this lane's first 16 bytes in the ring (top half of the item, rows g; then
-// rows g + 8; then the bottom half's); b: the lane's column at the same K indices, sixteen values a half.
-template <typename T, int SUBS>
-__device__ __forceinline__ void w8_item(uint32_t slot, const uint4 (&b)[SUBS][4], float (&acc)[SUBS][4]) {
+// Two e4m3 values (the low or the high half of a word) in f16.
+__device__ __forceinline__ uint32_t w8_pair(uint32_t two) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(two)));
+    return h;
+}
+// One item: sum[m][16 rows][8 columns] += scale x W x over 128 elements, scale s0 for rows g and s1 for rows g + 8.  slot: this lane's first 16 bytes in the ring
+// (of sixteen rows the first half of the elements, rows g; then rows g + 8; then the other half's); b: the lane's column at the same K indices, sixteen values a
+// half, of every part.
+template <int P, int MW>
+__device__ __forceinline__ void w8_item(uint32_t slot, const uint4 (&b)[P][4], const float (&s0)[MW], const float (&s1)[MW], float (&sum)[MW][4]) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const uint4 top = w8_lds(slot + half * 1024), bottom = w8_lds(slot + half * 1024 + 512);
-        const uint32_t t[4] = {top.x, top.y, top.z, top.w}, u[4] = {bottom.x, bottom.y, bottom.z, bottom.w};
+    for (int m = 0; m < MW; ++m) {
+        float acc[2][4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const uint32_t a0 = w8_pair<T>(t[q] & 0xFFFFu), a2 = w8_pair<T>(t[q] >> 16), a1 = w8_pair<T>(u[q] & 0xFFFFu), a3 = w8_pair<T>(u[q] >> 16);
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int s = 0; s < SUBS; ++s) {
-                const uint4& v = b[s][2 * half + (q >> 1)];
-                mma_16816<T>(acc[s], a0, a1, a2, a3, q & 1 ? v.z : v.x, q & 1 ? v.w : v.y);
+            for (int e = 0; e < 4; ++e) acc[c][e] = 0.f;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const uint4 top = w8_lds(slot + m * 2048 + half * 1024), bottom = w8_lds(slot + m * 2048 + half * 1024 + 512);
+            const uint32_t t[4] = {top.x, top.y, top.z, top.w}, u[4] = {bottom.x, bottom.y, bottom.z, bottom.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t a0 = w8_pair(t[q] & 0xFFFFu), a2 = w8_pair(t[q] >> 16), a1 = w8_pair(u[q] & 0xFFFFu), a3 = w8_pair(u[q] >> 16);
+#pragma unroll
+                for (int p = 0; p < P; ++p) {  // two chains
+                    const uint4& v = b[p][2 * half + (q >> 1)];
+                    mma_16816<__half>(acc[P == 2 ? p : q & 1], a0, a1, a2, a3, q & 1 ? v.z : v.x, q & 1 ? v.w : v.y);
+                }
             }
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[m][e] = fmaf(acc[0][e] + acc[1][e], e < 2 ? s0[m] : s1[m], sum[m][e]);
     }
 }
 
@@ -212,21 +307,25 @@ __device__ __forceinline__ void w8_copy(uint32_t to, const uint8_t* from) {
 }
 __device__ __forceinline__ void w8_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
-// A stream of items of a warp: tiles in order, each `items` items of 128 elements of K.  The owner says where a tile's rows lie for this lane.
+// A warp's stream of items: tiles in order, each `items` items of 128 elements of K.  The owner says where a tile's rows lie for this lane.
 struct W8Ring {
-    uint32_t base, slot;
+    uint32_t base;
     const uint8_t *top, *bottom;  // next item to ask for: this lane's bytes of rows g and g + 8
+    int step;                     // bytes from sixteen rows to the next sixteen
     int left, room;               // items not asked for yet, in all and of the tile
 };
 
-template <typename Open>
+template <int MW, typename Open>
 __device__ __forceinline__ void w8_issue(W8Ring& r, uint32_t slot, int items, Open&& open) {
     if (r.left > 0) {
         const uint32_t to = r.base + slot;
-        w8_copy(to, r.top);
-        w8_copy(to + 512, r.bottom);
-        w8_copy(to + 1024, r.top + 64);
-        w8_copy(to + 1536, r.bottom + 64);
+#pragma unroll
+        for (int m = 0; m < MW; ++m) {
+            w8_copy(to + m * 2048, r.top + m * r.step);
+            w8_copy(to + m * 2048 + 512, r.bottom + m * r.step);
+            w8_copy(to + m * 2048 + 1024, r.top + m * r.step + 64);
+            w8_copy(to + m * 2048 + 1536, r.bottom + m * r.step + 64);
+        }
         r.top += 128;
         r.bottom += 128;
         --r.left;
@@ -237,6 +336,33 @@ __device__ __forceinline__ void w8_issue(W8Ring& r, uint32_t slot, int items, Op
     }
     w8_commit();
 }
+
+// What a lane reads beside the weights, one item ahead: its column at its K indices, the two scales.
+template <int P, int MW>
+struct W8Ahead {
+    uint4 b[P][4];
+    float s0[MW], s1[MW];
+    const __half* col;        // null: none
+    const float *at0, *at1;   // scales; where they are per channel, those of the next sixteen rows `more` further
+    int k, more;              // 128-element block
+
+    // stride: elements between the parts; ONCE: nobody else of the CTA reads them
+    template <bool BLOCK, bool ONCE>
+    __device__ __forceinline__ void fetch(int stride) {
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint4* from = reinterpret_cast<const uint4*>(col + p * stride + k * 128 + (i >> 1) * 64 + (i & 1) * 8);
+                b[p][i] = col ? (ONCE ? __ldcg(from) : *from) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+        for (int m = 0; m < MW; ++m) {  // sixteen rows lie in one block of 128, and so do thirty-two
+            s0[m] = BLOCK && m ? s0[0] : __ldg(at0 + (BLOCK ? k : m * more));
+            s1[m] = BLOCK && m ? s1[0] : __ldg(at1 + (BLOCK ? k : m * more));
+        }
+    }
+};
 
 struct W8Block {
     int expert, row0, count;
@@ -258,22 +384,33 @@ __device__ __forceinline__ W8Block w8_block(const W8Params& p, const W8Plan& pla
     return k;
 }
 
-// ------------------------------------------------------------------------------------------------ spans of whole tiles (gate_up; down, general form)
-template <typename T, bool BLOCK, bool SELF, bool DOWN>
+// ------------------------------------------------------------------------------------------------ spans of whole tiles: gate_up; down, general form
+// OWN: the CTA brings x to f16.
+template <typename T, bool BLOCK, bool SELF, bool DOWN, bool OWN, int MW>
 __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __grid_constant__ W8Params p) {
-    constexpr int kSubs = DOWN ? 2 : 1;  // rows 0 .. 3 and 4 .. 7 of a block, each as value and remainder; or its eight rows as they are
+    constexpr int P = DOWN ? kW8PartsH : 1, kRing = w8_ring(MW), kItem = MW * 2048;
     extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ float own_scale[kW8SelfTokens];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, j = lane & 3;
-    float4* part = reinterpret_cast<float4*>(smem + kW8Warps * kW8Depth * kW8Item);  // [warps][first, last tile][kSubs][32]
-    W8Plan& plan = *reinterpret_cast<W8Plan*>(part + kW8Warps * 2 * kSubs * 32);
+    float4* part = reinterpret_cast<float4*>(smem + kW8Warps * kRing);  // [warps][first, last tile][MW][32]
+    W8Plan& plan = *reinterpret_cast<W8Plan*>(part + kW8Warps * 2 * MW * 32);
+    __half* own = reinterpret_cast<__half*>(reinterpret_cast<unsigned char*>(&plan) + (sizeof(W8Plan) + 15) / 16 * 16);  // [T][K + 8]
 
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // behind the wait: what follows may read this launch's inputs early
-    if (SELF) w8_plan(p, plan);
+    const int K = DOWN ? p.I : p.H, items = K / 128, own_stride = K + 8;
+    if (OWN) {
+        for (int t = warp; t < p.T; t += kW8Warps) {
+            __half* to = own + static_cast<size_t>(t) * P * own_stride;
+            const float down = w8_row_parts<P>(static_cast<const T*>(p.x) + static_cast<size_t>(t) * K, K, lane, 32, w8_warp_max,
+                                               [&](int q, int i, uint2 four) { *reinterpret_cast<uint2*>(to + q * own_stride + i) = four; });
+            if (lane == 0) own_scale[t] = down;
+        }
+    }
+    if (SELF) w8_plan(p, plan);  // ends behind a barrier
     const int n_blocks = SELF ? plan.n_blocks : *p.n_blocks;
-    const int K = DOWN ? p.I : p.H, items = K / 128;
-    const int tiles = DOWN ? p.H / 16 : p.I / 8;  // of a block
+    const int tiles = DOWN ? p.H / (16 * MW) : p.I / (8 * MW);  // of a block
     const int64_t units = static_cast<int64_t>(n_blocks) * tiles;
     const int64_t u0 = units * blockIdx.x / gridDim.x;
     const int span = static_cast<int>(units * (blockIdx.x + 1) / gridDim.x - u0);
@@ -282,101 +419,89 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
     const int64_t q0 = share(warp);
     const int n = static_cast<int>(share(warp + 1) - q0);
     const int first = static_cast<int>(q0 / items), skip = static_cast<int>(q0 - static_cast<int64_t>(first) * items);
+    const int block0 = static_cast<int>(u0 / tiles), tile0 = static_cast<int>(u0 - static_cast<int64_t>(block0) * tiles);
 
-    // tile `rel` of the span: block, channels, this lane's two rows of weights
-    auto block_of = [&](int rel) { return static_cast<int>((u0 + rel) / tiles); };
-    auto rows_of = [&](int rel, int k, const uint8_t*& top, const uint8_t*& bottom, int& expert, int& chan) {
-        const int b = block_of(rel);
-        chan = static_cast<int>(u0 + rel - static_cast<int64_t>(b) * tiles);
-        expert = w8_block<SELF>(p, plan, b).expert;
-        const int rows = DOWN ? p.H : 2 * p.I;
-        const int r0 = DOWN ? chan * 16 + g : chan * 8 + g;
-        top = p.w + (static_cast<size_t>(expert) * rows + r0) * K + k * 128 + 16 * j;
-        bottom = top + static_cast<size_t>(DOWN ? 8 : p.I) * K;
+    // tile `rel` of the span
+    struct Tile {
+        int block, chan;
+    };
+    auto tile_of = [&](int rel) {
+        const int over = (tile0 + rel) / tiles;
+        return Tile{block0 + over, tile0 + rel - over * tiles};
     };
     W8Ring ring;
-    ring.base = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * (kW8Depth * kW8Item) + lane * 16;
+    ring.base = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * kRing + lane * 16;
+    ring.step = (DOWN ? 16 : 8) * K;
     ring.left = n;
-    int ask = first;  // tile of the next item to ask for
-    int unused_e, unused_c;
-    if (n > 0) rows_of(ask, skip, ring.top, ring.bottom, unused_e, unused_c);
     ring.room = items - skip;
+    int ask = first;  // tile of the next item to ask for
+    auto rows_of = [&](int k) {
+        const Tile t = tile_of(ask);
+        const int expert = w8_block<SELF>(p, plan, t.block).expert, rows = DOWN ? p.H : 2 * p.I, r0 = t.chan * MW * (DOWN ? 16 : 8) + g;
+        ring.top = p.w + (static_cast<size_t>(expert) * rows + r0) * K + k * 128 + 16 * j;
+        ring.bottom = ring.top + static_cast<size_t>(DOWN ? 8 : p.I) * K;
+    };
     auto open = [&]() {
         ++ask;
-        rows_of(ask, 0, ring.top, ring.bottom, unused_e, unused_c);
+        rows_of(0);
     };
+    if (n > 0) rows_of(skip);
 #pragma unroll 1
-    for (int d = 0; d < kW8Depth; ++d) w8_issue(ring, d * kW8Item, items, open);
+    for (int d = 0; d < w8_depth(MW); ++d) w8_issue<MW>(ring, d * kItem, items, open);
 
-    // what a lane reads beside the weights, one item ahead: its column of the rows, the block's scales
-    uint4 next[kSubs][4];
-    float next_s0 = 1.f, next_s1 = 1.f;
-    int at = first, k_at = skip;   // the item that `next` holds
-    const T *col[kSubs];           // this lane's column of the tile that `next` is of
-    const float *s0 = nullptr, *s1 = nullptr;
-    auto enter = [&]() {           // a new tile
-        const W8Block blk = w8_block<SELF>(p, plan, block_of(at));
-        const int chan = static_cast<int>(u0 + at - static_cast<int64_t>(block_of(at)) * tiles);
-#pragma unroll
-        for (int s = 0; s < kSubs; ++s) {
+    W8Ahead<P, MW> next;
+    next.more = DOWN ? 16 : 8;
+    int at = first;  // the tile that `next` is of
+    next.k = skip;
+    auto enter = [&]() {
+        const Tile t = tile_of(at);
+        const W8Block blk = w8_block<SELF>(p, plan, t.block);
+        next.col = nullptr;
+        if (g < blk.count) {
             if (DOWN) {
-                const int r = 4 * s + (g & 3);
-                col[s] = r < blk.count ? static_cast<const T*>(g < 4 ? p.hi : p.lo) + static_cast<size_t>(blk.row0 + r) * K + 16 * j : nullptr;
+                next.col = p.parts + static_cast<size_t>(blk.row0 + g) * P * K + 16 * j;
             } else {
-                int token = 0;
-                if (g < blk.count) token = SELF ? plan.token[blk.row0 + g] : p.rows[blk.row0 + g] / p.topk;
-                col[s] = g < blk.count ? static_cast<const T*>(p.x) + static_cast<size_t>(token) * K + 16 * j : nullptr;
+                const int token = SELF ? plan.token[blk.row0 + g] : p.rows[blk.row0 + g] / p.topk;
+                next.col = OWN ? own + static_cast<size_t>(token) * P * own_stride + 16 * j : p.parts + static_cast<size_t>(token) * P * K + 16 * j;
             }
         }
         if (BLOCK) {
             const int rows = (DOWN ? p.H : 2 * p.I) / 128;
-            s0 = p.scale + (static_cast<size_t>(blk.expert) * rows + (DOWN ? chan / 8 : chan / 16)) * items;
-            s1 = DOWN ? s0 : s0 + static_cast<size_t>(p.I / 128) * items;
+            next.at0 = p.scale + (static_cast<size_t>(blk.expert) * rows + (DOWN ? t.chan * MW / 8 : t.chan * MW / 16)) * items;
+            next.at1 = DOWN ? next.at0 : next.at0 + static_cast<size_t>(p.I / 128) * items;
         } else {
-            s0 = p.scale + static_cast<size_t>(blk.expert) * (DOWN ? p.H : 2 * p.I) + (DOWN ? chan * 16 + g : chan * 8 + g);
-            s1 = s0 + (DOWN ? 8 : p.I);
+            next.at0 = p.scale + static_cast<size_t>(blk.expert) * (DOWN ? p.H : 2 * p.I) + t.chan * MW * (DOWN ? 16 : 8) + g;
+            next.at1 = next.at0 + (DOWN ? 8 : p.I);
         }
     };
     auto fetch = [&]() {
-#pragma unroll
-        for (int s = 0; s < kSubs; ++s)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                next[s][i] = col[s] ? (DOWN ? __ldcg(reinterpret_cast<const uint4*>(col[s] + k_at * 128 + (i >> 1) * 64 + (i & 1) * 8)) : *reinterpret_cast<const uint4*>(col[s] + k_at * 128 + (i >> 1) * 64 + (i & 1) * 8)) : make_uint4(0, 0, 0, 0);
-        if (BLOCK) {
-            next_s0 = __ldg(s0 + k_at);
-            next_s1 = __ldg(s1 + k_at);
-        } else {
-            next_s0 = __ldg(s0);
-            next_s1 = __ldg(s1);
-        }
+        next.template fetch<BLOCK, DOWN>(OWN ? own_stride : K);
     };
-    // the finished sums of a tile (lane: channels g and g + 8, or gate and up of channel g; columns 2 j, 2 j + 1)
-    auto finish = [&](int rel, float (&sum)[kSubs][4]) {
-        const int b = block_of(rel);
-        const W8Block blk = w8_block<SELF>(p, plan, b);
-        const int chan = static_cast<int>(u0 + rel - static_cast<int64_t>(b) * tiles);
-        if (!DOWN) {
+    // the finished sums of a tile (lane: channels g and g + 8, or gate and up of channel g; rows 2 j, 2 j + 1)
+    auto finish = [&](int rel, const float (&sum)[MW][4]) {
+        const Tile t = tile_of(rel);
+        const W8Block blk = w8_block<SELF>(p, plan, t.block);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int r = 2 * j + i;
-                if (r >= blk.count) continue;
-                const float gate = sum[0][i], up = sum[0][2 + i];
-                T hi, lo;
-                split16<T>(gate / (1.f + expf(-gate)) * up, hi, lo);
-                const size_t to = static_cast<size_t>(blk.row0 + r) * p.I + chan * 8 + g;
-                static_cast<T*>(p.hi)[to] = hi;
-                static_cast<T*>(p.lo)[to] = lo;
-            }
-        } else {
+        for (int i = 0; i < 2; ++i) {
+            const int r = 2 * j + i;
+            if (r >= blk.count) continue;
+            if (DOWN) {
+                const float down = __ldcg(p.part_scale + blk.row0 + r);
+                float* to = p.rows_out + static_cast<size_t>(p.rows[blk.row0 + r]) * p.H + t.chan * 16 * MW + g;
 #pragma unroll
-            for (int s = 0; s < kSubs; ++s)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float v = sum[s][i] + __shfl_xor_sync(0xFFFFFFFFu, sum[s][i], 2);  // value + remainder: columns r and r + 4
-                    const int r = 4 * s + 2 * j + (i & 1);
-                    if (j < 2 && r < blk.count) p.rows_out[static_cast<size_t>(p.rows[blk.row0 + r]) * p.H + chan * 16 + g + 8 * (i >> 1)] = v;
+                for (int m = 0; m < MW; ++m) {
+                    to[16 * m] = sum[m][i] * down;
+                    to[16 * m + 8] = sum[m][2 + i] * down;
                 }
+            } else {
+                const int token = SELF ? plan.token[blk.row0 + r] : p.rows[blk.row0 + r] / p.topk;
+                const float down = OWN ? own_scale[token] : p.part_scale ? __ldcg(p.part_scale + token) : 1.f;
+#pragma unroll
+                for (int m = 0; m < MW; ++m) {
+                    const float gate = sum[m][i] * down, up = sum[m][2 + i] * down;
+                    p.h[static_cast<size_t>(blk.row0 + r) * p.I + (t.chan * MW + m) * 8 + g] = gate / (1.f + expf(-gate)) * up;
+                }
+            }
         }
     };
 
@@ -384,53 +509,31 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
         enter();
         fetch();
     }
-    int slot = 0;
+    uint32_t slot = 0;
     int rel = first, it = skip;
     for (int i = 0; i < n;) {
         const int stretch = min(items - it, n - i);
-        float sum[kSubs][4];
-#pragma unroll
-        for (int s = 0; s < kSubs; ++s)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum[s][e] = 0.f;
+        float sum[MW][4] = {};
         for (int c = 0; c < stretch; ++c) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kW8Depth - 1) : "memory");
-            uint4 now[kSubs][4];
-#pragma unroll
-            for (int s = 0; s < kSubs; ++s)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) now[s][e] = next[s][e];
-            const float f0 = next_s0, f1 = next_s1;
+            asm volatile("cp.async.wait_group %0;" ::"n"(w8_depth(MW) - 1) : "memory");
+            const W8Ahead<P, MW> now = next;
             if (i + c + 1 < n) {
-                if (++k_at == items) {
-                    k_at = 0;
+                if (++next.k == items) {
+                    next.k = 0;
                     ++at;
                     enter();
                 }
                 fetch();
             }
-            float acc[kSubs][4];
-#pragma unroll
-            for (int s = 0; s < kSubs; ++s)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[s][e] = 0.f;
-            w8_item<T, kSubs>(ring.base + slot, now, acc);
-            w8_issue(ring, slot, items, open);
-            slot = slot + kW8Item == kW8Depth * kW8Item ? 0 : slot + kW8Item;
-#pragma unroll
-            for (int s = 0; s < kSubs; ++s) {
-                sum[s][0] = fmaf(acc[s][0], f0, sum[s][0]);
-                sum[s][1] = fmaf(acc[s][1], f0, sum[s][1]);
-                sum[s][2] = fmaf(acc[s][2], f1, sum[s][2]);
-                sum[s][3] = fmaf(acc[s][3], f1, sum[s][3]);
-            }
+            w8_item<P, MW>(ring.base + slot, now.b, now.s0, now.s1, sum);
+            w8_issue<MW>(ring, slot, items, open);
+            slot = slot + kItem == kRing ? 0 : slot + kItem;
         }
         if (stretch == items) {
             finish(rel, sum);
-        } else {  // a tile that another warp has a part of
+        } else {  // another warp has a part of the tile
 #pragma unroll
-            for (int s = 0; s < kSubs; ++s)
-                part[((warp * 2 + (rel == first ? 0 : 1)) * kSubs + s) * 32 + lane] = make_float4(sum[s][0], sum[s][1], sum[s][2], sum[s][3]);
+            for (int m = 0; m < MW; ++m) part[((warp * 2 + (rel == first ? 0 : 1)) * MW + m) * 32 + lane] = make_float4(sum[m][0], sum[m][1], sum[m][2], sum[m][3]);
         }
         i += stretch;
         it = 0;
@@ -440,54 +543,58 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
     // the shared tiles, in the order of the warps that have a part
     for (int t = warp; t < span; t += kW8Warps) {
         const int64_t lo_item = static_cast<int64_t>(t) * items, hi_item = lo_item + items;
-        float sum[kSubs][4];
-#pragma unroll
-        for (int s = 0; s < kSubs; ++s)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum[s][e] = 0.f;
+        float sum[MW][4] = {};
         int parts = 0;
-        bool whole = false;
         for (int w = 0; w < kW8Warps; ++w) {
             const int64_t a = share(w), b = share(w + 1);
-            if (a >= hi_item || b <= lo_item || a == b) continue;
-            if (a <= lo_item && b >= hi_item) {
-                whole = true;
-                break;
-            }
+            if (a >= hi_item || b <= lo_item || a == b || (a <= lo_item && b >= hi_item)) continue;
             ++parts;
-            const int which = static_cast<int>(a / items) == t ? 0 : 1;
 #pragma unroll
-            for (int s = 0; s < kSubs; ++s) {
-                const float4 v = part[((w * 2 + which) * kSubs + s) * 32 + lane];
-                sum[s][0] += v.x;
-                sum[s][1] += v.y;
-                sum[s][2] += v.z;
-                sum[s][3] += v.w;
+            for (int m = 0; m < MW; ++m) {
+                const float4 v = part[((w * 2 + (static_cast<int>(a / items) == t ? 0 : 1)) * MW + m) * 32 + lane];
+                sum[m][0] += v.x;
+                sum[m][1] += v.y;
+                sum[m][2] += v.z;
+                sum[m][3] += v.w;
             }
         }
-        if (!whole && parts) finish(t, sum);
+        if (parts) finish(t, sum);
     }
 }
 
 // ------------------------------------------------------------------------------------------------ down, sixteen channels of all blocks
-template <typename T, bool BLOCK>
+__device__ __forceinline__ float w8_peer(const float* mine, uint32_t rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(mine))), "r"(rank));
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+
+template <typename T, bool BLOCK, bool OWN, int MW>
 __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid_constant__ W8Params p) {
+    constexpr int P = kW8PartsH, kRing = w8_ring(MW), kItem = MW * 2048, kChan = 16 * MW;
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, j = lane & 3;
-    float* sums = reinterpret_cast<float*>(smem + kW8Warps * kW8Depth * kW8Item);  // [warps][T][16]
-    W8Plan& plan = *reinterpret_cast<W8Plan*>(sums + kW8Warps * p.T * 16);
-    // The launch before this one waited for what came before it ahead of letting this one start, so the logits may be read here and the
-    // weights asked for; what it computes is read behind the wait.
+    float* sums = reinterpret_cast<float*>(smem + kW8Warps * kRing);  // [warps][T][kChan]
+    W8Plan& plan = *reinterpret_cast<W8Plan*>(sums + kW8Warps * p.T * kChan);
+    __half* own = reinterpret_cast<__half*>(reinterpret_cast<unsigned char*>(&plan) + (sizeof(W8Plan) + 15) / 16 * 16);  // [picks][P][I + 8]
+    uint32_t rank, ctas;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
+    // The launches before this one each waited for what came before them ahead of letting the next start, so the logits may be read here and the
+    // weights asked for; what they compute is read behind the wait.
     w8_plan(p, plan);
-    for (int i = tid; i < kW8Warps * p.T * 16; i += kW8Threads) sums[i] = 0.f;
+    for (int i = tid; i < kW8Warps * p.T * kChan; i += kW8Threads) sums[i] = 0.f;
     __syncthreads();
-    const int items = p.I / 128, chan = blockIdx.x * 16;
-    const int total = plan.n_blocks * items;
-    const int q0 = total * warp / kW8Warps, n = total * (warp + 1) / kW8Warps - q0;
+    const int items = p.I / 128, chan = static_cast<int>(blockIdx.x / ctas) * kChan, own_stride = p.I + 8;
+    const int total = plan.n_blocks * items, shares = kW8Warps * ctas, mine = rank * kW8Warps + warp;
+    const int q0 = static_cast<int>(static_cast<int64_t>(total) * mine / shares), n = static_cast<int>(static_cast<int64_t>(total) * (mine + 1) / shares) - q0;
     const int first = q0 / items, skip = q0 - first * items;
     W8Ring ring;
-    ring.base = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * (kW8Depth * kW8Item) + lane * 16;
+    ring.base = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * kRing + lane * 16;
+    ring.step = 16 * p.I;
     ring.left = n;
     ring.room = items - skip;
     int ask = first;
@@ -498,104 +605,112 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
     if (n > 0) rows_of(ask, skip);
     auto open = [&]() { rows_of(++ask, 0); };
 #pragma unroll 1
-    for (int d = 0; d < kW8Depth; ++d) w8_issue(ring, d * kW8Item, items, open);
+    for (int d = 0; d < w8_depth(MW); ++d) w8_issue<MW>(ring, d * kItem, items, open);
 
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    uint4 next[2][4];
-    float next_s0 = 1.f, next_s1 = 1.f;
-    int at = first, k_at = skip;
-    const T* col[2];
-    const float *s0 = nullptr, *s1 = nullptr;
-    auto enter = [&]() {
-        const int row0 = plan.row0[at], count = plan.count[at], expert = plan.expert[at];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const int r = 4 * s + (g & 3);
-            col[s] = r < count ? static_cast<const T*>(g < 4 ? p.hi : p.lo) + static_cast<size_t>(row0 + r) * p.I + 16 * j : nullptr;
+    if (OWN) {
+        // (a row's factor goes to its weight in the token's sum)
+        const int picks = plan.row0[plan.n_blocks - 1] + plan.count[plan.n_blocks - 1];
+        for (int r = warp; r < picks; r += kW8Warps) {
+            __half* to = own + static_cast<size_t>(r) * P * own_stride;
+            const float down = w8_row_parts<P>(p.h + static_cast<size_t>(r) * p.I, p.I, lane, 32, w8_warp_max,
+                                               [&](int q, int i, uint2 four) { *reinterpret_cast<uint2*>(to + q * own_stride + i) = four; });
+            if (lane == 0) plan.score[r] *= down;
         }
+        __syncthreads();
+    }
+    W8Ahead<P, MW> next;
+    next.more = 16;
+    int at = first;
+    next.k = skip;
+    auto enter = [&]() {
+        const int row0 = plan.row0[at], expert = plan.expert[at];
+        next.col = nullptr;
+        if (g < plan.count[at]) next.col = OWN ? own + static_cast<size_t>(row0 + g) * P * own_stride + 16 * j : p.parts + static_cast<size_t>(row0 + g) * P * p.I + 16 * j;
         if (BLOCK) {
-            s0 = s1 = p.scale + (static_cast<size_t>(expert) * (p.H / 128) + chan / 128) * items;
+            next.at0 = next.at1 = p.scale + (static_cast<size_t>(expert) * (p.H / 128) + chan / 128) * items;
         } else {
-            s0 = p.scale + static_cast<size_t>(expert) * p.H + chan + g;
-            s1 = s0 + 8;
+            next.at0 = p.scale + static_cast<size_t>(expert) * p.H + chan + g;
+            next.at1 = next.at0 + 8;
         }
     };
     auto fetch = [&]() {
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                next[s][i] = col[s] ? __ldcg(reinterpret_cast<const uint4*>(col[s] + k_at * 128 + (i >> 1) * 64 + (i & 1) * 8)) : make_uint4(0, 0, 0, 0);
-        next_s0 = __ldg(BLOCK ? s0 + k_at : s0);
-        next_s1 = __ldg(BLOCK ? s1 + k_at : s1);
+        next.template fetch<BLOCK, !OWN>(OWN ? own_stride : p.I);
     };
     if (n > 0) {
         enter();
         fetch();
     }
-    float* mine = sums + warp * p.T * 16;
-    int slot = 0, rel = first, it = skip;
+    float* my_sums = sums + warp * p.T * kChan;
+    uint32_t slot = 0;
+    int rel = first, it = skip;
     for (int i = 0; i < n;) {
         const int stretch = min(items - it, n - i);
-        float sum[2][4];
+        const int row0 = plan.row0[rel], count = plan.count[rel];
+        float down[2] = {1.f, 1.f};
+        if (!OWN) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum[s][e] = 0.f;
+            for (int e = 0; e < 2; ++e)
+                if (2 * j + e < count) down[e] = __ldcg(p.part_scale + row0 + 2 * j + e);
+        }
+        float sum[MW][4] = {};
         for (int c = 0; c < stretch; ++c) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kW8Depth - 1) : "memory");
-            uint4 now[2][4];
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) now[s][e] = next[s][e];
-            const float f0 = next_s0, f1 = next_s1;
+            asm volatile("cp.async.wait_group %0;" ::"n"(w8_depth(MW) - 1) : "memory");
+            const W8Ahead<P, MW> now = next;
             if (i + c + 1 < n) {
-                if (++k_at == items) {
-                    k_at = 0;
+                if (++next.k == items) {
+                    next.k = 0;
                     ++at;
                     enter();
                 }
                 fetch();
             }
-            float acc[2][4];
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[s][e] = 0.f;
-            w8_item<T, 2>(ring.base + slot, now, acc);
-            w8_issue(ring, slot, items, open);
-            slot = slot + kW8Item == kW8Depth * kW8Item ? 0 : slot + kW8Item;
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                sum[s][0] = fmaf(acc[s][0], f0, sum[s][0]);
-                sum[s][1] = fmaf(acc[s][1], f0, sum[s][1]);
-                sum[s][2] = fmaf(acc[s][2], f1, sum[s][2]);
-                sum[s][3] = fmaf(acc[s][3], f1, sum[s][3]);
-            }
+            w8_item<P, MW>(ring.base + slot, now.b, now.s0, now.s1, sum);
+            w8_issue<MW>(ring, slot, items, open);
+            slot = slot + kItem == kRing ? 0 : slot + kItem;
         }
         // this warp's part of the block's rows, weighted, to its tokens' sums (the rows of a block are different tokens)
-        const int row0 = plan.row0[rel], count = plan.count[rel];
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int e = 0; e < 2; ++e) {
+            const int r = 2 * j + e;
+            if (r < count) {
+                const float weight = plan.score[row0 + r] * down[e];
+                float* to = my_sums + plan.token[row0 + r] * kChan + g;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float v = sum[s][e] + __shfl_xor_sync(0xFFFFFFFFu, sum[s][e], 2);
-                const int r = 4 * s + 2 * j + (e & 1);
-                if (j < 2 && r < count) mine[plan.token[row0 + r] * 16 + g + 8 * (e >> 1)] += plan.score[row0 + r] * v;
+                for (int m = 0; m < MW; ++m) {
+                    to[16 * m] += weight * sum[m][e];
+                    to[16 * m + 8] += weight * sum[m][2 + e];
+                }
             }
+        }
         __syncwarp();
         i += stretch;
         it = 0;
         ++rel;
     }
     __syncthreads();
-    for (int i = tid; i < p.T * 16; i += kW8Threads) {
+    // the warps' sums in warp order, the CTAs' in rank order
+    for (int i = tid; i < p.T * kChan; i += kW8Threads) {
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < kW8Warps; ++w) v += sums[w * p.T * 16 + i];
-        static_cast<T*>(p.y)[static_cast<size_t>(i >> 4) * p.H + chan + (i & 15)] = from_float<T>(v);
+        for (int w = 0; w < kW8Warps; ++w) v += sums[w * p.T * kChan + i];
+        sums[i] = v;
+    }
+    if (ctas > 1) {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else {
+        __syncthreads();
+    }
+    for (int i = rank * kW8Threads + tid; i < p.T * kChan; i += ctas * kW8Threads) {
+        float v = 0.f;
+        for (uint32_t c = 0; c < ctas; ++c) v += ctas > 1 ? w8_peer(sums + i, c) : sums[i];
+        static_cast<T*>(p.y)[static_cast<size_t>(i / kChan) * p.H + chan + i % kChan] = from_float<T>(v);
+    }
+    if (ctas > 1) {  // no CTA leaves while another may read its sums
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
 }
 
@@ -628,9 +743,9 @@ __global__ void __launch_bounds__(256) moe_w8_combine_kernel(const float4* __res
 static size_t w8_align(size_t v) { return (v + 255) / 256 * 256; }
 
 struct W8Workspace {
-    void *hi, *lo;
+    __half *x_parts, *h_parts;
+    float *x_scale, *h_scale, *h, *scores, *rows_out;
     int32_t *ids, *rows, *n_blocks;
-    float *scores, *rows_out;
     GroupBlock* blocks;
     size_t bytes;
 };
@@ -646,77 +761,99 @@ static W8Workspace w8_carve(void* base, int64_t T, int64_t E, int64_t topk, int6
         o += w8_align(bytes);
         return at;
     };
-    const int64_t R = T * topk;
-    w.hi = take(static_cast<size_t>(R) * I * 2);
-    w.lo = take(static_cast<size_t>(R) * I * 2);
+    const size_t R = static_cast<size_t>(T) * topk;
+    w.h = static_cast<float*>(take(R * I * 4));
+    w.x_parts = static_cast<__half*>(take(static_cast<size_t>(T) * H * 2));
+    w.x_scale = static_cast<float*>(take(static_cast<size_t>(T) * 4));
+    w.h_parts = static_cast<__half*>(take(R * kW8PartsH * I * 2));
+    w.h_scale = static_cast<float*>(take(R * 4));
     if (!w8_self(T, E)) {
         w.ids = static_cast<int32_t*>(take(R * 4));
         w.scores = static_cast<float*>(take(R * 4));
         w.rows = static_cast<int32_t*>(take(R * 4));
         w.n_blocks = static_cast<int32_t*>(take(4));
-        w.blocks = static_cast<GroupBlock*>(take(static_cast<size_t>(group_max_blocks(R, E, kW8BlockRows, false)) * sizeof(GroupBlock)));
-        w.rows_out = static_cast<float*>(take(static_cast<size_t>(R) * H * 4));
+        w.blocks = static_cast<GroupBlock*>(take(static_cast<size_t>(group_max_blocks(static_cast<int64_t>(R), E, kW8BlockRows, false)) * sizeof(GroupBlock)));
+        w.rows_out = static_cast<float*>(take(R * H * 4));
     }
     w.bytes = o;
     return w;
 }
 
-template <typename Kernel, typename... A>
-static int w8_launch(Kernel kernel, int64_t grid, size_t smem, cudaStream_t stream, A... args) {
-    EQ_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 * 1024));
+template <typename... P, typename... A>
+static int w8_launch(void (*kernel)(P...), int64_t grid, int cluster, size_t smem, cudaStream_t stream, A... args) {
+    if (smem > 48 * 1024) EQ_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(grid));
     cfg.blockDim = dim3(kW8Threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    EQ_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, args...));
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    EQ_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
     return EQ_OK;
 }
 
 template <typename T, bool BLOCK>
 static int w8_forward(W8Params p, const uint8_t* gate_up, const float* gate_up_scale, const uint8_t* down, const float* down_scale, const W8Workspace& w,
                       cudaStream_t stream) {
-    const size_t ring = static_cast<size_t>(kW8Warps) * kW8Depth * kW8Item;
-    const size_t part = kW8Warps * 2 * 32 * sizeof(float4);
+    const size_t plan = (sizeof(W8Plan) + 15) / 16 * 16;
+    const int64_t R = static_cast<int64_t>(p.T) * p.topk;
+    const bool self = w8_self(p.T, p.E);
+    const int64_t own_x = static_cast<int64_t>(p.T) * (p.H + 8) * 2, own_h = R * kW8PartsH * (p.I + 8) * 2;
+    constexpr bool f16 = std::is_same<T, __half>::value;  // x is read as it is
+    const bool x_own = self && !f16 && own_x <= kW8Own, h_own = self && own_h <= kW8Own && R * (p.I / 16) < 8 * 2 * sm_count();
+    int st = EQ_OK;
+    if constexpr (!f16) {
+        if (!x_own) st = w8_launch(w8_parts_kernel<1, T>, p.T, 1, 0, stream, static_cast<const T*>(p.x), p.H, w.x_parts, w.x_scale);
+    }
+    if (st == EQ_OK && !self) st = eq_moe_route(p.logits, p.T, p.E, p.topk, 1, w.ids, w.scores, stream);
+    if (st == EQ_OK && !self) st = group_rows_launch(w.ids, static_cast<int>(R), p.E, false, kW8BlockRows, false, w.blocks, w.n_blocks, w.rows, nullptr, stream);
+    if (st != EQ_OK) return st;
     p.w = gate_up;
     p.scale = gate_up_scale;
-    const int64_t R = static_cast<int64_t>(p.T) * p.topk;
-    if (w8_self(p.T, p.E)) {
-        const int64_t tiles = R * (p.I / 8);
-        int st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false>, tiles < sm_count() ? tiles : sm_count(), ring + part + sizeof(W8Plan), stream, p);
-        if (st != EQ_OK) return st;
-        p.w = down;
-        p.scale = down_scale;
-        return w8_launch(moe_w8_down_kernel<T, BLOCK>, p.H / 16, ring + static_cast<size_t>(kW8Warps) * p.T * 16 * sizeof(float) + sizeof(W8Plan), stream, p);
+    p.parts = f16 ? static_cast<const __half*>(p.x) : w.x_parts;
+    p.part_scale = f16 ? nullptr : w.x_scale;
+    const int64_t sms = sm_count(), most = 2 * sms;
+    auto smem = [&](int mw) { return static_cast<size_t>(kW8Warps) * (w8_ring(mw) + 2 * mw * 32 * sizeof(float4)); };
+    // Thirty-two rows a warp where there are enough of them: half as many reads of the activations, which lie in L1 and L2, for the same weights.
+    const bool wide = R * (p.I / 16) >= 8 * most;
+    if (self) {
+        const int64_t tiles = R * (p.I / (wide ? 16 : 8)), grid = tiles < most ? tiles : most;
+        if (x_own) st = wide ? w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, !f16, 2>, grid, 1, smem(2) + plan + own_x, stream, p)
+                             : w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, !f16, 1>, grid, 1, smem(1) + plan + own_x, stream, p);
+        else st = wide ? w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, false, 2>, grid, 1, smem(2) + plan, stream, p)
+                       : w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, false, 1>, grid, 1, smem(1) + plan, stream, p);
+    } else {
+        st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, false, false, false, 2>, most, 1, smem(2), stream, p);
     }
-    int st = eq_moe_route(p.logits, p.T, p.E, p.topk, 1, w.ids, w.scores, stream);
-    if (st != EQ_OK) return st;
-    st = group_rows_launch(w.ids, static_cast<int>(R), p.E, false, kW8BlockRows, false, w.blocks, w.n_blocks, w.rows, nullptr, stream);
-    if (st != EQ_OK) return st;
-    st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, false, false>, 2 * sm_count(), ring + part, stream, p);
     if (st != EQ_OK) return st;
     p.w = down;
     p.scale = down_scale;
-    st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, false, true>, 2 * sm_count(), ring + 2 * part, stream, p);
+    p.parts = w.h_parts;
+    p.part_scale = w.h_scale;
+    if (!h_own) st = w8_launch(w8_parts_kernel<kW8PartsH, float>, R, 1, 0, stream, static_cast<const float*>(w.h), p.I, w.h_parts, w.h_scale);
+    if (st != EQ_OK) return st;
+    if (self) {
+        const int mw = wide ? 2 : 1;
+        const int64_t slabs = p.H / (16 * mw);
+        int cluster = 8;  // two CTAs an SM at most
+        while (cluster > 1 && slabs * cluster > most) cluster /= 2;
+        const size_t bytes = static_cast<size_t>(kW8Warps) * (w8_ring(mw) + static_cast<size_t>(p.T) * 16 * mw * sizeof(float)) + plan;
+        if (wide) return w8_launch(moe_w8_down_kernel<T, BLOCK, false, 2>, slabs * cluster, cluster, bytes, stream, p);
+        return h_own ? w8_launch(moe_w8_down_kernel<T, BLOCK, true, 1>, slabs * cluster, cluster, bytes + own_h, stream, p)
+                     : w8_launch(moe_w8_down_kernel<T, BLOCK, false, 1>, slabs * cluster, cluster, bytes, stream, p);
+    }
+    st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, false, true, false, 2>, most, 1, smem(2), stream, p);
     if (st != EQ_OK) return st;
     const int64_t vecs = static_cast<int64_t>(p.T) * p.H / 4;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(ceil_div(vecs, 256)));
-    cfg.blockDim = dim3(256);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    EQ_CUDA_OK(cudaLaunchKernelEx(&cfg, moe_w8_combine_kernel<T>, reinterpret_cast<const float4*>(w.rows_out), static_cast<const float*>(w.scores), vecs, p.H / 4, p.topk,
-                                  static_cast<T*>(p.y)));
-    return EQ_OK;
+    return w8_launch(moe_w8_combine_kernel<T>, ceil_div(vecs, 256), 1, 0, stream, reinterpret_cast<const float4*>(w.rows_out), static_cast<const float*>(w.scores), vecs, p.H / 4,
+                     p.topk, static_cast<T*>(p.y));
 }
 
 }  // namespace eq
@@ -750,8 +887,7 @@ extern "C" int eq_moe_w8a16(const uint8_t* gate_up, const float* gate_up_scale, 
     W8Params p = {};
     p.logits = router_logits;
     p.x = x;
-    p.hi = w.hi;
-    p.lo = w.lo;
+    p.h = w.h;
     p.y = y;
     p.rows_out = w.rows_out;
     p.blocks = w.blocks;

@@ -1,10 +1,12 @@
 """The routed layer of a few tokens on FP8 experts, on the GPU against the formula in 64 bits.
 
 Tolerance of one value, from the arithmetic.  A chain of MMA steps of sixteen products is off by at most a step of the largest partial sum each
-(2^-23 of the sum of magnitudes), the scales and the joins of the warps' sums add a few steps of the same size: c = (K / 16 + K / 128 + 32) 2^-23.  With
-G = sum |w x| of gate and U of up, gate is off by c G and up by c U; silu has a slope below 1.1, so h = silu(gate) up is off by
-1.1 c G |up| + |silu(gate)| c U, by the exponential, the division and the product (8 x 2^-24 of it) and by its two-part form (2^-18 of it in bf16, 2^-22 in
-f16).  y adds p |W_down| of that, its own chains, 16 x 2^-24 for the shares, and half a step of its dtype for the one rounding."""
+(2^-23 of the sum of magnitudes), the scales and the joins of the warps' sums add a few steps of the same size: c = (K / 16 + K / 128 + 32) 2^-23.
+A row whose largest value is V enters a product in f16 after a power of two has taken V to 2^14 or more: its 8 or 11 bits are exact unless they reach below
+f16's smallest step, 2^-24, half of which is 2^-39 V; h enters as value + remainder, off by 2^-22 of itself or that.  With G = sum |w x| of gate and U of up, and W
+the sums of |w|, gate is off by dg = c G + 2^-39 X W and up by du alike; silu has a slope below 1.1, so h = silu(gate) up is off by 1.1 dg |up| + |silu(gate)| du,
+by the exponential, the division and the product (8 x 2^-24 of it) and by its two parts.  y adds p |W_down| of that, its own chains, 16 x 2^-24 for the shares, and
+half a step of its dtype for the one rounding.  (A row of f16 is read as it is: its own subnormals are its own.)"""
 
 import pytest
 import torch
@@ -51,15 +53,16 @@ def formula(x, logits, values, topk):
     ids, shares = routed(logits, topk)
     xd, (t, h), i = x.double(), x.shape, dnv.shape[2]
     ch, ci = (h / 16 + h / 128 + 32) * 2.0**-23, (i / 16 + i / 128 + topk + 32) * 2.0**-23
-    part = 2.0**-18 if x.dtype == BF16 else 2.0**-22
     y, limit = torch.zeros(t, h, dtype=torch.float64, device="cuda"), torch.zeros(t, h, dtype=torch.float64, device="cuda")
     for e in ids.unique().tolist():
         rows, slot = (ids == e).nonzero(as_tuple=True)
         gate, up = (xd[rows] @ guv[e].T).chunk(2, 1)
         sg, su = (xd[rows].abs() @ guv[e].abs().T).chunk(2, 1)
+        wg, wu = (xd[rows].abs().amax(1, keepdim=True) * guv[e].abs().sum(1)).chunk(2, 1)
+        dg, du = ch * sg + 2.0**-39 * wg, ch * su + 2.0**-39 * wu
         silu = gate * torch.sigmoid(gate)
         act = silu * up
-        off = 1.1 * ch * sg * up.abs() + silu.abs() * ch * su + act.abs() * (part + 8 * 2.0**-24) + (2.0**-25 if x.dtype == F16 else 0)
+        off = 1.1 * dg * up.abs() + silu.abs() * du + act.abs() * (2.0**-22 + 8 * 2.0**-24) + 2.0**-39 * act.abs().amax(1, keepdim=True)
         p = shares[rows, slot][:, None]
         y[rows] += p * (act @ dnv[e].T)
         limit[rows] += p * (off @ dnv[e].abs().T + (ci + 16 * 2.0**-24) * (act.abs() @ dnv[e].abs().T))
@@ -168,6 +171,35 @@ def test_tokens_do_not_reach_one_another():
         rest = torch.ones(t, dtype=torch.bool, device="cuda")
         rest[[3, 7]] = False
         assert torch.equal(got[rest], want[rest]) and got[3].isnan().all() and not torch.isfinite(got[7]).any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("t", [1, 3, 20, 40])
+def test_rows_of_every_size(t, dtype):
+    """Rows of zeros, of one value, of very large and very small ones, of a few outliers beside small values; h beyond f16's range."""
+    e, topk, h, i = 16, 4, 512, 256
+    w, values = experts(e, h, i, True, seed=13)
+    for seed in range(3):
+        x, logits = inputs(t, e, h, dtype, seed=seed)
+        top = 2.0**14 if dtype == F16 else 2.0**60
+        for r in range(t):
+            kind = (r + seed) % 6
+            if kind == 0:
+                x[r] = 0
+            elif kind == 1:
+                x[r, 1:] = 0
+            elif kind == 2:
+                x[r] = (x[r].float() * (2.0**9 if dtype == F16 else 2.0**20)).to(dtype)
+            elif kind == 3:
+                x[r] = (x[r].float() * 2.0**-14).to(dtype)
+            elif kind == 4:
+                x[r, ::100] *= 2.0**8
+            else:
+                x[r, 7] = 2.0**12
+        w_small = (w[0], w[1], w[2], w[3] * 2.0**-30) if dtype == F16 else w
+        v_small = (values[0], values[1] * 2.0**-30) if dtype == F16 else values
+        assert x.abs().max() <= top
+        close(call(x, logits, w_small, topk), x, logits, v_small, topk)
 
 
 def test_every_weight_code_and_wide_scales():
