@@ -211,32 +211,61 @@ __device__ __forceinline__ float4 w8_load4(const InT* p) {
         return make_float4(to_float(e[0]), to_float(e[1]), to_float(e[2]), to_float(e[3]));
     }
 }
-// A row of n values (a multiple of 128) by `threads` threads of which this one is `at`: parts to put(part, index, four f16).  `widest` reduces the
-// threads' largest finite value.  Returns the power of two that brings the parts back.
-template <int P, typename InT, typename Widest, typename Put>
-__device__ __forceinline__ float w8_row_parts(const InT* row, int n, int at, int threads, Widest&& widest, Put&& put) {
-    float big = 0.f;
-    for (int i = 4 * at; i < n; i += 4 * threads) {
-        const float4 v = w8_load4(row + i);
-        const float a[4] = {fabsf(v.x), fabsf(v.y), fabsf(v.z), fabsf(v.w)};
-#pragma unroll
-        for (int q = 0; q < 4; ++q) big = a[q] < INFINITY ? fmaxf(big, a[q]) : big;
-    }
-    const float up = w8_up(widest(big));
-    for (int i = 4 * at; i < n; i += 4 * threads) {
-        const float4 v = w8_load4(row + i);
-        uint32_t first[P], second[P];
-        w8_split<P>(v.x * up, v.y * up, first);
-        w8_split<P>(v.z * up, v.w * up, second);
-#pragma unroll
-        for (int p = 0; p < P; ++p) put(p, i, make_uint2(first[p], second[p]));
-    }
-    return 1.f / up;  // of a power of two: exact
-}
 __device__ __forceinline__ float w8_warp_max(float v) {
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, off));
     return v;
+}
+// Rows 0 .. count - 1 of n values (a multiple of 128) brought to f16 by the whole CTA: parts to put(row, part, index, four f16), the power of two that brings a
+// row's parts back to done(row, it).  A row is taken by 8, 4, 2 or 1 warps, so that few rows occupy all; a lane's first eight loads are in flight together and are
+// not read again.
+template <int P, typename InT, typename Put, typename Done>
+__device__ __forceinline__ void w8_rows_parts(const InT* rows, int count, int n, Put&& put, Done&& done) {
+    constexpr int kHeld = 8;
+    __shared__ float warps_max[kW8Warps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int wide = count == 1 ? 8 : count == 2 ? 4 : count <= 4 ? 2 : 1, at_once = kW8Warps / wide;
+    const int at = 4 * ((warp % wide) * 32 + lane), stride = 4 * 32 * wide;
+    for (int row0 = 0; row0 < count; row0 += at_once) {
+        const int row = row0 + warp / wide;
+        const bool live = row < count;
+        const InT* from = rows + static_cast<size_t>(live ? row : 0) * n;
+        float4 held[kHeld];
+        float big = 0.f;
+        auto look = [&](const float4& v) {
+            const float a[4] = {fabsf(v.x), fabsf(v.y), fabsf(v.z), fabsf(v.w)};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) big = a[q] < INFINITY ? fmaxf(big, a[q]) : big;
+        };
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) held[i] = live && at + i * stride < n ? w8_load4(from + at + i * stride) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) look(held[i]);
+        if (live)
+            for (int i = at + kHeld * stride; i < n; i += stride) look(w8_load4(from + i));
+        big = w8_warp_max(big);
+        if (wide > 1) {
+            __syncthreads();
+            if (lane == 0) warps_max[warp] = big;
+            __syncthreads();
+            for (int w = 0; w < wide; ++w) big = fmaxf(big, warps_max[warp / wide * wide + w]);
+        }
+        const float up = w8_up(big);
+        auto give = [&](const float4& v, int i) {
+            uint32_t first[P], second[P];
+            w8_split<P>(v.x * up, v.y * up, first);
+            w8_split<P>(v.z * up, v.w * up, second);
+#pragma unroll
+            for (int p = 0; p < P; ++p) put(row, p, i, make_uint2(first[p], second[p]));
+        };
+        if (live) {
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i)
+                if (at + i * stride < n) give(held[i], at + i * stride);
+            for (int i = at + kHeld * stride; i < n; i += stride) give(w8_load4(from + i), i);
+            if (at == 0) done(row, 1.f / up);  // of a power of two: exact
+        }
+    }
 }
 
 // A CTA a row.
@@ -244,19 +273,10 @@ template <int P, typename InT>
 __global__ void __launch_bounds__(kW8Threads) w8_parts_kernel(const InT* __restrict__ rows, int n, __half* __restrict__ parts, float* __restrict__ scale) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // behind the wait: what follows may read this launch's inputs early
-    __shared__ float warps[kW8Warps];
-    auto widest = [&](float v) {
-        v = w8_warp_max(v);
-        if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = v;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kW8Warps; ++w) v = fmaxf(v, warps[w]);
-        return v;
-    };
     __half* to = parts + static_cast<size_t>(blockIdx.x) * P * n;
-    const float down = w8_row_parts<P>(rows + static_cast<size_t>(blockIdx.x) * n, n, threadIdx.x, kW8Threads, widest,
-                                       [&](int p, int i, uint2 four) { *reinterpret_cast<uint2*>(to + static_cast<size_t>(p) * n + i) = four; });
-    if (threadIdx.x == 0) scale[blockIdx.x] = down;
+    w8_rows_parts<P>(rows + static_cast<size_t>(blockIdx.x) * n, 1, n,
+                     [&](int, int p, int i, uint2 four) { *reinterpret_cast<uint2*>(to + static_cast<size_t>(p) * n + i) = four; },
+                     [&](int, float down) { scale[blockIdx.x] = down; });
 }
 
 // ------------------------------------------------------------------------------------------------ the stream of weights
@@ -400,14 +420,9 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // behind the wait: what follows may read this launch's inputs early
     const int K = DOWN ? p.I : p.H, items = K / 128, own_stride = K + 8;
-    if (OWN) {
-        for (int t = warp; t < p.T; t += kW8Warps) {
-            __half* to = own + static_cast<size_t>(t) * P * own_stride;
-            const float down = w8_row_parts<P>(static_cast<const T*>(p.x) + static_cast<size_t>(t) * K, K, lane, 32, w8_warp_max,
-                                               [&](int q, int i, uint2 four) { *reinterpret_cast<uint2*>(to + q * own_stride + i) = four; });
-            if (lane == 0) own_scale[t] = down;
-        }
-    }
+    if (OWN)
+        w8_rows_parts<1>(static_cast<const T*>(p.x), p.T, K, [&](int t, int, int i, uint2 four) { *reinterpret_cast<uint2*>(own + static_cast<size_t>(t) * own_stride + i) = four; },
+                         [&](int t, float down) { own_scale[t] = down; });
     if (SELF) w8_plan(p, plan);  // ends behind a barrier
     const int n_blocks = SELF ? plan.n_blocks : *p.n_blocks;
     const int tiles = DOWN ? p.H / (16 * MW) : p.I / (8 * MW);  // of a block
@@ -612,12 +627,9 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
     if (OWN) {
         // (a row's factor goes to its weight in the token's sum)
         const int picks = plan.row0[plan.n_blocks - 1] + plan.count[plan.n_blocks - 1];
-        for (int r = warp; r < picks; r += kW8Warps) {
-            __half* to = own + static_cast<size_t>(r) * P * own_stride;
-            const float down = w8_row_parts<P>(p.h + static_cast<size_t>(r) * p.I, p.I, lane, 32, w8_warp_max,
-                                               [&](int q, int i, uint2 four) { *reinterpret_cast<uint2*>(to + q * own_stride + i) = four; });
-            if (lane == 0) plan.score[r] *= down;
-        }
+        w8_rows_parts<P>(p.h, picks, p.I,
+                         [&](int r, int q, int i, uint2 four) { *reinterpret_cast<uint2*>(own + (static_cast<size_t>(r) * P + q) * own_stride + i) = four; },
+                         [&](int r, float down) { plan.score[r] *= down; });
         __syncthreads();
     }
     W8Ahead<P, MW> next;
