@@ -19,9 +19,11 @@
 //   down     A cluster of CTAs has sixteen output channels of ALL the blocks: the picks of a token meet inside it (f32, a fixed order), y is written
 //            once, and nothing is combined in memory: no atomics, no counters.  It has routed the tokens and asked for its first weights before
 //            the launch ahead of it ends.
-// Where the activations are small (kW8Own bytes) each CTA brings them to f16 for itself, and these two launches are the layer; else
-// w8_parts_kernel does it, for x (of bf16) ahead of the first and for silu * up between the two.
-// Above, route + group.cu list the blocks, and both products run as streams of tiles; the down rows go to memory in f32 and
+// Where the activations are small (kW8Own bytes: a token or two) these two launches are the layer, one CTA an SM each, so that the second one is resident, has
+// routed and asked for its first weights while the first one runs.  Else w8_prep_kernel routes the tokens and brings x (of bf16) to f16 ahead of them.
+// Then no launch has to come between the two: the rows' largest values are found as they are written, and the second one splits what it reads of them.
+// Above, w8_prep_kernel and group.cu list the blocks, w8_parts_kernel splits the rows of silu * up (there are so many CTAs for each row that they would do it
+// many times: 64 tokens of 128 experts 152 us for 149), and both products run as streams of tiles; the down rows go to memory in f32 and
 // moe_w8_combine_kernel adds them.
 //
 // Weights reach a lane through a ring in shared memory that the lane fills by cp.async for itself (16 bytes of a row: K indices 16 j .. 16 j + 15
@@ -52,9 +54,14 @@ struct W8Params {
     const float* scale;       // [E][2I] / [E][H], or [E][2I / 128][H / 128] / [E][H / 128][I / 128]
     const float* logits;      // [T][E]
     const void* x;            // [T][H]
-    const __half* parts;      // this phase's activations: [T][H] or [picks][2][I], where the CTAs do not make them
-    const float* part_scale;  // [T] or [picks]: what brings them back; null: nothing does
+    const int32_t* ids;       // [T][topk] -1: dropped; null: the CTAs route
+    const float* shares;      // [T][topk]
+    const __half* x16;        // [T][H] x in f16, where the CTAs do not make it
+    const float* x_scale;     // [T] what brings it back; null: nothing does
     float* h;                 // [picks][I] silu(gate) * up, in expert order
+    uint32_t* h_max;          // [picks] bits of a row's largest finite magnitude; null: nobody reads them
+    const __half* h16;        // [picks][2][I] and what brings it back, general form
+    const float* h_scale;
     void* y;                  // [T][H]
     float* rows_out;          // [picks][H], general form
     const GroupBlock* blocks; // general form
@@ -67,7 +74,6 @@ struct W8Params {
 // The picks in expert order, worked out by a CTA for itself.
 struct W8Plan {
     uint32_t tokens[kW8SelfExperts];      // tokens that picked an expert
-    uint16_t first_block[kW8SelfExperts];
     uint16_t first_row[kW8SelfExperts];
     int16_t id[kW8SelfPicks];             // [token][topk], -1: dropped
     float share[kW8SelfPicks];
@@ -86,14 +92,14 @@ __device__ __forceinline__ uint32_t w8_key(float v) {
     return v != v ? 0u : (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// One warp, one token: picks in the order of their logits, and their shares.
-__device__ __forceinline__ void w8_route(const float* __restrict__ logits, int E, int topk, int16_t* id, float* share) {
-    constexpr int kNV = kW8SelfExperts / 32;
+// One warp, one token of at most 32 NV experts: picks in the order of their logits and their shares to store(place, id, share); -1: no such pick.
+template <int NV, typename Store>
+__device__ __forceinline__ void w8_route(const float* __restrict__ logits, int E, int topk, Store&& store) {
     const int lane = threadIdx.x & 31;
-    uint32_t key[kNV];
+    uint32_t key[NV];
     bool nan = false;
 #pragma unroll
-    for (int b = 0; b < kNV; ++b) {
+    for (int b = 0; b < NV; ++b) {
         const float v = lane + 32 * b < E ? logits[lane + 32 * b] : 0.f;
         nan = nan || v != v;
         key[b] = lane + 32 * b < E ? w8_key(v) : 0u;
@@ -105,7 +111,7 @@ __device__ __forceinline__ void w8_route(const float* __restrict__ logits, int E
         uint32_t best = 0;
         int at = 0;
 #pragma unroll
-        for (int b = 0; b < kNV; ++b)
+        for (int b = 0; b < NV; ++b)
             if (key[b] > best) {
                 best = key[b];
                 at = b;
@@ -114,7 +120,7 @@ __device__ __forceinline__ void w8_route(const float* __restrict__ logits, int E
         const uint32_t e = __reduce_min_sync(0xFFFFFFFFu, best == win && win ? static_cast<uint32_t>(lane + 32 * at) : 0xFFFFFFFFu);
         if (win && e == static_cast<uint32_t>(lane + 32 * at)) {
 #pragma unroll
-            for (int b = 0; b < kNV; ++b)
+            for (int b = 0; b < NV; ++b)
                 if (b == at) key[b] = 0u;
         }
         const float value = __uint_as_float((win & 0x80000000u) ? (win & 0x7FFFFFFFu) : ~win);
@@ -128,19 +134,48 @@ __device__ __forceinline__ void w8_route(const float* __restrict__ logits, int E
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
     if (lane == 0 && my_id < 0) my_id = E - 1;  // nothing but NaN: one pick, for the share below
-    if (lane < topk) {
-        id[lane] = static_cast<int16_t>(my_id);
-        share[lane] = nan ? __int_as_float(0x7FC00000) : p / sum;  // the softmax of a row that holds a NaN
-    }
+    if (lane < topk) store(lane, my_id, nan ? __int_as_float(0x7FC00000) : p / sum);  // the softmax of a row that holds a NaN
 }
 
-__device__ __forceinline__ void w8_plan(const W8Params& p, W8Plan& plan) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// The picks of all tokens: read, or routed by warps 0 .. warps - 1.  No barrier.
+__device__ __forceinline__ void w8_picks(const W8Params& p, W8Plan& plan, int warps) {
+    const int tid = threadIdx.x, warp = tid >> 5;
+    if (p.ids) {
+        for (int i = tid; i < p.T * p.topk; i += kW8Threads) {
+            plan.id[i] = static_cast<int16_t>(__ldcg(p.ids + i));
+            plan.share[i] = __ldcg(p.shares + i);
+        }
+    } else if (warp < warps) {
+        for (int t = warp; t < p.T; t += warps)
+            w8_route<kW8SelfExperts / 32>(p.logits + static_cast<size_t>(t) * p.E, p.E, p.topk, [&](int k, int id, float share) {
+                plan.id[t * p.topk + k] = static_cast<int16_t>(id);
+                plan.share[t * p.topk + k] = share;
+            });
+    }
+}
+// The blocks, from the picks.  Begins and ends with a barrier.
+__device__ __forceinline__ void w8_group(const W8Params& p, W8Plan& plan) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, picks = p.T * p.topk;
     static_assert(kW8SelfExperts == kW8Threads, "an expert a thread");
+    if (p.T == 1) {  // every pick is a block
+        __syncthreads();
+        if (tid < 32) {
+            const int e = tid < picks ? plan.id[tid] : -1;
+            if (e >= 0) {  // (no such pick: none behind it either)
+                plan.expert[tid] = static_cast<uint16_t>(e);
+                plan.row0[tid] = static_cast<uint16_t>(tid);
+                plan.count[tid] = 1;
+                plan.token[tid] = 0;
+                plan.score[tid] = plan.share[tid];
+            }
+            const uint32_t real = __ballot_sync(0xFFFFFFFFu, e >= 0);
+            if (tid == 0) plan.n_blocks = __popc(real);
+        }
+        __syncthreads();
+        return;
+    }
     plan.tokens[tid] = 0;
-    for (int t = warp; t < p.T; t += kW8Warps) w8_route(p.logits + static_cast<size_t>(t) * p.E, p.E, p.topk, plan.id + t * p.topk, plan.share + t * p.topk);
     __syncthreads();
-    const int picks = p.T * p.topk;
     for (int i = tid; i < picks; i += kW8Threads)
         if (plan.id[i] >= 0) atomicOr(plan.tokens + plan.id[i], 1u << (i / p.topk));
     __syncthreads();
@@ -165,7 +200,6 @@ __device__ __forceinline__ void w8_plan(const W8Params& p, W8Plan& plan) {
         block += plan.sums[kW8Warps + w];
     }
     plan.first_row[tid] = static_cast<uint16_t>(row);
-    plan.first_block[tid] = static_cast<uint16_t>(block);
     for (int r = 0; r < c; r += kW8BlockRows, ++block) {
         plan.expert[block] = static_cast<uint16_t>(tid);
         plan.row0[block] = static_cast<uint16_t>(row + r);
@@ -216,15 +250,21 @@ __device__ __forceinline__ float w8_warp_max(float v) {
     for (int off = 16; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, off));
     return v;
 }
-// Rows 0 .. count - 1 of n values (a multiple of 128) brought to f16 by the whole CTA: parts to put(row, part, index, four f16), the power of two that brings a
-// row's parts back to done(row, it).  A row is taken by 8, 4, 2 or 1 warps, so that few rows occupy all; a lane's first eight loads are in flight together and are
-// not read again.
+// Rows 0 .. count - 1 of n values (a multiple of 128) brought to f16 by `warps` warps (all 8, or 4), of which this is number `warp`: parts to
+// put(row, part, index, four f16), the power of two that brings a row's parts back to done(row, it).  A row is taken by as many of them as there are for it; a
+// lane's first eight loads are in flight together and are not read again.
 template <int P, typename InT, typename Put, typename Done>
-__device__ __forceinline__ void w8_rows_parts(const InT* rows, int count, int n, Put&& put, Done&& done) {
+__device__ __forceinline__ void w8_rows_parts(const InT* rows, int count, int n, int warp, int warps, Put&& put, Done&& done) {
     constexpr int kHeld = 8;
     __shared__ float warps_max[kW8Warps];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int wide = count == 1 ? 8 : count == 2 ? 4 : count <= 4 ? 2 : 1, at_once = kW8Warps / wide;
+    const int lane = threadIdx.x & 31;
+    int wide = warps;
+    while (wide > 1 && wide * count > warps) wide /= 2;
+    const int at_once = warps / wide;
+    auto meet = [&]() {
+        if (warps == kW8Warps) __syncthreads();
+        else asm volatile("bar.sync 1, 128;" ::: "memory");
+    };
     const int at = 4 * ((warp % wide) * 32 + lane), stride = 4 * 32 * wide;
     for (int row0 = 0; row0 < count; row0 += at_once) {
         const int row = row0 + warp / wide;
@@ -245,9 +285,8 @@ __device__ __forceinline__ void w8_rows_parts(const InT* rows, int count, int n,
             for (int i = at + kHeld * stride; i < n; i += stride) look(w8_load4(from + i));
         big = w8_warp_max(big);
         if (wide > 1) {
-            __syncthreads();
             if (lane == 0) warps_max[warp] = big;
-            __syncthreads();
+            meet();
             for (int w = 0; w < wide; ++w) big = fmaxf(big, warps_max[warp / wide * wide + w]);
         }
         const float up = w8_up(big);
@@ -268,15 +307,35 @@ __device__ __forceinline__ void w8_rows_parts(const InT* rows, int count, int n,
     }
 }
 
-// A CTA a row.
-template <int P, typename InT>
-__global__ void __launch_bounds__(kW8Threads) w8_parts_kernel(const InT* __restrict__ rows, int n, __half* __restrict__ parts, float* __restrict__ scale) {
+// A CTA a token: its picks, a clear word for each of its rows of silu * up, and (x of bf16) its row in f16.
+template <typename T, int NV>
+__global__ void __launch_bounds__(kW8Threads) w8_prep_kernel(const __grid_constant__ W8Params p, int32_t* __restrict__ ids, float* __restrict__ shares,
+                                                             __half* __restrict__ x16, float* __restrict__ x_scale) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // behind the wait: what follows may read this launch's inputs early
-    __half* to = parts + static_cast<size_t>(blockIdx.x) * P * n;
-    w8_rows_parts<P>(rows + static_cast<size_t>(blockIdx.x) * n, 1, n,
-                     [&](int, int p, int i, uint2 four) { *reinterpret_cast<uint2*>(to + static_cast<size_t>(p) * n + i) = four; },
-                     [&](int, float down) { scale[blockIdx.x] = down; });
+    const int t = blockIdx.x, warp = threadIdx.x >> 5;
+    if (warp < 4) {
+        if (warp == 0)
+            w8_route<NV>(p.logits + static_cast<size_t>(t) * p.E, p.E, p.topk, [&](int k, int id, float share) {
+                ids[static_cast<size_t>(t) * p.topk + k] = id;
+                shares[static_cast<size_t>(t) * p.topk + k] = share;
+                if (p.h_max) p.h_max[static_cast<size_t>(t) * p.topk + k] = 0u;
+            });
+    } else if constexpr (!std::is_same<T, __half>::value) {
+        w8_rows_parts<1>(static_cast<const T*>(p.x) + static_cast<size_t>(t) * p.H, 1, p.H, warp - 4, 4,
+                         [&](int, int, int i, uint2 four) { *reinterpret_cast<uint2*>(x16 + static_cast<size_t>(t) * p.H + i) = four; },
+                         [&](int, float down) { x_scale[t] = down; });
+    }
+}
+
+// A CTA a row of silu * up.
+__global__ void __launch_bounds__(kW8Threads) w8_parts_kernel(const float* __restrict__ h, int n, __half* __restrict__ parts, float* __restrict__ scale) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __half* to = parts + static_cast<size_t>(blockIdx.x) * kW8PartsH * n;
+    w8_rows_parts<kW8PartsH>(h + static_cast<size_t>(blockIdx.x) * n, 1, n, threadIdx.x >> 5, kW8Warps,
+                             [&](int, int p, int i, uint2 four) { *reinterpret_cast<uint2*>(to + static_cast<size_t>(p) * n + i) = four; },
+                             [&](int, float down) { scale[blockIdx.x] = down; });
 }
 
 // ------------------------------------------------------------------------------------------------ the stream of weights
@@ -362,20 +421,25 @@ template <int P, int MW>
 struct W8Ahead {
     uint4 b[P][4];
     float s0[MW], s1[MW];
-    const __half* col;        // null: none
+    const void* col;          // null: none
     const float *at0, *at1;   // scales; where they are per channel, those of the next sixteen rows `more` further
     int k, more;              // 128-element block
 
-    // stride: elements between the parts; ONCE: nobody else of the CTA reads them
-    template <bool BLOCK, bool ONCE>
+    // RAW: the column is f32, 32 of its values to b, for halves().  Else it is f16, `stride` elements between the parts.
+    template <bool BLOCK, bool RAW>
     __device__ __forceinline__ void fetch(int stride) {
+        if (RAW) {
+            static_assert(!RAW || P == 2, "32 values of f32 are two parts of f16");
 #pragma unroll
-        for (int p = 0; p < P; ++p)
+            for (int i = 0; i < 8; ++i)
+                b[i >> 2][i & 3] = col ? __ldcg(reinterpret_cast<const uint4*>(static_cast<const float*>(col) + k * 128 + (i >> 2) * 64 + (i & 3) * 4)) : make_uint4(0, 0, 0, 0);
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint4* from = reinterpret_cast<const uint4*>(col + p * stride + k * 128 + (i >> 1) * 64 + (i & 1) * 8);
-                b[p][i] = col ? (ONCE ? __ldcg(from) : *from) : make_uint4(0, 0, 0, 0);
-            }
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    b[p][i] = col ? *reinterpret_cast<const uint4*>(static_cast<const __half*>(col) + p * stride + k * 128 + (i >> 1) * 64 + (i & 1) * 8) : make_uint4(0, 0, 0, 0);
+        }
 #pragma unroll
         for (int m = 0; m < MW; ++m) {  // sixteen rows lie in one block of 128, and so do thirty-two
             s0[m] = BLOCK && m ? s0[0] : __ldg(at0 + (BLOCK ? k : m * more));
@@ -383,6 +447,24 @@ struct W8Ahead {
         }
     }
 };
+
+// 32 values of f32 as they were fetched, times `up`, as value and remainder.
+__device__ __forceinline__ void w8_halves(uint4 (&b)[2][4], float up) {
+    uint4 raw[2][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) raw[i >> 2][i & 3] = b[i >> 2][i & 3];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // eight values: the i-th sixteen bytes of either part
+        const uint4 &v = raw[i >> 1][2 * (i & 1)], &w = raw[i >> 1][2 * (i & 1) + 1];
+        uint32_t out[4][2];
+        w8_split<2>(__uint_as_float(v.x) * up, __uint_as_float(v.y) * up, out[0]);
+        w8_split<2>(__uint_as_float(v.z) * up, __uint_as_float(v.w) * up, out[1]);
+        w8_split<2>(__uint_as_float(w.x) * up, __uint_as_float(w.y) * up, out[2]);
+        w8_split<2>(__uint_as_float(w.z) * up, __uint_as_float(w.w) * up, out[3]);
+        b[0][i] = make_uint4(out[0][0], out[1][0], out[2][0], out[3][0]);
+        b[1][i] = make_uint4(out[0][1], out[1][1], out[2][1], out[3][1]);
+    }
+}
 
 struct W8Block {
     int expert, row0, count;
@@ -417,24 +499,32 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
     W8Plan& plan = *reinterpret_cast<W8Plan*>(part + kW8Warps * 2 * MW * 32);
     __half* own = reinterpret_cast<__half*>(reinterpret_cast<unsigned char*>(&plan) + (sizeof(W8Plan) + 15) / 16 * 16);  // [T][K + 8]
 
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // behind the wait: what follows may read this launch's inputs early
+    if (!DOWN) {  // (the launches ahead of the down product each waited before they let the next start: the blocks may be read and weights asked for)
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // behind the wait: what follows may read this launch's inputs early
+    }
     const int K = DOWN ? p.I : p.H, items = K / 128, own_stride = K + 8;
-    if (OWN)
-        w8_rows_parts<1>(static_cast<const T*>(p.x), p.T, K, [&](int t, int, int i, uint2 four) { *reinterpret_cast<uint2*>(own + static_cast<size_t>(t) * own_stride + i) = four; },
-                         [&](int t, float down) { own_scale[t] = down; });
-    if (SELF) w8_plan(p, plan);  // ends behind a barrier
+    if (SELF) {
+        // the first four warps route, the others bring x to f16
+        w8_picks(p, plan, OWN ? 4 : kW8Warps);
+        if (OWN && warp >= 4)
+            w8_rows_parts<1>(static_cast<const T*>(p.x), p.T, K, warp - 4, 4,
+                             [&](int t, int, int i, uint2 four) { *reinterpret_cast<uint2*>(own + static_cast<size_t>(t) * own_stride + i) = four; },
+                             [&](int t, float down) { own_scale[t] = down; });
+        w8_group(p, plan);
+    }
     const int n_blocks = SELF ? plan.n_blocks : *p.n_blocks;
     const int tiles = DOWN ? p.H / (16 * MW) : p.I / (8 * MW);  // of a block
-    const int64_t units = static_cast<int64_t>(n_blocks) * tiles;
-    const int64_t u0 = units * blockIdx.x / gridDim.x;
-    const int span = static_cast<int>(units * (blockIdx.x + 1) / gridDim.x - u0);
-    const int64_t total = static_cast<int64_t>(span) * items;
+    using Int = typename std::conditional<SELF, int, int64_t>::type;  // up to 512 blocks of 65536-wide experts: 32 bits, whose divisions are short
+    const Int units = static_cast<Int>(n_blocks) * tiles;
+    const Int u0 = units * static_cast<int>(blockIdx.x) / static_cast<int>(gridDim.x);
+    const int span = static_cast<int>(units * static_cast<int>(blockIdx.x + 1) / static_cast<int>(gridDim.x) - u0);
+    const Int total = static_cast<Int>(span) * items;
     auto share = [&](int w) { return total * w / kW8Warps; };
-    const int64_t q0 = share(warp);
+    const Int q0 = share(warp);
     const int n = static_cast<int>(share(warp + 1) - q0);
-    const int first = static_cast<int>(q0 / items), skip = static_cast<int>(q0 - static_cast<int64_t>(first) * items);
-    const int block0 = static_cast<int>(u0 / tiles), tile0 = static_cast<int>(u0 - static_cast<int64_t>(block0) * tiles);
+    const int first = static_cast<int>(q0 / items), skip = static_cast<int>(q0 - static_cast<Int>(first) * items);
+    const int block0 = static_cast<int>(u0 / tiles), tile0 = static_cast<int>(u0 - static_cast<Int>(block0) * tiles);
 
     // tile `rel` of the span
     struct Tile {
@@ -464,6 +554,10 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
 #pragma unroll 1
     for (int d = 0; d < w8_depth(MW); ++d) w8_issue<MW>(ring, d * kItem, items, open);
 
+    if (DOWN) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    }
     W8Ahead<P, MW> next;
     next.more = DOWN ? 16 : 8;
     int at = first;  // the tile that `next` is of
@@ -474,10 +568,10 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
         next.col = nullptr;
         if (g < blk.count) {
             if (DOWN) {
-                next.col = p.parts + static_cast<size_t>(blk.row0 + g) * P * K + 16 * j;
+                next.col = p.h16 + static_cast<size_t>(blk.row0 + g) * P * K + 16 * j;
             } else {
                 const int token = SELF ? plan.token[blk.row0 + g] : p.rows[blk.row0 + g] / p.topk;
-                next.col = OWN ? own + static_cast<size_t>(token) * P * own_stride + 16 * j : p.parts + static_cast<size_t>(token) * P * K + 16 * j;
+                next.col = (OWN ? own + static_cast<size_t>(token) * own_stride : p.x16 + static_cast<size_t>(token) * K) + 16 * j;
             }
         }
         if (BLOCK) {
@@ -489,9 +583,7 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
             next.at1 = next.at0 + (DOWN ? 8 : p.I);
         }
     };
-    auto fetch = [&]() {
-        next.template fetch<BLOCK, DOWN>(OWN ? own_stride : K);
-    };
+    auto fetch = [&]() { next.template fetch<BLOCK, false>(K); };
     // the finished sums of a tile (lane: channels g and g + 8, or gate and up of channel g; rows 2 j, 2 j + 1)
     auto finish = [&](int rel, const float (&sum)[MW][4]) {
         const Tile t = tile_of(rel);
@@ -499,9 +591,10 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int r = 2 * j + i;
-            if (r >= blk.count) continue;
+            const bool in = r < blk.count;
             if (DOWN) {
-                const float down = __ldcg(p.part_scale + blk.row0 + r);
+                if (!in) continue;
+                const float down = __ldcg(p.h_scale + blk.row0 + r);
                 float* to = p.rows_out + static_cast<size_t>(p.rows[blk.row0 + r]) * p.H + t.chan * 16 * MW + g;
 #pragma unroll
                 for (int m = 0; m < MW; ++m) {
@@ -509,12 +602,21 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
                     to[16 * m + 8] = sum[m][2 + i] * down;
                 }
             } else {
-                const int token = SELF ? plan.token[blk.row0 + r] : p.rows[blk.row0 + r] / p.topk;
-                const float down = OWN ? own_scale[token] : p.part_scale ? __ldcg(p.part_scale + token) : 1.f;
+                float big = 0.f;
+                if (in) {
+                    const int token = SELF ? plan.token[blk.row0 + r] : p.rows[blk.row0 + r] / p.topk;
+                    const float down = OWN ? own_scale[token] : p.x_scale ? __ldcg(p.x_scale + token) : 1.f;
 #pragma unroll
-                for (int m = 0; m < MW; ++m) {
-                    const float gate = sum[m][i] * down, up = sum[m][2 + i] * down;
-                    p.h[static_cast<size_t>(blk.row0 + r) * p.I + (t.chan * MW + m) * 8 + g] = gate / (1.f + expf(-gate)) * up;
+                    for (int m = 0; m < MW; ++m) {
+                        const float gate = sum[m][i] * down, up_ = sum[m][2 + i] * down, h = gate / (1.f + expf(-gate)) * up_;
+                        p.h[static_cast<size_t>(blk.row0 + r) * p.I + (t.chan * MW + m) * 8 + g] = h;
+                        big = fabsf(h) < INFINITY ? fmaxf(big, fabsf(h)) : big;
+                    }
+                }
+                if (p.h_max) {  // the maximum does not depend on the order of its atomics
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, off));
+                    if (in && g == 0) atomicMax(p.h_max + blk.row0 + r, __float_as_uint(big));
                 }
             }
         }
@@ -588,6 +690,7 @@ __device__ __forceinline__ float w8_peer(const float* mine, uint32_t rank) {
 
 template <typename T, bool BLOCK, bool OWN, int MW>
 __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid_constant__ W8Params p) {
+    constexpr bool kRaw = !OWN;
     constexpr int P = kW8PartsH, kRing = w8_ring(MW), kItem = MW * 2048, kChan = 16 * MW;
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -600,7 +703,8 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
     // The launches before this one each waited for what came before them ahead of letting the next start, so the logits may be read here and the
     // weights asked for; what they compute is read behind the wait.
-    w8_plan(p, plan);
+    w8_picks(p, plan, kW8Warps);
+    w8_group(p, plan);
     for (int i = tid; i < kW8Warps * p.T * kChan; i += kW8Threads) sums[i] = 0.f;
     __syncthreads();
     const int items = p.I / 128, chan = static_cast<int>(blockIdx.x / ctas) * kChan, own_stride = p.I + 8;
@@ -627,7 +731,7 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
     if (OWN) {
         // (a row's factor goes to its weight in the token's sum)
         const int picks = plan.row0[plan.n_blocks - 1] + plan.count[plan.n_blocks - 1];
-        w8_rows_parts<P>(p.h, picks, p.I,
+        w8_rows_parts<P>(p.h, picks, p.I, warp, kW8Warps,
                          [&](int r, int q, int i, uint2 four) { *reinterpret_cast<uint2*>(own + (static_cast<size_t>(r) * P + q) * own_stride + i) = four; },
                          [&](int r, float down) { plan.score[r] *= down; });
         __syncthreads();
@@ -636,10 +740,18 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
     next.more = 16;
     int at = first;
     next.k = skip;
+    float up = 1.f;  // what brings this lane's row of h to f16
     auto enter = [&]() {
         const int row0 = plan.row0[at], expert = plan.expert[at];
         next.col = nullptr;
-        if (g < plan.count[at]) next.col = OWN ? own + static_cast<size_t>(row0 + g) * P * own_stride + 16 * j : p.parts + static_cast<size_t>(row0 + g) * P * p.I + 16 * j;
+        if (g < plan.count[at]) {
+            if (OWN) {
+                next.col = own + static_cast<size_t>(row0 + g) * P * own_stride + 16 * j;
+            } else {
+                next.col = p.h + static_cast<size_t>(row0 + g) * p.I + 16 * j;
+                up = w8_up(__uint_as_float(__ldcg(p.h_max + row0 + g)));
+            }
+        }
         if (BLOCK) {
             next.at0 = next.at1 = p.scale + (static_cast<size_t>(expert) * (p.H / 128) + chan / 128) * items;
         } else {
@@ -647,9 +759,7 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
             next.at1 = next.at0 + 8;
         }
     };
-    auto fetch = [&]() {
-        next.template fetch<BLOCK, !OWN>(OWN ? own_stride : p.I);
-    };
+    auto fetch = [&]() { next.template fetch<BLOCK, kRaw>(own_stride); };
     if (n > 0) {
         enter();
         fetch();
@@ -664,12 +774,13 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
         if (!OWN) {
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-                if (2 * j + e < count) down[e] = __ldcg(p.part_scale + row0 + 2 * j + e);
+                if (2 * j + e < count) down[e] = 1.f / w8_up(__uint_as_float(__ldcg(p.h_max + row0 + 2 * j + e)));
         }
         float sum[MW][4] = {};
         for (int c = 0; c < stretch; ++c) {
             asm volatile("cp.async.wait_group %0;" ::"n"(w8_depth(MW) - 1) : "memory");
-            const W8Ahead<P, MW> now = next;
+            W8Ahead<P, MW> now = next;
+            const float now_up = up;
             if (i + c + 1 < n) {
                 if (++next.k == items) {
                     next.k = 0;
@@ -678,6 +789,7 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
                 }
                 fetch();
             }
+            if constexpr (kRaw) w8_halves(now.b, now_up);
             w8_item<P, MW>(ring.base + slot, now.b, now.s0, now.s1, sum);
             w8_issue<MW>(ring, slot, items, open);
             slot = slot + kItem == kRing ? 0 : slot + kItem;
@@ -726,7 +838,7 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
     }
 }
 
-// y[t] = sum_j score[t, j] rows[t topk + j], four channels a thread, picks in ascending expert order.
+// y[t] = sum_j score[t, j] rows[t topk + j], four channels a thread, picks in the order of their logits.
 template <typename T>
 __global__ void __launch_bounds__(256) moe_w8_combine_kernel(const float4* __restrict__ rows, const float* __restrict__ scores, int64_t vecs, int row_vecs, int topk,
                                                              T* __restrict__ y) {
@@ -755,14 +867,16 @@ __global__ void __launch_bounds__(256) moe_w8_combine_kernel(const float4* __res
 static size_t w8_align(size_t v) { return (v + 255) / 256 * 256; }
 
 struct W8Workspace {
-    __half *x_parts, *h_parts;
-    float *x_scale, *h_scale, *h, *scores, *rows_out;
+    __half *x16, *h16;
+    float *x_scale, *h, *shares, *rows_out, *h_scale;
+    uint32_t* h_max;
     int32_t *ids, *rows, *n_blocks;
     GroupBlock* blocks;
     size_t bytes;
 };
 
-static bool w8_self(int64_t T, int64_t E) { return T <= kW8SelfTokens && E <= kW8SelfExperts; }
+// (wider experts than 65536: the general form, whose indices have 64 bits)
+static bool w8_self(int64_t T, int64_t E, int64_t H, int64_t I) { return T <= kW8SelfTokens && E <= kW8SelfExperts && H <= 65536 && I <= 65536; }
 
 static W8Workspace w8_carve(void* base, int64_t T, int64_t E, int64_t topk, int64_t H, int64_t I) {
     W8Workspace w = {};
@@ -775,17 +889,18 @@ static W8Workspace w8_carve(void* base, int64_t T, int64_t E, int64_t topk, int6
     };
     const size_t R = static_cast<size_t>(T) * topk;
     w.h = static_cast<float*>(take(R * I * 4));
-    w.x_parts = static_cast<__half*>(take(static_cast<size_t>(T) * H * 2));
+    w.h_max = static_cast<uint32_t*>(take(R * 4));
+    w.x16 = static_cast<__half*>(take(static_cast<size_t>(T) * H * 2));
     w.x_scale = static_cast<float*>(take(static_cast<size_t>(T) * 4));
-    w.h_parts = static_cast<__half*>(take(R * kW8PartsH * I * 2));
-    w.h_scale = static_cast<float*>(take(R * 4));
-    if (!w8_self(T, E)) {
-        w.ids = static_cast<int32_t*>(take(R * 4));
-        w.scores = static_cast<float*>(take(R * 4));
+    w.ids = static_cast<int32_t*>(take(R * 4));
+    w.shares = static_cast<float*>(take(R * 4));
+    if (!w8_self(T, E, H, I)) {
         w.rows = static_cast<int32_t*>(take(R * 4));
         w.n_blocks = static_cast<int32_t*>(take(4));
         w.blocks = static_cast<GroupBlock*>(take(static_cast<size_t>(group_max_blocks(static_cast<int64_t>(R), E, kW8BlockRows, false)) * sizeof(GroupBlock)));
         w.rows_out = static_cast<float*>(take(R * H * 4));
+        w.h16 = static_cast<__half*>(take(R * kW8PartsH * I * 2));
+        w.h_scale = static_cast<float*>(take(R * 4));
     }
     w.bytes = o;
     return w;
@@ -816,55 +931,58 @@ static int w8_forward(W8Params p, const uint8_t* gate_up, const float* gate_up_s
                       cudaStream_t stream) {
     const size_t plan = (sizeof(W8Plan) + 15) / 16 * 16;
     const int64_t R = static_cast<int64_t>(p.T) * p.topk;
-    const bool self = w8_self(p.T, p.E);
-    const int64_t own_x = static_cast<int64_t>(p.T) * (p.H + 8) * 2, own_h = R * kW8PartsH * (p.I + 8) * 2;
+    const bool self = w8_self(p.T, p.E, p.H, p.I);
     constexpr bool f16 = std::is_same<T, __half>::value;  // x is read as it is
-    const bool x_own = self && !f16 && own_x <= kW8Own, h_own = self && own_h <= kW8Own && R * (p.I / 16) < 8 * 2 * sm_count();
+    const int64_t own_x = f16 ? 0 : static_cast<int64_t>(p.T) * (p.H + 8) * 2, own_h = R * kW8PartsH * (p.I + 8) * 2;
+    const int64_t sms = sm_count(), most = 2 * sms;
+    // Thirty-two rows a warp where there are enough of them: half as many reads of the activations, which lie in L1 and L2, for the same weights.
+    const bool wide = R * (p.I / 16) >= 8 * most, own = self && !wide && own_x <= kW8Own && own_h <= kW8Own;
     int st = EQ_OK;
-    if constexpr (!f16) {
-        if (!x_own) st = w8_launch(w8_parts_kernel<1, T>, p.T, 1, 0, stream, static_cast<const T*>(p.x), p.H, w.x_parts, w.x_scale);
+    p.h_max = self && !own ? w.h_max : nullptr;
+    p.h16 = w.h16;
+    p.h_scale = w.h_scale;
+    if (own) {
+        p.x16 = static_cast<const __half*>(p.x);  // of f16
+    } else {
+        auto prep = [&](auto kernel) { return w8_launch(kernel, p.T, 1, 0, stream, p, w.ids, w.shares, w.x16, w.x_scale); };
+        st = p.E <= 128 ? prep(w8_prep_kernel<T, 4>) : p.E <= 256 ? prep(w8_prep_kernel<T, 8>) : prep(w8_prep_kernel<T, 32>);
+        p.ids = w.ids;
+        p.shares = w.shares;
+        p.x16 = f16 ? static_cast<const __half*>(p.x) : w.x16;
+        p.x_scale = f16 ? nullptr : w.x_scale;
+        if (st == EQ_OK && !self) st = group_rows_launch(w.ids, static_cast<int>(R), p.E, false, kW8BlockRows, false, w.blocks, w.n_blocks, w.rows, nullptr, stream);
     }
-    if (st == EQ_OK && !self) st = eq_moe_route(p.logits, p.T, p.E, p.topk, 1, w.ids, w.scores, stream);
-    if (st == EQ_OK && !self) st = group_rows_launch(w.ids, static_cast<int>(R), p.E, false, kW8BlockRows, false, w.blocks, w.n_blocks, w.rows, nullptr, stream);
     if (st != EQ_OK) return st;
     p.w = gate_up;
     p.scale = gate_up_scale;
-    p.parts = f16 ? static_cast<const __half*>(p.x) : w.x_parts;
-    p.part_scale = f16 ? nullptr : w.x_scale;
-    const int64_t sms = sm_count(), most = 2 * sms;
     auto smem = [&](int mw) { return static_cast<size_t>(kW8Warps) * (w8_ring(mw) + 2 * mw * 32 * sizeof(float4)); };
-    // Thirty-two rows a warp where there are enough of them: half as many reads of the activations, which lie in L1 and L2, for the same weights.
-    const bool wide = R * (p.I / 16) >= 8 * most;
     if (self) {
-        const int64_t tiles = R * (p.I / (wide ? 16 : 8)), grid = tiles < most ? tiles : most;
-        if (x_own) st = wide ? w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, !f16, 2>, grid, 1, smem(2) + plan + own_x, stream, p)
-                             : w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, !f16, 1>, grid, 1, smem(1) + plan + own_x, stream, p);
-        else st = wide ? w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, false, 2>, grid, 1, smem(2) + plan, stream, p)
-                       : w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, false, 1>, grid, 1, smem(1) + plan, stream, p);
+        const int64_t tiles = R * (p.I / (wide ? 16 : 8)), at_once = own ? sms : most, grid = tiles < at_once ? tiles : at_once;
+        if (own) st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, !f16, 1>, grid, 1, smem(1) + plan + own_x, stream, p);
+        else if (wide) st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, false, 2>, grid, 1, smem(2) + plan, stream, p);
+        else st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, false, 1>, grid, 1, smem(1) + plan, stream, p);
     } else {
         st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, false, false, false, 2>, most, 1, smem(2), stream, p);
     }
     if (st != EQ_OK) return st;
     p.w = down;
     p.scale = down_scale;
-    p.parts = w.h_parts;
-    p.part_scale = w.h_scale;
-    if (!h_own) st = w8_launch(w8_parts_kernel<kW8PartsH, float>, R, 1, 0, stream, static_cast<const float*>(w.h), p.I, w.h_parts, w.h_scale);
-    if (st != EQ_OK) return st;
     if (self) {
         const int mw = wide ? 2 : 1;
         const int64_t slabs = p.H / (16 * mw);
-        int cluster = 8;  // two CTAs an SM at most
-        while (cluster > 1 && slabs * cluster > most) cluster /= 2;
+        int cluster = 8;  // two CTAs an SM at most, one beside the launch ahead
+        while (cluster > 1 && slabs * cluster > (own ? sms : most)) cluster /= 2;
         const size_t bytes = static_cast<size_t>(kW8Warps) * (w8_ring(mw) + static_cast<size_t>(p.T) * 16 * mw * sizeof(float)) + plan;
         if (wide) return w8_launch(moe_w8_down_kernel<T, BLOCK, false, 2>, slabs * cluster, cluster, bytes, stream, p);
-        return h_own ? w8_launch(moe_w8_down_kernel<T, BLOCK, true, 1>, slabs * cluster, cluster, bytes + own_h, stream, p)
+        return own ? w8_launch(moe_w8_down_kernel<T, BLOCK, true, 1>, slabs * cluster, cluster, bytes + own_h, stream, p)
                      : w8_launch(moe_w8_down_kernel<T, BLOCK, false, 1>, slabs * cluster, cluster, bytes, stream, p);
     }
+    st = w8_launch(w8_parts_kernel, R, 1, 0, stream, static_cast<const float*>(w.h), p.I, w.h16, w.h_scale);
+    if (st != EQ_OK) return st;
     st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, false, true, false, 2>, most, 1, smem(2), stream, p);
     if (st != EQ_OK) return st;
     const int64_t vecs = static_cast<int64_t>(p.T) * p.H / 4;
-    return w8_launch(moe_w8_combine_kernel<T>, ceil_div(vecs, 256), 1, 0, stream, reinterpret_cast<const float4*>(w.rows_out), static_cast<const float*>(w.scores), vecs, p.H / 4,
+    return w8_launch(moe_w8_combine_kernel<T>, ceil_div(vecs, 256), 1, 0, stream, reinterpret_cast<const float4*>(w.rows_out), static_cast<const float*>(w.shares), vecs, p.H / 4,
                      p.topk, static_cast<T*>(p.y));
 }
 

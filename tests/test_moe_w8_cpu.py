@@ -34,7 +34,7 @@ def test_moe_w8a16_validates_before_it_launches(eq):
     for name in ("gate_up_scale", "down_scale", "logits"):
         assert call(**{name: 4098}) == L.EQ_ERR_BAD_ALIGN
     need = eq.eq_moe_w8a16_workspace_bytes(4, 8, 2, 256, 128)
-    assert need >= 4 * 2 * 128 * 8  # silu * up in f32 and its four parts
+    assert need >= 4 * 2 * 128 * 4 + 4 * 256 * 2  # silu * up in f32, x in f16
     assert call(ws=null) == call(ws_bytes=need - 1) == call(ws=C.c_void_p(4096 + 128)) == L.EQ_ERR_WORKSPACE
 
 
