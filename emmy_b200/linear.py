@@ -14,7 +14,7 @@ import torch
 from torch import nn
 
 from . import lib as L
-from . import ops, ops_moe, ops_nvfp4
+from . import ops, ops_lora, ops_moe, ops_nvfp4
 
 # The custom ops take the repacked weights as TENSORS (plus plain ints), never as process-local handles: the packed
 # blobs are module buffers, so they follow module.to(), are freed with the module, and a traced graph holds nothing
@@ -118,13 +118,37 @@ def _(x, router_logits, gate_up, down, experts, hidden, inter, group, scale_bf16
     return torch.empty_like(x)
 
 
+def _moe_w8(x: torch.Tensor, router_logits: torch.Tensor, gate_up: torch.Tensor, gate_up_scale: torch.Tensor, down: torch.Tensor,
+            down_scale: torch.Tensor, topk: int) -> torch.Tensor:
+    return ops_moe.moe_w8a16(x.contiguous(), router_logits.float().contiguous(), gate_up, gate_up_scale, down, down_scale, topk)
+
+
+_moe_w8_op = torch.library.custom_op("emmyq::moe_w8a16", mutates_args=(), device_types="cuda")(_moe_w8)
+
+
+@_moe_w8_op.register_fake
+def _(x, router_logits, gate_up, gate_up_scale, down, down_scale, topk):
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
+@torch.library.custom_op("emmyq::lora_add", mutates_args=(), device_types="cuda")
+def _lora_add_op(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor, adapter_ids: torch.Tensor,
+                 sections: list[int]) -> torch.Tensor:
+    return ops_lora.lora_add(y.contiguous(), x.contiguous(), a, b, scaling, adapter_ids.contiguous(), sections=sections)
+
+
+@_lora_add_op.register_fake
+def _(y, x, a, b, scaling, adapter_ids, sections):
+    return torch.empty_like(y, memory_format=torch.contiguous_format)
+
+
 # An eager call on plain CUDA tensors needs nothing of the dispatcher: going through the custom op's Python layers costs about 20 us,
 # four times the kernel at one token (with the lighter calls of ops.py a 4096 x 4096 W4A16Linear of one row 49 -> 19 us a call,
 # FP8Linear of 32 rows 43 -> 27, NVFP4Linear of 40 rows 47 -> 28, QuantMoE of one token 56 -> 35).  "Plain" is decided on each call,
 # by what would make the dispatcher do anything else: tracing or compilation, a tensor or function mode, vmap and the other function
 # transforms (all visible in the thread's included keys), a tensor subclass or wrapper (visible in the tensor's own keys), gradients
 # and forward-mode levels, a profiler that wants to see the operator.  Any of them takes the operator as before.
-# W4A16Linear, FP8Linear with per-token scales, FP8BlockLinear, NVFP4Linear and QuantMoE ask; FP8Linear with a static input_scale and
+# W4A16Linear, FP8Linear with per-token scales, FP8BlockLinear, NVFP4Linear, QuantMoE and LoRALinear ask; FP8Linear with a static input_scale and
 # the fused operators always go through the dispatcher.
 _K = torch._C.DispatchKey
 _PLAIN_THREAD = {(torch._C.DispatchKeySet(_K.BackendSelect) | torch._C.DispatchKeySet(_K.ADInplaceOrView)).raw_repr(),
@@ -300,27 +324,139 @@ class NVFP4Linear(nn.Module):
 
 
 class QuantMoE(nn.Module):
-    """Routed MoE block on AWQ experts.  Expert program inputs keep the reference's names and meaning
+    """Routed MoE block on AWQ or FP8 experts.  Expert program inputs keep the reference's names and meaning
     (`w_gate_up` = gate rows then up rows, `w_down`; emmy/compiler/trace/huggingface.py:1702-1717), here as the
-    stacked int4 triplets of each."""
+    stacked int4 triplets of each, or as e4m3 bits with their scales."""
 
     def __init__(self, top_k: int):
         super().__init__()
         self.top_k = top_k
         self.register_buffer("packed_gate_up", None, persistent=False)
         self.register_buffer("packed_down", None, persistent=False)
+        self.register_buffer("gate_up_scale", None, persistent=False)  # FP8 experts only
+        self.register_buffer("down_scale", None, persistent=False)
         self._geometry = None
+
+    def _apply(self, fn, *args, **kwargs):
+        scales = self.gate_up_scale, self.down_scale
+        super()._apply(fn, *args, **kwargs)
+        if scales[0] is not None:  # they move with the module and stay f32
+            self.gate_up_scale, self.down_scale = (s.to(t.device) for s, t in zip(scales, (self.gate_up_scale, self.down_scale)))
+        return self
 
     def load_experts(self, w_gate_up, w_down, group_size: int = 128, fmt: str = "awq") -> "QuantMoE":
         w = ops_moe.moe_repack(w_gate_up, w_down, group_size, fmt)
         self.packed_gate_up, self.packed_down = w.gate_up, w.down
+        self.gate_up_scale = self.down_scale = None
         self._geometry = (w.experts, w.hidden, w.inter, w.group, w.scale_dtype == torch.bfloat16)
+        return self
+
+    def load_fp8_experts(self, w_gate_up: torch.Tensor, gate_up_scale: torch.Tensor, w_down: torch.Tensor, down_scale: torch.Tensor) -> "QuantMoE":
+        """e4m3 weights [E, 2I, H] (gate rows, then up rows) and [E, H, I] with multipliers per output channel ([E, 2I], [E, H]) or per
+        128 x 128 block ([E, 2I / 128, H / 128], [E, H / 128, I / 128]).  Activations stay in their type (W8A16), so a layer of a few
+        tokens reads the picked experts' bytes and nothing else."""
+        e, n2, h = w_gate_up.shape
+        if n2 % 256 or h % 128 or tuple(w_down.shape) != (e, h, n2 // 2):
+            raise ValueError(f"expert shapes do not chain in whole blocks of 128: gate_up {tuple(w_gate_up.shape)}, down {tuple(w_down.shape)}")
+        block = gate_up_scale.dim() == 3
+        want = ((e, n2 // 128, h // 128), (e, h // 128, n2 // 256)) if block else ((e, n2), (e, h))
+        if (tuple(gate_up_scale.shape), tuple(down_scale.shape)) != want:
+            raise ValueError(f"scales {tuple(gate_up_scale.shape)} and {tuple(down_scale.shape)} are neither per channel nor per 128 x 128 block")
+        bits = lambda t: t.view(torch.uint8).contiguous()
+        self.packed_gate_up, self.packed_down = bits(w_gate_up), bits(w_down)
+        self.gate_up_scale, self.down_scale = gate_up_scale.float().contiguous(), down_scale.float().contiguous()
+        self._geometry = (e, h, n2 // 2)
         return self
 
     def forward(self, x: torch.Tensor, router_logits: torch.Tensor) -> torch.Tensor:
         if self._geometry is None:
             raise RuntimeError("QuantMoE.forward: load_experts() has not been called")
         x2, lead = _flat(x)
-        op = _moe if _direct(x2, router_logits, self.packed_gate_up, self.packed_down) else _moe_op
-        y = op(x2, router_logits.reshape(-1, router_logits.shape[-1]), self.packed_gate_up, self.packed_down, *self._geometry, self.top_k)
+        logits = router_logits.reshape(-1, router_logits.shape[-1])
+        direct = _direct(x2, router_logits, self.packed_gate_up, self.packed_down)
+        if self.gate_up_scale is not None:
+            op = _moe_w8 if direct else _moe_w8_op
+            y = op(x2, logits, self.packed_gate_up, self.gate_up_scale, self.packed_down, self.down_scale, self.top_k)
+        else:
+            op = _moe if direct else _moe_op
+            y = op(x2, logits, self.packed_gate_up, self.packed_down, *self._geometry, self.top_k)
         return y.reshape(*lead, x.shape[-1])
+
+
+class LoRALinear(nn.Module):
+    """A linear of any family with `slots` low-rank adapters beside it, one of them per row of x (or none):
+        y[t] = base(x)[t] + scaling[l] B[l] A[l] x[t],  l = adapter_ids[t],  rows with l outside 0 .. slots - 1 keep base(x).
+
+    `sections`: widths of the linears that `base` holds side by side (a fused qkv or gate_up projection), each with its own A.
+    Adapters of smaller rank than `rank` are padded with zeros.  `load_adapter` and `clear_adapter` write into the module's buffers in
+    place, so a captured graph that holds the module's call sees the new adapter.  The buffers are not part of the state dict:
+    adapters come and go with requests, the base's tensors stay under their own names below `base.`."""
+
+    def __init__(self, base: nn.Module, slots: int, rank: int, dtype=torch.bfloat16, sections=None):
+        super().__init__()
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"adapters are f16 or bf16, got {dtype}")
+        self.base, self.slots, self.rank = base, slots, -(-rank // 8) * 8  # the kernels take ranks in eights
+        self.in_features, self.out_features = base.in_features, base.out_features
+        self.sections = tuple(sections) if sections is not None else (base.out_features,)
+        if slots < 1 or rank < 1 or sum(self.sections) != base.out_features:
+            raise ValueError(f"{slots} slots of rank {rank}, sections {self.sections} of {base.out_features} outputs")
+        device = next((t.device for t in (*base.parameters(), *base.buffers())), None)
+        make = lambda *shape, of=dtype: torch.zeros(shape, dtype=of, device=device)
+        self.register_buffer("lora_a", make(slots, len(self.sections), self.rank, self.in_features), persistent=False)
+        self.register_buffer("lora_b", make(slots, self.out_features, self.rank), persistent=False)
+        self.register_buffer("scaling", make(slots, of=torch.float32), persistent=False)
+
+    def _apply(self, fn, *args, **kwargs):
+        scaling = self.scaling
+        super()._apply(fn, *args, **kwargs)
+        self.scaling = scaling.to(self.scaling.device)  # moves with the module and stays f32
+        return self
+
+    def check_adapter(self, slot: int, a, b) -> None:
+        """Raises unless `load_adapter` can take the adapter (lists of one A and one B per section)."""
+        if not 0 <= slot < self.slots:
+            raise ValueError(f"slot {slot} of {self.slots}")
+        if len(a) != len(self.sections) or len(b) != len(a):
+            raise ValueError(f"{len(a)} A and {len(b)} B for {len(self.sections)} sections")
+        for ai, bi, width in zip(a, b, self.sections):
+            if (ai is None) != (bi is None):
+                raise ValueError("a section has an A without a B (or the reverse)")
+            if ai is not None and (ai.dim() != 2 or bi.dim() != 2 or ai.shape[1] != self.in_features or tuple(bi.shape) != (width, ai.shape[0])
+                                   or ai.shape[0] > self.rank):
+                raise ValueError(f"adapter {tuple(ai.shape)} / {tuple(bi.shape)} does not fit {self.in_features} -> {width} at rank {self.rank}")
+
+    def load_adapter(self, slot: int, a, b, scaling: float) -> "LoRALinear":
+        """a [r, K] and b [N, r], or one of each per section (None for a section that the adapter leaves alone); r <= rank."""
+        a, b = (list(t) if isinstance(t, (list, tuple)) else [t] for t in (a, b))
+        self.check_adapter(slot, a, b)
+        self.clear_adapter(slot)
+        first = 0
+        for s, (ai, bi, width) in enumerate(zip(a, b, self.sections)):
+            if ai is not None:
+                r = ai.shape[0]
+                self.lora_a[slot, s, :r].copy_(ai)
+                self.lora_b[slot, first : first + width, :r].copy_(bi)
+            first += width
+        self.scaling[slot] = scaling
+        return self
+
+    def clear_adapter(self, slot: int) -> "LoRALinear":
+        if not 0 <= slot < self.slots:
+            raise ValueError(f"slot {slot} of {self.slots}")
+        for t in (self.lora_a, self.lora_b, self.scaling):
+            t[slot].zero_()
+        return self
+
+    def forward(self, x: torch.Tensor, adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
+        """adapter_ids: int32, one per row of x (x.shape[:-1]); None: the base alone."""
+        y = self.base(x)
+        if adapter_ids is None:
+            return y
+        x2, lead = _flat(x)
+        y2, ids = y.reshape(-1, self.out_features), adapter_ids.reshape(-1)
+        if _direct(x2, y2, ids, self.lora_a, self.lora_b):
+            out = ops_lora.lora_add(y2.contiguous(), x2.contiguous(), self.lora_a, self.lora_b, self.scaling, ids.contiguous(), sections=self.sections)
+        else:
+            out = _lora_add_op(y2, x2, self.lora_a, self.lora_b, self.scaling, ids, list(self.sections))
+        return out.reshape(*lead, self.out_features)

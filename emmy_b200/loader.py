@@ -13,7 +13,10 @@ recognized linear to the operators of this package:
                   `<m>.input_scale` | `<m>.activation_scale`]  -> FP8Linear (per-tensor / per-channel scales) or
                   FP8BlockLinear (2-D block scales)
     routed experts  per-expert `gate_proj` / `up_proj` / `down_proj` modules, or fused `gate_up_proj` tensors with gate and
-                  up interleaved on even / odd columns (de-interleaved at load) -> stacked [gate | up] and down, QuantMoE
+                  up interleaved on even / odd columns (de-interleaved at load) -> stacked [gate | up] and down, QuantMoE; AWQ
+                  int4, or FP8 with per-tensor, per-channel or 128 x 128 block scales
+    adapters      `adapter_config.json` + `adapter_model.safetensors` (`...<module>.lora_A.weight` / `lora_B.weight`) -> slots of
+                  LoRALinear modules
 
 `scan()` works on the host alone (it reads headers, not tensors) and returns one `LinearSpec` per recognized linear;
 `load_linear()` / `load_experts()` read the tensors and build the modules on a CUDA device.  One difference from the
@@ -373,6 +376,44 @@ def stack_experts(per_expert: dict[int, dict[str, tuple]]):
     return pack(gate_up), pack(down)
 
 
+def stack_fp8_experts(index: CheckpointIndex, experts: dict[int, dict[str, LinearSpec]], device="cpu", interleaved_gate_up: bool = False):
+    """One layer's FP8 experts -> (gate_up bits [E, 2I, H], its scales, down bits [E, H, I], its scales) with gate rows before up rows;
+    scales per output channel (a per-tensor scale is repeated), or per 128 x 128 block.  Activation scales of a statically calibrated
+    checkpoint are not read: the kernels leave activations in 16 bits."""
+    order = sorted(experts)
+    if order != list(range(len(order))):
+        raise ValueError(f"experts {order[:4]}... are not 0..{len(order) - 1}")
+
+    def pair(spec):
+        if spec.block not in (None, (128, 128)):
+            raise ValueError(f"{spec.module}: FP8 expert kernels take 128 x 128 weight blocks, got {spec.block}")
+        bits, scale = _bits(index.tensor(spec.keys["weight"])).to(device), index.tensor(spec.keys["weight_scale"]).to(device).float()
+        if spec.block is None:
+            scale = scale.reshape(-1).expand(spec.out_features)
+        return bits, scale
+
+    out = [[], [], [], []]
+    for e in order:
+        entry = experts[e]
+        if "gate_up" in entry:
+            spec = entry["gate_up"]
+            bits, scale = pair(spec)
+            if interleaved_gate_up:
+                if spec.block is not None:
+                    raise ValueError(f"{spec.module}: gate and up rows that alternate share their scale blocks and cannot be taken apart")
+                bits, scale = (torch.cat([t[0::2], t[1::2]]) for t in (bits, scale))
+        elif "gate" in entry and "up" in entry:
+            (gate, gate_scale), (up, up_scale) = pair(entry["gate"]), pair(entry["up"])
+            bits, scale = torch.cat([gate, up]), torch.cat([gate_scale, up_scale])
+        else:
+            raise ValueError(f"expert {e} has a gate without an up projection (or the reverse)")
+        if "down" not in entry:
+            raise ValueError(f"expert {e} has no down projection")
+        for to, t in zip(out, (bits, scale, *pair(entry["down"]))):
+            to.append(t)
+    return tuple(torch.stack(t).contiguous() for t in out)
+
+
 _EXPERT_RE = re.compile(r"^(?P<prefix>.*\.experts)\.(?P<e>\d+)\.(?P<proj>gate_proj|up_proj|down_proj|gate_up_proj)$")
 
 
@@ -388,18 +429,20 @@ def scan_experts(specs: dict[str, LinearSpec]) -> dict[str, dict[int, dict[str, 
 
 
 def load_experts(index: CheckpointIndex, experts: dict[int, dict[str, LinearSpec]], device, top_k: int, interleaved_gate_up: bool = False):
-    """One MoE layer's routed experts (AWQ int4) -> QuantMoE.  `interleaved_gate_up`: the fused gate_up_proj tensors hold
+    """One MoE layer's routed experts (AWQ int4 or FP8) -> QuantMoE.  `interleaved_gate_up`: the fused gate_up_proj tensors hold
     gate and up on even / odd columns and are de-interleaved first."""
     from . import linear as L
 
     dev = torch.device(device)
+    if {spec.family for projs in experts.values() for spec in projs.values()} in ({"fp8"}, {"fp8_block"}):
+        return L.QuantMoE(top_k).to(dev).load_fp8_experts(*stack_fp8_experts(index, experts, dev, interleaved_gate_up))
     per: dict = {}
     group = None
     for e, projs in experts.items():
         entry = {}
         for role, spec in projs.items():
             if spec.family != "awq":
-                raise ValueError(f"expert {e} {role}: the grouped expert kernels take AWQ int4 weights, got {spec.family}")
+                raise ValueError(f"expert {e} {role}: the grouped expert kernels take AWQ int4 weights or FP8 throughout a layer, got {spec.family}")
             group = spec.group_size
             triple = tuple(index.tensor(spec.keys[k]).to(dev) for k in ("qweight", "qzeros", "scales"))
             if role == "gate_up" and interleaved_gate_up:
@@ -408,3 +451,65 @@ def load_experts(index: CheckpointIndex, experts: dict[int, dict[str, LinearSpec
         per[e] = entry
     gate_up, down = stack_experts(per)
     return L.QuantMoE(top_k).to(dev).load_experts(gate_up, down, group, "awq")
+
+
+# ---------------------------------------------------------------------------------------------- low-rank adapters
+
+_ADAPTER_RE = re.compile(r"^(?:base_model\.model\.)?(?P<module>.+)\.lora_(?P<ab>[AB])\.weight$")
+
+
+def read_adapter(adapter_dir) -> dict[str, tuple[torch.Tensor, torch.Tensor, float]]:
+    """module path -> (A [r, K], B [N, r], scaling) of a low-rank adapter directory, on the host.  scaling = alpha / r, or alpha / sqrt(r)
+    with `use_rslora`, alpha by `alpha_pattern` where an entry names the module (path or dotted suffix).  What is not such a product
+    (trained biases, embeddings or saved modules, a magnitude vector, transposed weights) raises."""
+    cfg = json.loads((Path(adapter_dir) / "adapter_config.json").read_text())
+    if cfg.get("peft_type", "LORA") != "LORA":
+        raise ValueError(f"adapter of type {cfg['peft_type']!r}, not LORA")
+    for key, plain in (("bias", (None, "none")), ("use_dora", (None, False)), ("fan_in_fan_out", (None, False)), ("modules_to_save", (None, []))):
+        if cfg.get(key) not in plain:
+            raise ValueError(f"unsupported adapter: {key}={cfg[key]!r}")
+    index = CheckpointIndex(adapter_dir)
+    pairs: dict = {}
+    for key in index.keys():
+        m = _ADAPTER_RE.match(key)
+        if not m:
+            raise ValueError(f"unsupported adapter tensor {key!r}")
+        pairs.setdefault(m["module"], {})[m["ab"]] = index.tensor(key)
+    out = {}
+    for module, ab in pairs.items():
+        if set(ab) != {"A", "B"}:
+            raise ValueError(f"adapter of {module!r} lacks lora_A or lora_B")
+        a, b = ab["A"], ab["B"]
+        if a.dim() != 2 or b.dim() != 2 or a.shape[0] != b.shape[1] or a.shape[0] == 0:
+            raise ValueError(f"adapter of {module!r}: A {tuple(a.shape)} and B {tuple(b.shape)} do not chain")
+        alpha = cfg.get("lora_alpha", a.shape[0])
+        for pattern, value in (cfg.get("alpha_pattern") or {}).items():
+            if re.match(rf"(.*\.)?({pattern})$", module):
+                alpha = value
+                break
+        out[module] = (a, b, alpha / (a.shape[0] ** 0.5 if cfg.get("use_rslora") else a.shape[0]))
+    return out
+
+
+def load_adapter(adapter_dir, modules: dict, slot: int) -> None:
+    """Loads an adapter directory into `slot` of LoRALinear modules, keyed by module path, or by the tuple of the paths whose linears a
+    fused projection holds side by side.  Modules that the adapter does not touch have the slot cleared; an adapted module that is not
+    among the keys raises, before anything is written."""
+    adapters = read_adapter(adapter_dir)
+    paths = {key: (key,) if isinstance(key, str) else tuple(key) for key in modules}
+    rest = set(adapters) - {p for ps in paths.values() for p in ps}
+    if rest:
+        raise ValueError(f"the adapter changes modules that were not given: {sorted(rest)[:4]}")
+    plan = []
+    for key, mod in modules.items():
+        parts = [adapters.get(p) for p in paths[key]]
+        if len(parts) != len(mod.sections):
+            raise ValueError(f"{key}: {len(parts)} modules for {len(mod.sections)} sections")
+        mod.check_adapter(slot, [p and p[0] for p in parts], [p and p[1] for p in parts])
+        plan.append((mod, parts))
+    for mod, parts in plan:
+        # one scaling a slot: where the sections' differ, the first one's; the others' B bring the quotient
+        scales = [p[2] for p in parts if p is not None]
+        lead = next((s for s in scales if s), 1.0)
+        b = [p and (p[1] if p[2] == lead else p[1].double() * (p[2] / lead)) for p in parts]
+        mod.load_adapter(slot, [p and p[0] for p in parts], b, lead if scales else 0.0)

@@ -37,6 +37,15 @@ def _need_cuda(*tensors):
                 raise ValueError("emmy_b200 operators take contiguous tensors")
 
 
+def _need_here(*tensors):
+    """_need_cuda, and every tensor on the current device, whose stream the call is queued on."""
+    _need_cuda(*tensors)
+    here = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise ValueError(f"a tensor is on cuda:{t.get_device()}, the current device is cuda:{here}: call under torch.cuda.device()")
+
+
 def unpack_int4(words: torch.Tensor, fmt: str, along_rows: bool = False) -> torch.Tensor:
     _need_cuda(words)
     rows, cols = words.shape

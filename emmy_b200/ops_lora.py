@@ -7,7 +7,7 @@ import ctypes as C
 import torch
 
 from . import lib as L
-from .ops import _DTYPE, _need_cuda, _scratch, _stream
+from .ops import _DTYPE, _need_here, _scratch, _stream
 
 _widths: dict = {}
 
@@ -27,7 +27,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
 
     y [T, N] is a linear's output for x [T, K]; a [L, R, K] (or [L, S, R, K] for a projection of S linears side by side whose widths are
     `sections`), b [L, N, R], scaling f32 [L], adapter_ids int32 [T].  `out` may be y."""
-    _need_cuda(y, x, a, b, scaling, adapter_ids, out)
+    _need_here(y, x, a, b, scaling, adapter_ids, out, workspace)
     t, k = x.shape
     n = y.shape[1]
     adapters, s, r = a.shape[0], (a.shape[1] if a.dim() == 4 else 1), a.shape[-2]

@@ -7,7 +7,7 @@ import ctypes as C
 import torch
 
 from . import lib as L
-from .ops import _DTYPE, _FMT, _need_cuda, _ptr, _scratch, _stream
+from .ops import _DTYPE, _FMT, _need_cuda, _need_here, _ptr, _scratch, _stream
 
 
 class MoEWeights:
@@ -117,7 +117,7 @@ def moe_w8a16(x, router_logits, gate_up, gate_up_scale, down, down_scale, topk: 
 
     gate_up e4m3 bits [E, 2I, H] (uint8; gate rows, then up rows), down [E, H, I]; scales f32, per output channel ([E, 2I] and [E, H]) or
     per 128 x 128 block ([E, 2I / 128, H / 128] and [E, H / 128, I / 128])."""
-    _need_cuda(x, router_logits, gate_up, gate_up_scale, down, down_scale, workspace, out)
+    _need_here(x, router_logits, gate_up, gate_up_scale, down, down_scale, workspace, out)
     t, h = x.shape
     e, n2, k = gate_up.shape
     i = down.shape[2]

@@ -80,6 +80,24 @@ def column_slice_nvfp4(weight, weight_scale, weight_scale_2, rank: int, world: i
     return weight[c].contiguous(), weight_scale[c].contiguous(), weight_scale_2
 
 
+def column_slice_lora(a, b, rank: int, world: int, sections=None):
+    """Output-column shard of an adapter a [.., R, K], b [.., N, R] of a column-parallel linear: every rank has all of A and its rows of
+    each section's B.  -> (a, b, the shard's section widths)."""
+    widths, parts, first = [], [], 0
+    for width in sections if sections is not None else (b.shape[-2],):
+        c = _cols(width, rank, world, 8)
+        parts.append(b[..., first + c.start : first + c.stop, :])
+        widths.append(c.stop - c.start)
+        first += width
+    return a, torch.cat(parts, dim=-2).contiguous(), tuple(widths)
+
+
+def row_slice_lora(a, b, rank: int, world: int):
+    """Input-row shard of an adapter of a row-parallel linear: a rank's columns of A and all of B, so that the adapters' parts add up in
+    the linear's own sum over the ranks (A's columns are split, B is applied to each part)."""
+    return a[..., _cols(a.shape[-1], rank, world, 8)].contiguous(), b
+
+
 def expert_owner(expert_ids: torch.Tensor, num_experts: int, world: int) -> torch.Tensor:
     """Rank that holds each expert: contiguous blocks of E / W experts."""
     if num_experts % world:
