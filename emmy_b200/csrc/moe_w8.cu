@@ -350,11 +350,11 @@ __device__ __forceinline__ uint32_t w8_pair(uint32_t two) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(two)));
     return h;
 }
-// One item: sum[m][16 rows][8 columns] += scale x W x over 128 elements, scale s0 for rows g and s1 for rows g + 8.  slot: this lane's first 16 bytes in the ring
-// (of sixteen rows the first half of the elements, rows g; then rows g + 8; then the other half's); b: the lane's column at the same K indices, sixteen values a
-// half, of every part.
-template <int P, int MW>
-__device__ __forceinline__ void w8_item(uint32_t slot, const uint4 (&b)[P][4], const float (&s0)[MW], const float (&s1)[MW], float (&sum)[MW][4]) {
+// One item, or with two groups of eight columns half of one: sum[c][m][16 rows][8 columns] += scale x W x over 128 or 64 elements, scale s0 for rows g and s1 for
+// rows g + 8.  slot: this lane's first 16 bytes in the ring (of sixteen rows the first half of the elements, rows g; then rows g + 8; then the other
+// half's); b: the lane's column of a group at the same K indices, sixteen values a half, of every part.
+template <int P, int MW, int RB>
+__device__ __forceinline__ void w8_item(uint32_t slot, const uint4 (&b)[RB][P][4 / RB], const float (&s0)[MW], const float (&s1)[MW], float (&sum)[RB][MW][4]) {
 #pragma unroll
     for (int m = 0; m < MW; ++m) {
         float acc[2][4];
@@ -363,21 +363,25 @@ __device__ __forceinline__ void w8_item(uint32_t slot, const uint4 (&b)[P][4], c
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[c][e] = 0.f;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+        for (int half = 0; half < 2 / RB; ++half) {
             const uint4 top = w8_lds(slot + m * 2048 + half * 1024), bottom = w8_lds(slot + m * 2048 + half * 1024 + 512);
             const uint32_t t[4] = {top.x, top.y, top.z, top.w}, u[4] = {bottom.x, bottom.y, bottom.z, bottom.w};
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const uint32_t a0 = w8_pair(t[q] & 0xFFFFu), a2 = w8_pair(t[q] >> 16), a1 = w8_pair(u[q] & 0xFFFFu), a3 = w8_pair(u[q] >> 16);
 #pragma unroll
-                for (int p = 0; p < P; ++p) {  // two chains
-                    const uint4& v = b[p][2 * half + (q >> 1)];
-                    mma_16816<__half>(acc[P == 2 ? p : q & 1], a0, a1, a2, a3, q & 1 ? v.z : v.x, q & 1 ? v.w : v.y);
-                }
+                for (int p = 0; p < P; ++p)
+#pragma unroll
+                    for (int c = 0; c < RB; ++c) {  // two chains
+                        const uint4& v = b[c][p][2 * half + (q >> 1)];
+                        mma_16816<__half>(acc[RB == 2 ? c : P == 2 ? p : q & 1], a0, a1, a2, a3, q & 1 ? v.z : v.x, q & 1 ? v.w : v.y);
+                    }
             }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[m][e] = fmaf(acc[0][e] + acc[1][e], e < 2 ? s0[m] : s1[m], sum[m][e]);
+        for (int c = 0; c < RB; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[c][m][e] = fmaf(RB == 2 ? acc[c][e] : acc[0][e] + acc[1][e], e < 2 ? s0[m] : s1[m], sum[c][m][e]);
     }
 }
 
@@ -416,30 +420,34 @@ __device__ __forceinline__ void w8_issue(W8Ring& r, uint32_t slot, int items, Op
     w8_commit();
 }
 
-// What a lane reads beside the weights, one item ahead: its column at its K indices, the two scales.
-template <int P, int MW>
+// What a lane reads beside the weights, an item (half an item, with two groups of columns) ahead: its columns at its K indices, the two scales.
+template <int P, int MW, int RB>
 struct W8Ahead {
-    uint4 b[P][4];
+    uint4 b[RB][P][4 / RB];
     float s0[MW], s1[MW];
-    const void* col;          // null: none
+    const void* col[RB];      // null: none
     const float *at0, *at1;   // scales; where they are per channel, those of the next sixteen rows `more` further
     int k, more;              // 128-element block
 
     // RAW: the column is f32, 32 of its values to b, for halves().  Else it is f16, `stride` elements between the parts.
     template <bool BLOCK, bool RAW>
-    __device__ __forceinline__ void fetch(int stride) {
-        if (RAW) {
-            static_assert(!RAW || P == 2, "32 values of f32 are two parts of f16");
+    __device__ __forceinline__ void fetch(int stride, int half) {
+        if constexpr (RAW) {
+            static_assert(P == 2 && RB == 1, "32 values of f32 are two parts of f16");
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                b[i >> 2][i & 3] = col ? __ldcg(reinterpret_cast<const uint4*>(static_cast<const float*>(col) + k * 128 + (i >> 2) * 64 + (i & 3) * 4)) : make_uint4(0, 0, 0, 0);
+                b[0][i >> 2][i & 3] = col[0] ? __ldcg(reinterpret_cast<const uint4*>(static_cast<const float*>(col[0]) + k * 128 + (i >> 2) * 64 + (i & 3) * 4)) : make_uint4(0, 0, 0, 0);
         } else {
 #pragma unroll
-            for (int p = 0; p < P; ++p)
+            for (int c = 0; c < RB; ++c)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    b[p][i] = col ? *reinterpret_cast<const uint4*>(static_cast<const __half*>(col) + p * stride + k * 128 + (i >> 1) * 64 + (i & 1) * 8) : make_uint4(0, 0, 0, 0);
+                for (int p = 0; p < P; ++p)
+#pragma unroll
+                    for (int i = 0; i < 4 / RB; ++i)
+                        b[c][p][i] = col[c] ? *reinterpret_cast<const uint4*>(static_cast<const __half*>(col[c]) + p * stride + k * 128 + (half + (i >> 1)) * 64 + (i & 1) * 8)
+                                            : make_uint4(0, 0, 0, 0);
         }
+        if (half) return;  // the scales are the item's
 #pragma unroll
         for (int m = 0; m < MW; ++m) {  // sixteen rows lie in one block of 128, and so do thirty-two
             s0[m] = BLOCK && m ? s0[0] : __ldg(at0 + (BLOCK ? k : m * more));
@@ -487,16 +495,16 @@ __device__ __forceinline__ W8Block w8_block(const W8Params& p, const W8Plan& pla
 }
 
 // ------------------------------------------------------------------------------------------------ spans of whole tiles: gate_up; down, general form
-// OWN: the CTA brings x to f16.
-template <typename T, bool BLOCK, bool SELF, bool DOWN, bool OWN, int MW>
+// OWN: the CTA brings x to f16.  RB: groups of eight rows that a block has at most.
+template <typename T, bool BLOCK, bool SELF, bool DOWN, bool OWN, int MW, int RB>
 __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __grid_constant__ W8Params p) {
-    constexpr int P = DOWN ? kW8PartsH : 1, kRing = w8_ring(MW), kItem = MW * 2048;
+    constexpr int P = DOWN ? kW8PartsH : 1, kSums = MW * RB, kRing = w8_ring(MW), kItem = MW * 2048;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ float own_scale[kW8SelfTokens];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, j = lane & 3;
-    float4* part = reinterpret_cast<float4*>(smem + kW8Warps * kRing);  // [warps][first, last tile][MW][32]
-    W8Plan& plan = *reinterpret_cast<W8Plan*>(part + kW8Warps * 2 * MW * 32);
+    float4* part = reinterpret_cast<float4*>(smem + kW8Warps * kRing);  // [warps][first, last tile][RB][MW][32]
+    W8Plan& plan = *reinterpret_cast<W8Plan*>(part + kW8Warps * 2 * kSums * 32);
     __half* own = reinterpret_cast<__half*>(reinterpret_cast<unsigned char*>(&plan) + (sizeof(W8Plan) + 15) / 16 * 16);  // [T][K + 8]
 
     if (!DOWN) {  // (the launches ahead of the down product each waited before they let the next start: the blocks may be read and weights asked for)
@@ -558,20 +566,24 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
         asm volatile("griddepcontrol.wait;" ::: "memory");
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     }
-    W8Ahead<P, MW> next;
+    W8Ahead<P, MW, RB> next;
     next.more = DOWN ? 16 : 8;
     int at = first;  // the tile that `next` is of
     next.k = skip;
     auto enter = [&]() {
         const Tile t = tile_of(at);
         const W8Block blk = w8_block<SELF>(p, plan, t.block);
-        next.col = nullptr;
-        if (g < blk.count) {
-            if (DOWN) {
-                next.col = p.h16 + static_cast<size_t>(blk.row0 + g) * P * K + 16 * j;
-            } else {
-                const int token = SELF ? plan.token[blk.row0 + g] : p.rows[blk.row0 + g] / p.topk;
-                next.col = (OWN ? own + static_cast<size_t>(token) * own_stride : p.x16 + static_cast<size_t>(token) * K) + 16 * j;
+#pragma unroll
+        for (int c = 0; c < RB; ++c) {
+            const int r = g + 8 * c;
+            next.col[c] = nullptr;
+            if (r < blk.count) {
+                if (DOWN) {
+                    next.col[c] = p.h16 + static_cast<size_t>(blk.row0 + r) * P * K + 16 * j;
+                } else {
+                    const int token = SELF ? plan.token[blk.row0 + r] : p.rows[blk.row0 + r] / p.topk;
+                    next.col[c] = (OWN ? own + static_cast<size_t>(token) * own_stride : p.x16 + static_cast<size_t>(token) * K) + 16 * j;
+                }
             }
         }
         if (BLOCK) {
@@ -583,14 +595,14 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
             next.at1 = next.at0 + (DOWN ? 8 : p.I);
         }
     };
-    auto fetch = [&]() { next.template fetch<BLOCK, false>(K); };
+    auto fetch = [&](int half) { next.template fetch<BLOCK, false>(K, half); };
     // the finished sums of a tile (lane: channels g and g + 8, or gate and up of channel g; rows 2 j, 2 j + 1)
-    auto finish = [&](int rel, const float (&sum)[MW][4]) {
+    auto finish = [&](int rel, const float (&sum)[RB][MW][4]) {
         const Tile t = tile_of(rel);
         const W8Block blk = w8_block<SELF>(p, plan, t.block);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = 2 * j + i;
+        for (int ci = 0; ci < 2 * RB; ++ci) {
+            const int c = ci >> 1, i = ci & 1, r = 8 * c + 2 * j + i;
             const bool in = r < blk.count;
             if (DOWN) {
                 if (!in) continue;
@@ -598,8 +610,8 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
                 float* to = p.rows_out + static_cast<size_t>(p.rows[blk.row0 + r]) * p.H + t.chan * 16 * MW + g;
 #pragma unroll
                 for (int m = 0; m < MW; ++m) {
-                    to[16 * m] = sum[m][i] * down;
-                    to[16 * m + 8] = sum[m][2 + i] * down;
+                    to[16 * m] = sum[c][m][i] * down;
+                    to[16 * m + 8] = sum[c][m][2 + i] * down;
                 }
             } else {
                 float big = 0.f;
@@ -608,7 +620,7 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
                     const float down = OWN ? own_scale[token] : p.x_scale ? __ldcg(p.x_scale + token) : 1.f;
 #pragma unroll
                     for (int m = 0; m < MW; ++m) {
-                        const float gate = sum[m][i] * down, up_ = sum[m][2 + i] * down, h = gate / (1.f + expf(-gate)) * up_;
+                        const float gate = sum[c][m][i] * down, up_ = sum[c][m][2 + i] * down, h = gate / (1.f + expf(-gate)) * up_;
                         p.h[static_cast<size_t>(blk.row0 + r) * p.I + (t.chan * MW + m) * 8 + g] = h;
                         big = fabsf(h) < INFINITY ? fmaxf(big, fabsf(h)) : big;
                     }
@@ -624,25 +636,31 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
 
     if (n > 0) {
         enter();
-        fetch();
+        fetch(0);
     }
     uint32_t slot = 0;
     int rel = first, it = skip;
     for (int i = 0; i < n;) {
         const int stretch = min(items - it, n - i);
-        float sum[MW][4] = {};
+        float sum[RB][MW][4] = {};
         for (int c = 0; c < stretch; ++c) {
             asm volatile("cp.async.wait_group %0;" ::"n"(w8_depth(MW) - 1) : "memory");
-            const W8Ahead<P, MW> now = next;
+            W8Ahead<P, MW, RB> now = next;
+            if constexpr (RB == 2) {
+                fetch(1);
+                w8_item<P, MW, RB>(ring.base + slot, now.b, now.s0, now.s1, sum);
+#pragma unroll
+                for (int q = 0; q < 2 * P * 2; ++q) now.b[q & 1][(q >> 1) & (P - 1)][q / (2 * P)] = next.b[q & 1][(q >> 1) & (P - 1)][q / (2 * P)];
+            }
             if (i + c + 1 < n) {
                 if (++next.k == items) {
                     next.k = 0;
                     ++at;
                     enter();
                 }
-                fetch();
+                fetch(0);
             }
-            w8_item<P, MW>(ring.base + slot, now.b, now.s0, now.s1, sum);
+            w8_item<P, MW, RB>(ring.base + slot + (RB - 1) * 1024, now.b, now.s0, now.s1, sum);
             w8_issue<MW>(ring, slot, items, open);
             slot = slot + kItem == kRing ? 0 : slot + kItem;
         }
@@ -650,7 +668,10 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
             finish(rel, sum);
         } else {  // another warp has a part of the tile
 #pragma unroll
-            for (int m = 0; m < MW; ++m) part[((warp * 2 + (rel == first ? 0 : 1)) * MW + m) * 32 + lane] = make_float4(sum[m][0], sum[m][1], sum[m][2], sum[m][3]);
+            for (int q = 0; q < kSums; ++q) {
+                const float(&v)[4] = sum[q / MW][q % MW];
+                part[((warp * 2 + (rel == first ? 0 : 1)) * kSums + q) * 32 + lane] = make_float4(v[0], v[1], v[2], v[3]);
+            }
         }
         i += stretch;
         it = 0;
@@ -660,19 +681,20 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
     // the shared tiles, in the order of the warps that have a part
     for (int t = warp; t < span; t += kW8Warps) {
         const int64_t lo_item = static_cast<int64_t>(t) * items, hi_item = lo_item + items;
-        float sum[MW][4] = {};
+        float sum[RB][MW][4] = {};
         int parts = 0;
         for (int w = 0; w < kW8Warps; ++w) {
             const int64_t a = share(w), b = share(w + 1);
             if (a >= hi_item || b <= lo_item || a == b || (a <= lo_item && b >= hi_item)) continue;
             ++parts;
 #pragma unroll
-            for (int m = 0; m < MW; ++m) {
-                const float4 v = part[((w * 2 + (static_cast<int>(a / items) == t ? 0 : 1)) * MW + m) * 32 + lane];
-                sum[m][0] += v.x;
-                sum[m][1] += v.y;
-                sum[m][2] += v.z;
-                sum[m][3] += v.w;
+            for (int q = 0; q < kSums; ++q) {
+                const float4 v = part[((w * 2 + (static_cast<int>(a / items) == t ? 0 : 1)) * kSums + q) * 32 + lane];
+                float(&to)[4] = sum[q / MW][q % MW];
+                to[0] += v.x;
+                to[1] += v.y;
+                to[2] += v.z;
+                to[3] += v.w;
             }
         }
         if (parts) finish(t, sum);
@@ -736,19 +758,19 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
                          [&](int r, float down) { plan.score[r] *= down; });
         __syncthreads();
     }
-    W8Ahead<P, MW> next;
+    W8Ahead<P, MW, 1> next;
     next.more = 16;
     int at = first;
     next.k = skip;
     float up = 1.f;  // what brings this lane's row of h to f16
     auto enter = [&]() {
         const int row0 = plan.row0[at], expert = plan.expert[at];
-        next.col = nullptr;
+        next.col[0] = nullptr;
         if (g < plan.count[at]) {
             if (OWN) {
-                next.col = own + static_cast<size_t>(row0 + g) * P * own_stride + 16 * j;
+                next.col[0] = own + static_cast<size_t>(row0 + g) * P * own_stride + 16 * j;
             } else {
-                next.col = p.h + static_cast<size_t>(row0 + g) * p.I + 16 * j;
+                next.col[0] = p.h + static_cast<size_t>(row0 + g) * p.I + 16 * j;
                 up = w8_up(__uint_as_float(__ldcg(p.h_max + row0 + g)));
             }
         }
@@ -759,7 +781,7 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
             next.at1 = next.at0 + 8;
         }
     };
-    auto fetch = [&]() { next.template fetch<BLOCK, kRaw>(own_stride); };
+    auto fetch = [&]() { next.template fetch<BLOCK, kRaw>(own_stride, 0); };
     if (n > 0) {
         enter();
         fetch();
@@ -776,10 +798,10 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
             for (int e = 0; e < 2; ++e)
                 if (2 * j + e < count) down[e] = 1.f / w8_up(__uint_as_float(__ldcg(p.h_max + row0 + 2 * j + e)));
         }
-        float sum[MW][4] = {};
+        float sum[1][MW][4] = {};
         for (int c = 0; c < stretch; ++c) {
             asm volatile("cp.async.wait_group %0;" ::"n"(w8_depth(MW) - 1) : "memory");
-            W8Ahead<P, MW> now = next;
+            W8Ahead<P, MW, 1> now = next;
             const float now_up = up;
             if (i + c + 1 < n) {
                 if (++next.k == items) {
@@ -789,8 +811,8 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
                 }
                 fetch();
             }
-            if constexpr (kRaw) w8_halves(now.b, now_up);
-            w8_item<P, MW>(ring.base + slot, now.b, now.s0, now.s1, sum);
+            if constexpr (kRaw) w8_halves(now.b[0], now_up);
+            w8_item<P, MW, 1>(ring.base + slot, now.b, now.s0, now.s1, sum);
             w8_issue<MW>(ring, slot, items, open);
             slot = slot + kItem == kRing ? 0 : slot + kItem;
         }
@@ -803,8 +825,8 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
                 float* to = my_sums + plan.token[row0 + r] * kChan + g;
 #pragma unroll
                 for (int m = 0; m < MW; ++m) {
-                    to[16 * m] += weight * sum[m][e];
-                    to[16 * m + 8] += weight * sum[m][2 + e];
+                    to[16 * m] += weight * sum[0][m][e];
+                    to[16 * m + 8] += weight * sum[0][m][2 + e];
                 }
             }
         }
@@ -937,6 +959,9 @@ static int w8_forward(W8Params p, const uint8_t* gate_up, const float* gate_up_s
     const int64_t sms = sm_count(), most = 2 * sms;
     // Thirty-two rows a warp where there are enough of them: half as many reads of the activations, which lie in L1 and L2, for the same weights.
     const bool wide = R * (p.I / 16) >= 8 * most, own = self && !wide && own_x <= kW8Own && own_h <= kW8Own;
+    // Sixteen rows a block where experts have that many: the weights of an expert with nine to sixteen rows are read and expanded once and not twice, but half as
+    // far ahead.  128 experts of 2048 x 768, top 8, us a layer with 8 and 16: 128 tokens 175 and 187, 160 194 and 192, 200 236 and 203, 256 296 and 248.
+    const int rb = R > 10 * static_cast<int64_t>(p.E) ? 2 : 1;
     int st = EQ_OK;
     p.h_max = self && !own ? w.h_max : nullptr;
     p.h16 = w.h16;
@@ -950,19 +975,20 @@ static int w8_forward(W8Params p, const uint8_t* gate_up, const float* gate_up_s
         p.shares = w.shares;
         p.x16 = f16 ? static_cast<const __half*>(p.x) : w.x16;
         p.x_scale = f16 ? nullptr : w.x_scale;
-        if (st == EQ_OK && !self) st = group_rows_launch(w.ids, static_cast<int>(R), p.E, false, kW8BlockRows, false, w.blocks, w.n_blocks, w.rows, nullptr, stream);
+        if (st == EQ_OK && !self) st = group_rows_launch(w.ids, static_cast<int>(R), p.E, false, rb * kW8BlockRows, false, w.blocks, w.n_blocks, w.rows, nullptr, stream);
     }
     if (st != EQ_OK) return st;
     p.w = gate_up;
     p.scale = gate_up_scale;
-    auto smem = [&](int mw) { return static_cast<size_t>(kW8Warps) * (w8_ring(mw) + 2 * mw * 32 * sizeof(float4)); };
+    auto smem = [&](int mw, int rb = 1) { return static_cast<size_t>(kW8Warps) * (w8_ring(mw) + 2 * mw * rb * 32 * sizeof(float4)); };
     if (self) {
         const int64_t tiles = R * (p.I / (wide ? 16 : 8)), at_once = own ? sms : most, grid = tiles < at_once ? tiles : at_once;
-        if (own) st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, !f16, 1>, grid, 1, smem(1) + plan + own_x, stream, p);
-        else if (wide) st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, false, 2>, grid, 1, smem(2) + plan, stream, p);
-        else st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, false, 1>, grid, 1, smem(1) + plan, stream, p);
+        if (own) st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, !f16, 1, 1>, grid, 1, smem(1) + plan + own_x, stream, p);
+        else if (wide) st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, false, 2, 1>, grid, 1, smem(2) + plan, stream, p);
+        else st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, false, 1, 1>, grid, 1, smem(1) + plan, stream, p);
     } else {
-        st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, false, false, false, 2>, most, 1, smem(2), stream, p);
+        st = rb == 2 ? w8_launch(moe_w8_tiles_kernel<T, BLOCK, false, false, false, 2, 2>, most, 1, smem(2, 2), stream, p)
+                     : w8_launch(moe_w8_tiles_kernel<T, BLOCK, false, false, false, 2, 1>, most, 1, smem(2), stream, p);
     }
     if (st != EQ_OK) return st;
     p.w = down;
@@ -979,7 +1005,8 @@ static int w8_forward(W8Params p, const uint8_t* gate_up, const float* gate_up_s
     }
     st = w8_launch(w8_parts_kernel, R, 1, 0, stream, static_cast<const float*>(w.h), p.I, w.h16, w.h_scale);
     if (st != EQ_OK) return st;
-    st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, false, true, false, 2>, most, 1, smem(2), stream, p);
+    st = rb == 2 ? w8_launch(moe_w8_tiles_kernel<T, BLOCK, false, true, false, 2, 2>, most, 1, smem(2, 2), stream, p)
+                 : w8_launch(moe_w8_tiles_kernel<T, BLOCK, false, true, false, 2, 1>, most, 1, smem(2), stream, p);
     if (st != EQ_OK) return st;
     const int64_t vecs = static_cast<int64_t>(p.T) * p.H / 4;
     return w8_launch(moe_w8_combine_kernel<T>, ceil_div(vecs, 256), 1, 0, stream, reinterpret_cast<const float4*>(w.rows_out), static_cast<const float*>(w.shares), vecs, p.H / 4,

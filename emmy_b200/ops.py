@@ -39,11 +39,15 @@ def _need_cuda(*tensors):
 
 def _need_here(*tensors):
     """_need_cuda, and every tensor on the current device, whose stream the call is queued on."""
-    _need_cuda(*tensors)
-    here = torch._C._cuda_getDevice()
+    here = None
     for t in tensors:
-        if t is not None and t.get_device() != here:
-            raise ValueError(f"a tensor is on cuda:{t.get_device()}, the current device is cuda:{here}: call under torch.cuda.device()")
+        if t is not None:
+            if not t.is_cuda or not t.is_contiguous():
+                _need_cuda(t)
+            if here is None:
+                here = torch._C._cuda_getDevice()
+            if t.get_device() != here:
+                raise ValueError(f"a tensor is on cuda:{t.get_device()}, the current device is cuda:{here}: call under torch.cuda.device()")
 
 
 def unpack_int4(words: torch.Tensor, fmt: str, along_rows: bool = False) -> torch.Tensor:

@@ -28,31 +28,32 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     y [T, N] is a linear's output for x [T, K]; a [L, R, K] (or [L, S, R, K] for a projection of S linears side by side whose widths are
     `sections`), b [L, N, R], scaling f32 [L], adapter_ids int32 [T].  `out` may be y."""
     _need_here(y, x, a, b, scaling, adapter_ids, out, workspace)
-    t, k = x.shape
-    n = y.shape[1]
-    adapters, s, r = a.shape[0], (a.shape[1] if a.dim() == 4 else 1), a.shape[-2]
-    if a.dim() not in (3, 4) or a.shape[-1] != k or tuple(b.shape) != (adapters, n, r) or y.shape[0] != t:
+    (t, k), n = x.shape, y.shape[1]
+    if a.dim() == 4:
+        adapters, s, r, ka = a.shape
+    else:
+        (adapters, r, ka), s = a.shape, 1
+    if ka != k or b.shape != (adapters, n, r) or y.shape != (t, n):
         raise ValueError(f"lora_add: y {tuple(y.shape)}, x {tuple(x.shape)}, a {tuple(a.shape)}, b {tuple(b.shape)} do not fit")
-    if scaling.shape != (adapters,) or adapter_ids.shape != (t,) or scaling.dtype != torch.float32 or adapter_ids.dtype != torch.int32:
+    if scaling.shape != (adapters,) or adapter_ids.shape != (t,) or scaling.dtype is not torch.float32 or adapter_ids.dtype is not torch.int32:
         raise ValueError("lora_add: scaling is f32 with one value per adapter, adapter_ids int32 with one per row")
     dtype = x.dtype
-    if dtype not in (torch.float16, torch.bfloat16) or y.dtype != dtype or a.dtype != dtype or b.dtype != dtype:
+    if not (dtype is y.dtype is a.dtype is b.dtype) or (dtype is not torch.bfloat16 and dtype is not torch.float16):
         raise ValueError(f"lora_add: y, x, a and b share one 16-bit dtype, got {y.dtype}, {x.dtype}, {a.dtype}, {b.dtype}")
-    if (len(sections) if sections is not None else 1) != s:
+    widths = _section_array(sections, n)
+    if len(widths) != s:
         raise ValueError(f"lora_add: a holds {s} sections, sections are {sections}")
     if out is None:
         out = torch.empty_like(y)
-    elif out.shape != y.shape or out.dtype != dtype:
+    elif out.shape != y.shape or out.dtype is not dtype:
         raise ValueError(f"lora_add: out {tuple(out.shape)} {out.dtype} does not fit y {tuple(y.shape)} {dtype}")
     lib = L.load()
-    ws = workspace
-    if ws is None and t > 256:
-        ws = _scratch(lib.eq_lora_workspace_bytes(t, adapters, s, r), x.device)
-    L.check(
-        lib.eq_lora_add(
-            y.data_ptr(), x.data_ptr(), a.data_ptr(), b.data_ptr(), scaling.data_ptr(), adapter_ids.data_ptr(), t, k, n, r, adapters, s,
-            C.addressof(_section_array(sections, n)), _DTYPE[dtype], out.data_ptr(), ws.data_ptr() if ws is not None else None,
-            ws.numel() if ws is not None else 0, _stream(),
-        )
+    if workspace is None and t > 256:
+        workspace = _scratch(lib.eq_lora_workspace_bytes(t, adapters, s, r), x.device)
+    status = lib.eq_lora_add(
+        y.data_ptr(), x.data_ptr(), a.data_ptr(), b.data_ptr(), scaling.data_ptr(), adapter_ids.data_ptr(), t, k, n, r, adapters, s, widths, _DTYPE[dtype],
+        out.data_ptr(), workspace.data_ptr() if workspace is not None else None, workspace.numel() if workspace is not None else 0, _stream(),
     )
+    if status:
+        L.check(status)
     return out
