@@ -20,13 +20,14 @@ __device__ __forceinline__ int group_scan(int v, int32_t* warp_sums) {
     }
     if (lane == 31) warp_sums[warp] = sum;
     __syncthreads();
-    int before = sum - v;
-    for (int w = 0; w < warp; ++w) before += warp_sums[w];
+    int others = lane < warp ? warp_sums[lane] : 0;  // (32 warps at most)
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) others += __shfl_xor_sync(0xFFFFFFFFu, others, d);
     __syncthreads();
-    return before;
+    return others + sum - v;
 }
 
-__global__ void __launch_bounds__(32 * kGroupWarps) group_rows_kernel(const int32_t* __restrict__ ids, int T, int keys, int keep_rest, int block_rows, int cut,
+__global__ void __launch_bounds__(32 * kGroupWarps) group_rows_kernel(const int32_t* __restrict__ ids, int T, int keys, int keep_rest, int block_shift, int cut,
                                                                       GroupBlock* __restrict__ blocks, int32_t* __restrict__ n_blocks, int32_t* rows,
                                                                       int* __restrict__ status) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -52,6 +53,7 @@ __global__ void __launch_bounds__(32 * kGroupWarps) group_rows_kernel(const int3
         for (int a = 0; a < kAhead; ++a) kind[a] = kind_of(t + 32 * a + lane);
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
+            if (t + 32 * a >= t1) break;
             const uint32_t same = __match_any_sync(0xFFFFFFFFu, kind[a]);
             if (kind[a] >= 0 && __ffs(same) - 1 == lane) mine[kind[a]] += __popc(same);
             __syncwarp();
@@ -86,6 +88,7 @@ __global__ void __launch_bounds__(32 * kGroupWarps) group_rows_kernel(const int3
         for (int a = 0; a < kAhead; ++a) kind[a] = kind_of(t + 32 * a + lane);
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
+            if (t + 32 * a >= t1) break;
             const uint32_t same = __match_any_sync(0xFFFFFFFFu, kind[a]);
             if (kind[a] >= 0) rows[mine[kind[a]] + __popc(same & ((1u << lane) - 1))] = t + 32 * a + lane;
             __syncwarp();
@@ -118,7 +121,8 @@ __global__ void __launch_bounds__(32 * kGroupWarps) group_rows_kernel(const int3
         }
         __syncthreads();
     }
-    auto blocks_of = [&](int n) { return (n + block_rows - 1) / block_rows; };
+    const int block_rows = 1 << block_shift;
+    auto blocks_of = [&](int n) { return (n + block_rows - 1) >> block_shift; };
     int bsum = 0;
     for (int i = from; i < to; ++i) bsum += blocks_of(kind_head[i]) + blocks_of(kind_rows[i] - kind_head[i]);
     int bat = group_scan(bsum, warp_sums);
@@ -131,10 +135,11 @@ __global__ void __launch_bounds__(32 * kGroupWarps) group_rows_kernel(const int3
         if (status) *status = 0;
     }
     __syncthreads();
-    for (int i = warp; i < kinds; i += warps) {  // a warp lists a kind's blocks
+    constexpr int kListers = 8;  // lanes that list a kind's blocks: most kinds have a few, a prompt's adapter hundreds
+    for (int i = tid / kListers; i < kinds; i += threads / kListers) {
         const int c = kind_rows[i], head = kind_head[i], first = kind_first[i], block = kind_block[i], heads = blocks_of(head);
-        for (int b = lane; b < heads + blocks_of(c - head); b += 32) {
-            const int r = b < heads ? b * block_rows : head + (b - heads) * block_rows;
+        for (int b = tid % kListers; b < heads + blocks_of(c - head); b += kListers) {
+            const int r = b < heads ? b << block_shift : head + ((b - heads) << block_shift);
             blocks[block + b].key = i < keys ? i : -1;
             blocks[block + b].first = first + r;
             blocks[block + b].count = min(block_rows, (b < heads ? head : c) - r);
@@ -146,6 +151,8 @@ int group_rows_launch(const int32_t* ids, int T, int keys, bool keep_rest, int b
                       int* status, cudaStream_t stream) {
     constexpr int kMost = 208 * 1024;
     static_assert((kGroupFew + 1) * (kGroupWarps + 4) * 4 <= kMost && (kGroupMaxKeys + 1) * (kGroupManyWarps + 4) * 4 <= kMost, "the counters");
+    int shift = 0;
+    while ((1 << shift) < block_rows) ++shift;
     EQ_REQUIRE(keys <= kGroupMaxKeys, EQ_ERR_UNSUPPORTED, "at most %d keys", kGroupMaxKeys);
     EQ_CUDA_OK(cudaFuncSetAttribute(group_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
     const int warps = keys <= kGroupFew ? kGroupWarps : kGroupManyWarps;
@@ -159,7 +166,7 @@ int group_rows_launch(const int32_t* ids, int T, int keys, bool keep_rest, int b
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    EQ_CUDA_OK(cudaLaunchKernelEx(&cfg, group_rows_kernel, ids, T, keys, static_cast<int>(keep_rest), block_rows, static_cast<int>(cut), blocks, n_blocks, rows, status));
+    EQ_CUDA_OK(cudaLaunchKernelEx(&cfg, group_rows_kernel, ids, T, keys, static_cast<int>(keep_rest), shift, static_cast<int>(cut), blocks, n_blocks, rows, status));
     return EQ_OK;
 }
 

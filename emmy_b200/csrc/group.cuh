@@ -19,7 +19,7 @@ inline int64_t group_max_blocks(int64_t T, int64_t keys, int64_t block_rows, boo
 }
 
 // rows[0, ..): the indices 0 .. T - 1 in order of their ids (those outside [0, keys) last, or left out unless keep_rest); blocks: each at
-// most block_rows rows of one key; n_blocks: how many; status (may be null): set to zero.  The rows of a key stay in their order.  One launch, a
+// most block_rows (a power of two) rows of one key; n_blocks: how many; status (may be null): set to zero.  The rows of a key stay in their order.  One launch, a
 // programmatic dependent.  cut: a key's rows are cut ahead of the last run of neighbours among them (kGroupRun rows and more), so that the prompt behind a few
 // rows that decode lies in blocks of neighbours.
 constexpr int kGroupMaxKeys = 4096;

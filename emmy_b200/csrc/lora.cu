@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid
     const float scaling = __ldg(p.scaling + adapter);
     float* part = reinterpret_cast<float*>(smem);  // [kRows][ranks]: this CTA's share of K
     float* red = part + kRows * ranks;             // [warps][kRows][kLoraPass + 8]; the split h lies here afterwards
-    lora_shrink<T, 2 * kChunks>(p, adapter, count, rows_s, part, red, cta * kLoraWarps + warp, ctas * kLoraWarps);
+    lora_shrink<T, kChunks + 1>(p, adapter, count, rows_s, part, red, cta * kLoraWarps + warp, ctas * kLoraWarps);
     lora_cluster_arrive();
 
     // ---- expand: this warp's groups of 32 columns, each in steps of 64 ranks; a step's B and its group's y are asked for one step ahead
@@ -906,7 +906,7 @@ static int lora_cluster(int64_t units, int most) {
 }
 
 static int lora_launch(void (*kernel)(const LoraParams), const LoraParams& p, int64_t grid, int cluster, size_t smem, cudaStream_t stream) {
-    EQ_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024));
+    if (smem > 48 * 1024) EQ_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(grid));
     cfg.blockDim = dim3(kLoraThreads);
