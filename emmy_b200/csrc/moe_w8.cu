@@ -19,7 +19,7 @@
 //   down     A cluster of CTAs has sixteen output channels of ALL the blocks: the picks of a token meet inside it (f32, a fixed order), y is written
 //            once, and nothing is combined in memory: no atomics, no counters.  It has routed the tokens and asked for its first weights before
 //            the launch ahead of it ends.
-// Where the activations are small (kW8Own bytes: a token or two) these two launches are the layer, one CTA an SM each, so that the second one is resident, has
+// Where the activations are small (kW8Own: a token or two) these two launches are the layer, one CTA an SM each, so that the second one is resident, has
 // routed and asked for its first weights while the first one runs.  Else w8_prep_kernel routes the tokens and brings x (of bf16) to f16 ahead of them.
 // Then no launch has to come between the two: the rows' largest values are found as they are written, and the second one splits what it reads of them.
 // Above, w8_prep_kernel and group.cu list the blocks, w8_parts_kernel splits the rows of silu * up (there are so many CTAs for each row that they would do it
@@ -39,15 +39,16 @@ namespace eq {
 constexpr int kW8Threads = 256;
 constexpr int kW8Warps = kW8Threads / 32;
 // A warp's items are MW x 16 rows x 128 elements, in a ring of w8_depth(MW).
-constexpr int w8_depth(int mw) { return mw == 1 ? 3 : 2; }
-constexpr int w8_ring(int mw) { return w8_depth(mw) * mw * 2048; }
+// With one CTA of either launch on an SM (few) it is deeper: half of what a warp reads is asked for at once.
+constexpr int w8_depth(int mw, bool few) { return few ? 5 : mw == 1 ? 3 : 2; }
+constexpr int w8_ring(int mw, bool few) { return w8_depth(mw, few) * mw * 2048; }
 constexpr int kW8SelfTokens = 32;       // tokens up to which the CTAs route and group themselves (one bit each of a word)
 constexpr int kW8SelfExperts = 256;
 constexpr int kW8MaxTopK = 16;
 constexpr int kW8SelfPicks = kW8SelfTokens * kW8MaxTopK;
 constexpr int kW8BlockRows = 8;
 constexpr int kW8PartsH = 2;            // value and remainder of silu(gate) * up
-constexpr int kW8Own = 32 * 1024;       // bytes of f16 activations that a CTA makes for itself
+constexpr int kW8Own = 36 * 1024;       // bytes of f16 activations that the two launches of a few tokens make for themselves, a CTA of either on an SM
 
 struct W8Params {
     const uint8_t* w;         // this phase's weights: gate_up [E][2I][H] or down [E][H][I]
@@ -495,10 +496,11 @@ __device__ __forceinline__ W8Block w8_block(const W8Params& p, const W8Plan& pla
 }
 
 // ------------------------------------------------------------------------------------------------ spans of whole tiles: gate_up; down, general form
-// OWN: the CTA brings x to f16.  RB: groups of eight rows that a block has at most.
-template <typename T, bool BLOCK, bool SELF, bool DOWN, bool OWN, int MW, int RB>
+// FEW: one CTA an SM, which brings x of bf16 to f16 itself.  RB: groups of eight rows that a block has at most.
+template <typename T, bool BLOCK, bool SELF, bool DOWN, bool FEW, int MW, int RB>
 __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __grid_constant__ W8Params p) {
-    constexpr int P = DOWN ? kW8PartsH : 1, kSums = MW * RB, kRing = w8_ring(MW), kItem = MW * 2048;
+    constexpr int P = DOWN ? kW8PartsH : 1, kSums = MW * RB, kRing = w8_ring(MW, FEW), kDepth = w8_depth(MW, FEW), kItem = MW * 2048;
+    constexpr bool OWN = FEW && !std::is_same<T, __half>::value;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ float own_scale[kW8SelfTokens];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -560,7 +562,7 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
     };
     if (n > 0) rows_of(skip);
 #pragma unroll 1
-    for (int d = 0; d < w8_depth(MW); ++d) w8_issue<MW>(ring, d * kItem, items, open);
+    for (int d = 0; d < kDepth; ++d) w8_issue<MW>(ring, d * kItem, items, open);
 
     if (DOWN) {
         asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -644,7 +646,7 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
         const int stretch = min(items - it, n - i);
         float sum[RB][MW][4] = {};
         for (int c = 0; c < stretch; ++c) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(w8_depth(MW) - 1) : "memory");
+            asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
             W8Ahead<P, MW, RB> now = next;
             if constexpr (RB == 2) {
                 fetch(1);
@@ -680,16 +682,16 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
     __syncthreads();
     // the shared tiles, in the order of the warps that have a part
     for (int t = warp; t < span; t += kW8Warps) {
-        const int64_t lo_item = static_cast<int64_t>(t) * items, hi_item = lo_item + items;
+        const Int lo_item = static_cast<Int>(t) * items, hi_item = lo_item + items;
         float sum[RB][MW][4] = {};
         int parts = 0;
         for (int w = 0; w < kW8Warps; ++w) {
-            const int64_t a = share(w), b = share(w + 1);
+            const Int a = share(w), b = share(w + 1);
             if (a >= hi_item || b <= lo_item || a == b || (a <= lo_item && b >= hi_item)) continue;
             ++parts;
 #pragma unroll
             for (int q = 0; q < kSums; ++q) {
-                const float4 v = part[((w * 2 + (static_cast<int>(a / items) == t ? 0 : 1)) * kSums + q) * 32 + lane];
+                const float4 v = part[((w * 2 + (a >= lo_item ? 0 : 1)) * kSums + q) * 32 + lane];
                 float(&to)[4] = sum[q / MW][q % MW];
                 to[0] += v.x;
                 to[1] += v.y;
@@ -713,7 +715,7 @@ __device__ __forceinline__ float w8_peer(const float* mine, uint32_t rank) {
 template <typename T, bool BLOCK, bool OWN, int MW>
 __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid_constant__ W8Params p) {
     constexpr bool kRaw = !OWN;
-    constexpr int P = kW8PartsH, kRing = w8_ring(MW), kItem = MW * 2048, kChan = 16 * MW;
+    constexpr int P = kW8PartsH, kRing = w8_ring(MW, OWN), kDepth = w8_depth(MW, OWN), kItem = MW * 2048, kChan = 16 * MW;
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, j = lane & 3;
@@ -746,7 +748,7 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
     if (n > 0) rows_of(ask, skip);
     auto open = [&]() { rows_of(++ask, 0); };
 #pragma unroll 1
-    for (int d = 0; d < w8_depth(MW); ++d) w8_issue<MW>(ring, d * kItem, items, open);
+    for (int d = 0; d < kDepth; ++d) w8_issue<MW>(ring, d * kItem, items, open);
 
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -800,7 +802,7 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
         }
         float sum[1][MW][4] = {};
         for (int c = 0; c < stretch; ++c) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(w8_depth(MW) - 1) : "memory");
+            asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
             W8Ahead<P, MW, 1> now = next;
             const float now_up = up;
             if (i + c + 1 < n) {
@@ -958,7 +960,7 @@ static int w8_forward(W8Params p, const uint8_t* gate_up, const float* gate_up_s
     const int64_t own_x = f16 ? 0 : static_cast<int64_t>(p.T) * (p.H + 8) * 2, own_h = R * kW8PartsH * (p.I + 8) * 2;
     const int64_t sms = sm_count(), most = 2 * sms;
     // Thirty-two rows a warp where there are enough of them: half as many reads of the activations, which lie in L1 and L2, for the same weights.
-    const bool wide = R * (p.I / 16) >= 8 * most, own = self && !wide && own_x <= kW8Own && own_h <= kW8Own;
+    const bool wide = R * (p.I / 16) >= 8 * most, own = self && !wide && own_x + own_h <= kW8Own;
     // Sixteen rows a block where experts have that many: the weights of an expert with nine to sixteen rows are read and expanded once and not twice, but half as
     // far ahead.  128 experts of 2048 x 768, top 8, us a layer with 8 and 16: 128 tokens 175 and 187, 160 194 and 192, 200 236 and 203, 256 296 and 248.
     const int rb = R > 10 * static_cast<int64_t>(p.E) ? 2 : 1;
@@ -980,10 +982,10 @@ static int w8_forward(W8Params p, const uint8_t* gate_up, const float* gate_up_s
     if (st != EQ_OK) return st;
     p.w = gate_up;
     p.scale = gate_up_scale;
-    auto smem = [&](int mw, int rb = 1) { return static_cast<size_t>(kW8Warps) * (w8_ring(mw) + 2 * mw * rb * 32 * sizeof(float4)); };
+    auto smem = [&](int mw, int rb = 1, bool few = false) { return static_cast<size_t>(kW8Warps) * (w8_ring(mw, few) + 2 * mw * rb * 32 * sizeof(float4)); };
     if (self) {
         const int64_t tiles = R * (p.I / (wide ? 16 : 8)), at_once = own ? sms : most, grid = tiles < at_once ? tiles : at_once;
-        if (own) st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, !f16, 1, 1>, grid, 1, smem(1) + plan + own_x, stream, p);
+        if (own) st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, true, 1, 1>, grid, 1, smem(1, 1, true) + plan + own_x, stream, p);
         else if (wide) st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, false, 2, 1>, grid, 1, smem(2) + plan, stream, p);
         else st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, false, 1, 1>, grid, 1, smem(1) + plan, stream, p);
     } else {
@@ -998,7 +1000,7 @@ static int w8_forward(W8Params p, const uint8_t* gate_up, const float* gate_up_s
         const int64_t slabs = p.H / (16 * mw);
         int cluster = 8;  // two CTAs an SM at most, one beside the launch ahead
         while (cluster > 1 && slabs * cluster > (own ? sms : most)) cluster /= 2;
-        const size_t bytes = static_cast<size_t>(kW8Warps) * (w8_ring(mw) + static_cast<size_t>(p.T) * 16 * mw * sizeof(float)) + plan;
+        const size_t bytes = static_cast<size_t>(kW8Warps) * (w8_ring(mw, own) + static_cast<size_t>(p.T) * 16 * mw * sizeof(float)) + plan;
         if (wide) return w8_launch(moe_w8_down_kernel<T, BLOCK, false, 2>, slabs * cluster, cluster, bytes, stream, p);
         return own ? w8_launch(moe_w8_down_kernel<T, BLOCK, true, 1>, slabs * cluster, cluster, bytes + own_h, stream, p)
                      : w8_launch(moe_w8_down_kernel<T, BLOCK, false, 1>, slabs * cluster, cluster, bytes, stream, p);
