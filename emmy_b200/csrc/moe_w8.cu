@@ -42,6 +42,9 @@ constexpr int kW8Warps = kW8Threads / 32;
 // With one CTA of either launch on an SM (few) it is deeper: half of what a warp reads is asked for at once.
 constexpr int w8_depth(int mw, bool few) { return few ? 5 : mw == 1 ? 3 : 2; }
 constexpr int w8_ring(int mw, bool few) { return w8_depth(mw, few) * mw * 2048; }
+// Their scales come with them: of sixteen rows eight pairs (rows g, g + 8), of a 128 x 128 block's rows all alike.
+constexpr int w8_scales(int mw, bool block) { return 64 * (block ? 1 : mw); }
+constexpr int w8_stage(int mw, bool few, bool block) { return w8_depth(mw, few) * w8_scales(mw, block); }
 constexpr int kW8SelfTokens = 32;       // tokens up to which the CTAs route and group themselves (one bit each of a word)
 constexpr int kW8SelfExperts = 256;
 constexpr int kW8MaxTopK = 16;
@@ -397,18 +400,37 @@ struct W8Ring {
     const uint8_t *top, *bottom;  // next item to ask for: this lane's bytes of rows g and g + 8
     int step;                     // bytes from sixteen rows to the next sixteen
     int left, room;               // items not asked for yet, in all and of the tile
+    uint32_t scales;              // where this lane's rows' scales go
+    const float *at0, *at1;       // theirs; per channel, those of the next sixteen rows `more` further
+    int more;
 };
 
-template <int MW, typename Open>
-__device__ __forceinline__ void w8_issue(W8Ring& r, uint32_t slot, int items, Open&& open) {
+__device__ __forceinline__ void w8_copy_scale(uint32_t to, const float* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+
+// The next item to stage `stage`.  (The lanes of a warp come here together: the scales are the one thing that they read from one another's copies.)
+template <bool BLOCK, int MW, typename Open>
+__device__ __forceinline__ void w8_issue(W8Ring& r, int stage, int items, Open&& open) {
     if (r.left > 0) {
-        const uint32_t to = r.base + slot;
+        const uint32_t to = r.base + stage * MW * 2048;
 #pragma unroll
         for (int m = 0; m < MW; ++m) {
             w8_copy(to + m * 2048, r.top + m * r.step);
             w8_copy(to + m * 2048 + 512, r.bottom + m * r.step);
             w8_copy(to + m * 2048 + 1024, r.top + m * r.step + 64);
             w8_copy(to + m * 2048 + 1536, r.bottom + m * r.step + 64);
+        }
+        if ((threadIdx.x & 3) == 0) {
+#pragma unroll
+            for (int m = 0; m < (BLOCK ? 1 : MW); ++m) {
+                w8_copy_scale(r.scales + stage * w8_scales(MW, BLOCK) + m * 8, r.at0 + m * r.more);
+                w8_copy_scale(r.scales + stage * w8_scales(MW, BLOCK) + m * 8 + 4, r.at1 + m * r.more);
+            }
+        }
+        if (BLOCK) {
+            ++r.at0;
+            ++r.at1;
         }
         r.top += 128;
         r.bottom += 128;
@@ -420,18 +442,29 @@ __device__ __forceinline__ void w8_issue(W8Ring& r, uint32_t slot, int items, Op
     }
     w8_commit();
 }
+// A stage's scales, once its copies and the warp have met.
+template <bool BLOCK, int MW>
+__device__ __forceinline__ void w8_read_scales(const W8Ring& r, int stage, float (&s0)[MW], float (&s1)[MW]) {
+#pragma unroll
+    for (int m = 0; m < MW; ++m) {
+        if (BLOCK && m) {  // sixteen rows lie in one block of 128, and so do thirty-two
+            s0[m] = s0[0];
+            s1[m] = s1[0];
+        } else {
+            asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(s0[m]), "=f"(s1[m]) : "r"(r.scales + stage * w8_scales(MW, BLOCK) + m * 8) : "memory");
+        }
+    }
+}
 
-// What a lane reads beside the weights, an item (half an item, with two groups of columns) ahead: its columns at its K indices, the two scales.
-template <int P, int MW, int RB>
+// What a lane reads beside the weights, an item (half an item, with two groups of columns) ahead: its columns at its K indices.
+template <int P, int RB>
 struct W8Ahead {
     uint4 b[RB][P][4 / RB];
-    float s0[MW], s1[MW];
     const void* col[RB];      // null: none
-    const float *at0, *at1;   // scales; where they are per channel, those of the next sixteen rows `more` further
-    int k, more;              // 128-element block
+    int k;                    // 128-element block
 
     // RAW: the column is f32, 32 of its values to b, for halves().  Else it is f16, `stride` elements between the parts.
-    template <bool BLOCK, bool RAW>
+    template <bool RAW>
     __device__ __forceinline__ void fetch(int stride, int half) {
         if constexpr (RAW) {
             static_assert(P == 2 && RB == 1, "32 values of f32 are two parts of f16");
@@ -447,12 +480,6 @@ struct W8Ahead {
                     for (int i = 0; i < 4 / RB; ++i)
                         b[c][p][i] = col[c] ? *reinterpret_cast<const uint4*>(static_cast<const __half*>(col[c]) + p * stride + k * 128 + (half + (i >> 1)) * 64 + (i & 1) * 8)
                                             : make_uint4(0, 0, 0, 0);
-        }
-        if (half) return;  // the scales are the item's
-#pragma unroll
-        for (int m = 0; m < MW; ++m) {  // sixteen rows lie in one block of 128, and so do thirty-two
-            s0[m] = BLOCK && m ? s0[0] : __ldg(at0 + (BLOCK ? k : m * more));
-            s1[m] = BLOCK && m ? s1[0] : __ldg(at1 + (BLOCK ? k : m * more));
         }
     }
 };
@@ -499,14 +526,15 @@ __device__ __forceinline__ W8Block w8_block(const W8Params& p, const W8Plan& pla
 // FEW: one CTA an SM, which brings x of bf16 to f16 itself.  RB: groups of eight rows that a block has at most.
 template <typename T, bool BLOCK, bool SELF, bool DOWN, bool FEW, int MW, int RB>
 __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __grid_constant__ W8Params p) {
-    constexpr int P = DOWN ? kW8PartsH : 1, kSums = MW * RB, kRing = w8_ring(MW, FEW), kDepth = w8_depth(MW, FEW), kItem = MW * 2048;
+    constexpr int P = DOWN ? kW8PartsH : 1, kSums = MW * RB, kRing = w8_ring(MW, FEW), kDepth = w8_depth(MW, FEW), kStage = w8_stage(MW, FEW, BLOCK);
     constexpr bool OWN = FEW && !std::is_same<T, __half>::value;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ float own_scale[kW8SelfTokens];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, j = lane & 3;
     float4* part = reinterpret_cast<float4*>(smem + kW8Warps * kRing);  // [warps][first, last tile][RB][MW][32]
-    W8Plan& plan = *reinterpret_cast<W8Plan*>(part + kW8Warps * 2 * kSums * 32);
+    unsigned char* scales = reinterpret_cast<unsigned char*>(part + kW8Warps * 2 * kSums * 32);  // [warps][kDepth]
+    W8Plan& plan = *reinterpret_cast<W8Plan*>(scales + kW8Warps * kStage);
     __half* own = reinterpret_cast<__half*>(reinterpret_cast<unsigned char*>(&plan) + (sizeof(W8Plan) + 15) / 16 * 16);  // [T][K + 8]
 
     if (!DOWN) {  // (the launches ahead of the down product each waited before they let the next start: the blocks may be read and weights asked for)
@@ -547,6 +575,8 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
     W8Ring ring;
     ring.base = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * kRing + lane * 16;
     ring.step = (DOWN ? 16 : 8) * K;
+    ring.scales = static_cast<uint32_t>(__cvta_generic_to_shared(scales)) + warp * kStage + g * (w8_scales(MW, BLOCK) / 8);
+    ring.more = DOWN ? 16 : 8;
     ring.left = n;
     ring.room = items - skip;
     int ask = first;  // tile of the next item to ask for
@@ -555,6 +585,13 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
         const int expert = w8_block<SELF>(p, plan, t.block).expert, rows = DOWN ? p.H : 2 * p.I, r0 = t.chan * MW * (DOWN ? 16 : 8) + g;
         ring.top = p.w + (static_cast<size_t>(expert) * rows + r0) * K + k * 128 + 16 * j;
         ring.bottom = ring.top + static_cast<size_t>(DOWN ? 8 : p.I) * K;
+        if (BLOCK) {
+            ring.at0 = p.scale + (static_cast<size_t>(expert) * (rows / 128) + (DOWN ? t.chan * MW / 8 : t.chan * MW / 16)) * items + k;
+            ring.at1 = DOWN ? ring.at0 : ring.at0 + static_cast<size_t>(p.I / 128) * items;
+        } else {
+            ring.at0 = p.scale + static_cast<size_t>(expert) * rows + r0;
+            ring.at1 = ring.at0 + (DOWN ? 8 : p.I);
+        }
     };
     auto open = [&]() {
         ++ask;
@@ -562,14 +599,13 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
     };
     if (n > 0) rows_of(skip);
 #pragma unroll 1
-    for (int d = 0; d < kDepth; ++d) w8_issue<MW>(ring, d * kItem, items, open);
+    for (int d = 0; d < kDepth; ++d) w8_issue<BLOCK, MW>(ring, d, items, open);
 
     if (DOWN) {
         asm volatile("griddepcontrol.wait;" ::: "memory");
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     }
-    W8Ahead<P, MW, RB> next;
-    next.more = DOWN ? 16 : 8;
+    W8Ahead<P, RB> next;
     int at = first;  // the tile that `next` is of
     next.k = skip;
     auto enter = [&]() {
@@ -588,16 +624,8 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
                 }
             }
         }
-        if (BLOCK) {
-            const int rows = (DOWN ? p.H : 2 * p.I) / 128;
-            next.at0 = p.scale + (static_cast<size_t>(blk.expert) * rows + (DOWN ? t.chan * MW / 8 : t.chan * MW / 16)) * items;
-            next.at1 = DOWN ? next.at0 : next.at0 + static_cast<size_t>(p.I / 128) * items;
-        } else {
-            next.at0 = p.scale + static_cast<size_t>(blk.expert) * (DOWN ? p.H : 2 * p.I) + t.chan * MW * (DOWN ? 16 : 8) + g;
-            next.at1 = next.at0 + (DOWN ? 8 : p.I);
-        }
     };
-    auto fetch = [&](int half) { next.template fetch<BLOCK, false>(K, half); };
+    auto fetch = [&](int half) { next.template fetch<false>(K, half); };
     // the finished sums of a tile (lane: channels g and g + 8, or gate and up of channel g; rows 2 j, 2 j + 1)
     auto finish = [&](int rel, const float (&sum)[RB][MW][4]) {
         const Tile t = tile_of(rel);
@@ -640,17 +668,21 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
         enter();
         fetch(0);
     }
-    uint32_t slot = 0;
+    int stage = 0;
     int rel = first, it = skip;
     for (int i = 0; i < n;) {
         const int stretch = min(items - it, n - i);
         float sum[RB][MW][4] = {};
         for (int c = 0; c < stretch; ++c) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
-            W8Ahead<P, MW, RB> now = next;
+            __syncwarp();
+            float s0[MW], s1[MW];
+            w8_read_scales<BLOCK, MW>(ring, stage, s0, s1);
+            const uint32_t slot = ring.base + stage * MW * 2048;
+            W8Ahead<P, RB> now = next;
             if constexpr (RB == 2) {
                 fetch(1);
-                w8_item<P, MW, RB>(ring.base + slot, now.b, now.s0, now.s1, sum);
+                w8_item<P, MW, RB>(slot, now.b, s0, s1, sum);
 #pragma unroll
                 for (int q = 0; q < 2 * P * 2; ++q) now.b[q & 1][(q >> 1) & (P - 1)][q / (2 * P)] = next.b[q & 1][(q >> 1) & (P - 1)][q / (2 * P)];
             }
@@ -662,9 +694,10 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
                 }
                 fetch(0);
             }
-            w8_item<P, MW, RB>(ring.base + slot + (RB - 1) * 1024, now.b, now.s0, now.s1, sum);
-            w8_issue<MW>(ring, slot, items, open);
-            slot = slot + kItem == kRing ? 0 : slot + kItem;
+            w8_item<P, MW, RB>(slot + (RB - 1) * 1024, now.b, s0, s1, sum);
+            __syncwarp();
+            w8_issue<BLOCK, MW>(ring, stage, items, open);
+            stage = stage + 1 == kDepth ? 0 : stage + 1;
         }
         if (stretch == items) {
             finish(rel, sum);
@@ -715,12 +748,13 @@ __device__ __forceinline__ float w8_peer(const float* mine, uint32_t rank) {
 template <typename T, bool BLOCK, bool OWN, int MW>
 __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid_constant__ W8Params p) {
     constexpr bool kRaw = !OWN;
-    constexpr int P = kW8PartsH, kRing = w8_ring(MW, OWN), kDepth = w8_depth(MW, OWN), kItem = MW * 2048, kChan = 16 * MW;
+    constexpr int P = kW8PartsH, kRing = w8_ring(MW, OWN), kDepth = w8_depth(MW, OWN), kStage = w8_stage(MW, OWN, BLOCK), kChan = 16 * MW;
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, j = lane & 3;
     float* sums = reinterpret_cast<float*>(smem + kW8Warps * kRing);  // [warps][T][kChan]
-    W8Plan& plan = *reinterpret_cast<W8Plan*>(sums + kW8Warps * p.T * kChan);
+    unsigned char* scales = reinterpret_cast<unsigned char*>(sums + kW8Warps * p.T * kChan);  // [warps][kDepth]
+    W8Plan& plan = *reinterpret_cast<W8Plan*>(scales + kW8Warps * kStage);
     __half* own = reinterpret_cast<__half*>(reinterpret_cast<unsigned char*>(&plan) + (sizeof(W8Plan) + 15) / 16 * 16);  // [picks][P][I + 8]
     uint32_t rank, ctas;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -738,17 +772,25 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
     W8Ring ring;
     ring.base = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * kRing + lane * 16;
     ring.step = 16 * p.I;
+    ring.scales = static_cast<uint32_t>(__cvta_generic_to_shared(scales)) + warp * kStage + g * (w8_scales(MW, BLOCK) / 8);
+    ring.more = 16;
     ring.left = n;
     ring.room = items - skip;
     int ask = first;
     auto rows_of = [&](int b, int k) {
         ring.top = p.w + (static_cast<size_t>(plan.expert[b]) * p.H + chan + g) * p.I + k * 128 + 16 * j;
         ring.bottom = ring.top + static_cast<size_t>(8) * p.I;
+        if (BLOCK) {
+            ring.at0 = ring.at1 = p.scale + (static_cast<size_t>(plan.expert[b]) * (p.H / 128) + chan / 128) * items + k;
+        } else {
+            ring.at0 = p.scale + static_cast<size_t>(plan.expert[b]) * p.H + chan + g;
+            ring.at1 = ring.at0 + 8;
+        }
     };
     if (n > 0) rows_of(ask, skip);
     auto open = [&]() { rows_of(++ask, 0); };
 #pragma unroll 1
-    for (int d = 0; d < kDepth; ++d) w8_issue<MW>(ring, d * kItem, items, open);
+    for (int d = 0; d < kDepth; ++d) w8_issue<BLOCK, MW>(ring, d, items, open);
 
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -760,13 +802,12 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
                          [&](int r, float down) { plan.score[r] *= down; });
         __syncthreads();
     }
-    W8Ahead<P, MW, 1> next;
-    next.more = 16;
+    W8Ahead<P, 1> next;
     int at = first;
     next.k = skip;
     float up = 1.f;  // what brings this lane's row of h to f16
     auto enter = [&]() {
-        const int row0 = plan.row0[at], expert = plan.expert[at];
+        const int row0 = plan.row0[at];
         next.col[0] = nullptr;
         if (g < plan.count[at]) {
             if (OWN) {
@@ -776,20 +817,14 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
                 up = w8_up(__uint_as_float(__ldcg(p.h_max + row0 + g)));
             }
         }
-        if (BLOCK) {
-            next.at0 = next.at1 = p.scale + (static_cast<size_t>(expert) * (p.H / 128) + chan / 128) * items;
-        } else {
-            next.at0 = p.scale + static_cast<size_t>(expert) * p.H + chan + g;
-            next.at1 = next.at0 + 8;
-        }
     };
-    auto fetch = [&]() { next.template fetch<BLOCK, kRaw>(own_stride, 0); };
+    auto fetch = [&]() { next.template fetch<kRaw>(own_stride, 0); };
     if (n > 0) {
         enter();
         fetch();
     }
     float* my_sums = sums + warp * p.T * kChan;
-    uint32_t slot = 0;
+    int stage = 0;
     int rel = first, it = skip;
     for (int i = 0; i < n;) {
         const int stretch = min(items - it, n - i);
@@ -803,7 +838,10 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
         float sum[1][MW][4] = {};
         for (int c = 0; c < stretch; ++c) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
-            W8Ahead<P, MW, 1> now = next;
+            __syncwarp();
+            float s0[MW], s1[MW];
+            w8_read_scales<BLOCK, MW>(ring, stage, s0, s1);
+            W8Ahead<P, 1> now = next;
             const float now_up = up;
             if (i + c + 1 < n) {
                 if (++next.k == items) {
@@ -814,9 +852,10 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
                 fetch();
             }
             if constexpr (kRaw) w8_halves(now.b[0], now_up);
-            w8_item<P, MW, 1>(ring.base + slot, now.b, now.s0, now.s1, sum);
-            w8_issue<MW>(ring, slot, items, open);
-            slot = slot + kItem == kRing ? 0 : slot + kItem;
+            w8_item<P, MW, 1>(ring.base + stage * MW * 2048, now.b, s0, s1, sum);
+            __syncwarp();
+            w8_issue<BLOCK, MW>(ring, stage, items, open);
+            stage = stage + 1 == kDepth ? 0 : stage + 1;
         }
         // this warp's part of the block's rows, weighted, to its tokens' sums (the rows of a block are different tokens)
 #pragma unroll
@@ -982,7 +1021,7 @@ static int w8_forward(W8Params p, const uint8_t* gate_up, const float* gate_up_s
     if (st != EQ_OK) return st;
     p.w = gate_up;
     p.scale = gate_up_scale;
-    auto smem = [&](int mw, int rb = 1, bool few = false) { return static_cast<size_t>(kW8Warps) * (w8_ring(mw, few) + 2 * mw * rb * 32 * sizeof(float4)); };
+    auto smem = [&](int mw, int rb = 1, bool few = false) { return static_cast<size_t>(kW8Warps) * (w8_ring(mw, few) + w8_stage(mw, few, BLOCK) + 2 * mw * rb * 32 * sizeof(float4)); };
     if (self) {
         const int64_t tiles = R * (p.I / (wide ? 16 : 8)), at_once = own ? sms : most, grid = tiles < at_once ? tiles : at_once;
         if (own) st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, true, 1, 1>, grid, 1, smem(1, 1, true) + plan + own_x, stream, p);
@@ -1000,7 +1039,7 @@ static int w8_forward(W8Params p, const uint8_t* gate_up, const float* gate_up_s
         const int64_t slabs = p.H / (16 * mw);
         int cluster = 8;  // two CTAs an SM at most, one beside the launch ahead
         while (cluster > 1 && slabs * cluster > (own ? sms : most)) cluster /= 2;
-        const size_t bytes = static_cast<size_t>(kW8Warps) * (w8_ring(mw, own) + static_cast<size_t>(p.T) * 16 * mw * sizeof(float)) + plan;
+        const size_t bytes = static_cast<size_t>(kW8Warps) * (w8_ring(mw, own) + w8_stage(mw, own, BLOCK) + static_cast<size_t>(p.T) * 16 * mw * sizeof(float)) + plan;
         if (wide) return w8_launch(moe_w8_down_kernel<T, BLOCK, false, 2>, slabs * cluster, cluster, bytes, stream, p);
         return own ? w8_launch(moe_w8_down_kernel<T, BLOCK, true, 1>, slabs * cluster, cluster, bytes + own_h, stream, p)
                      : w8_launch(moe_w8_down_kernel<T, BLOCK, false, 1>, slabs * cluster, cluster, bytes, stream, p);
