@@ -13,9 +13,9 @@
 //   expand   every CTA takes a share of the columns in groups of 32: rows as M, columns as N, R as K.  The columns of a group are dealt
 //            to the four MMA tiles so that a lane ends with eight neighbouring ones: y is read and written 16 bytes at a time.  The
 //            next group's B and y are on their way while a group is multiplied, the first one's before the CTAs have met.
-// Above, two, the first of them group.cu's list of the blocks; for larger calls (lora_block_rows) three: blocks of at most 128 rows, lora_shrink_kernel writes h, lora_expand_kernel adds B h to y in tiles of 128 rows x
-// 128 columns.  Both products run on tcgen05: the rows of a block lie anywhere, so the threads gather them by cp.async into the swizzled tile that
-// the MMA reads, one or two steps ahead; two CTAs an SM, so that the sums of one are turned and added while the other's copies land.
+// Above, two, the first of them group.cu's list of the blocks; for larger calls (lora_block_rows) three: blocks of at most 128 rows, lora_shrink_kernel
+// writes h, lora_expand_kernel adds B h to y in tiles of 128 rows x 128 columns.  Both products run on tcgen05.  The shrink's threads gather the rows of a
+// block, which lie anywhere, by cp.async into the swizzled tile that the MMA reads, three to six steps ahead; the expand's tiles come and go by TMA.
 // h is kept in f32 and enters the second product as two 16-bit numbers, value and remainder (bf16: 16 bits of fraction, f16: 22, after
 // the row is brought to the top of f16's range by a power of two): the result is rounded once, as it is stored.
 // Up to 16 rows a block, mma.sync and not tcgen05: a decode batch is bound by the bytes of A and B and by latency, and fragments need no trip through
@@ -199,7 +199,9 @@ __device__ __forceinline__ uint4 lora_add8(uint4 v, const float (&acc)[4][4], in
     return v;
 }
 
-// ------------------------------------------------------------------------------------------------ up to 256 rows (or more than 256 ranks): blocks of 16 rows
+// ------------------------------------------------------------------------------------------------ blocks of 16 rows
+// Bound by latency for few bytes: one row of K=N=4096, rank 16, takes 6.0 us a launch beside 0.04 us of bytes, 17 rows of K=14336 N=4096, rank 32, 8.9 us (0.8), and
+// by how soon A's and B's bytes are asked for: 256 rows of 64 adapters, K=5120 N=34816, rank 64, 91 us for 396 MB, 4.4 TB/s.
 // kChunks: of 32 ranks, what a lane asks for at a time; one where there are no more (K=14336 N=4096, rank 32, 17 rows 8.8 us against 10.2; three CTAs an
 // SM then, of 80 registers, 10.5).
 template <typename T, int kChunks>
@@ -960,7 +962,8 @@ static int lora_forward(LoraParams p, int64_t T_, int64_t L, unsigned char* base
         const int ctas = lora_cluster(units, 4);
         return lora_launch(p.R <= 32 ? lora_rows_kernel<T, 1> : lora_rows_kernel<T, 2>, p, units * ctas, ctas, static_cast<size_t>(16) * ranks * sizeof(float) + (red > split ? red : split), stream);
     }
-    // 64 steps of 5120 x 16 ranks, us: three stages .. six ..
+    // Steps ahead: six where two CTAs an SM have room for them.  24 adapters of rank 16, prompts, us a call with three and with six: 8192 rows of K=N=5120
+    // 82 and 73, 4096 of K=14336 N=5120 75 and 64.
     p.stages = kLoraStages * (kLoraSub + lora_stage_rows(ranks)) <= 110 * 1024 ? kLoraStages : 3;
     const size_t stages = p.stages * (kLoraSub + lora_stage_rows(ranks)), sums = static_cast<size_t>(kLoraRows) * (ranks + 4) * sizeof(float);
     const int ctas = lora_cluster(units, 3);

@@ -6,28 +6,31 @@
 // to f16 by one conversion a pair, exactly, whatever the activations' type, and these are brought to f16 without loss: a row of bf16 is multiplied by a power of
 // two that takes its largest value to [2^14, 2^15) (its eight bits are exact in f16 down to 2^-31 of that, and off by 2^-39 of it below); a row of silu(gate) * up,
 // in f32, the same way, as two numbers, value and remainder (2^-22 of itself, 2^-39 of the largest).  Products are mma.sync m16n8k16 with f32 sums.  The layer
-// rounds once, as y is stored.  (bf16 MMAs want two conversions and a packing more a pair: 264 instructions per 2 KB of weights where this takes ..., beside the
-// 89 cycles that HBM needs for them; 16 tokens of 128 experts of 2048 x 768 123 us a layer.  m16n8k32 on e4m3 parts of the activations converts both operands
-// inside every MMA: 189 us.)
+// rounds once, as y is stored.  (16 tokens of 128 experts of 2048 x 768 take 87 us a layer.  bf16 MMAs want two conversions and a packing more a pair, 264
+// instructions per 2 KB of weights beside the 89 cycles that HBM needs for them: 123 us.  m16n8k32 on e4m3 parts of the activations converts both
+// operands inside every MMA: 189 us.)
+//
+// What bounds it: the bytes of the picked experts, as long as few rows share one.  5 tokens of 8 experts of 4096 x 14336 stream them at 5.5 TB/s (194 us),
+// 16 tokens as above at 4.5 beside routing, the seam of the two products and their ends; one token (38 MB, 17.6 us, 5.8 at the rate of HBM) is a chain of latencies,
+// of which routing takes 2.8 us, the seam with the split of silu * up 2 and each product 4.  With more rows the MMAs' operands: 200 tokens 199 us for 93 of bytes.
 //
 // Up to 32 tokens and 256 experts:
-//   gate_up  Every CTA routes the tokens and groups the picks by expert itself: a block is at most eight rows (picks) of one expert, so
+//   gate_up  Every CTA groups the picks by expert itself: a block is at most eight rows (picks) of one expert, so
 //            an expert that several tokens picked is read once.  The blocks' tiles of eight gate and the same eight up rows (one MMA
 //            A operand of sixteen rows) are one stream, cut into equal spans over the CTAs and in a CTA into equal shares of 128-element items over its
 //            warps.  A tile's silu and product happen in the registers of whoever has its sums; tiles that several warps share meet in shared
 //            memory in warp order.
 //   down     A cluster of CTAs has sixteen output channels of ALL the blocks: the picks of a token meet inside it (f32, a fixed order), y is written
-//            once, and nothing is combined in memory: no atomics, no counters.  It has routed the tokens and asked for its first weights before
-//            the launch ahead of it ends.
-// Where the activations are small (kW8Own: a token or two) these two launches are the layer, one CTA an SM each, so that the second one is resident, has
-// routed and asked for its first weights while the first one runs.  Else w8_prep_kernel routes the tokens and brings x (of bf16) to f16 ahead of them.
+//            once, and nothing is combined in memory.  It has grouped the picks and asked for its first weights before the launch ahead of it ends.
+// Where the activations are small (kW8Own: a token or two) these two launches are the layer, one CTA an SM each, so that the second one is resident, has routed
+// too and asked for its first weights while the first one runs.  Else w8_prep_kernel routes the tokens and brings x (of bf16) to f16 ahead of them.
 // Then no launch has to come between the two: the rows' largest values are found as they are written, and the second one splits what it reads of them.
 // Above, w8_prep_kernel and group.cu list the blocks, w8_parts_kernel splits the rows of silu * up (there are so many CTAs for each row that they would do it
-// many times: 64 tokens of 128 experts 152 us for 149), and both products run as streams of tiles; the down rows go to memory in f32 and
+// many times: 64 tokens of 128 experts of 2048 x 768 152 us for 143), and both products run as streams of tiles; the down rows go to memory in f32 and
 // moe_w8_combine_kernel adds them.
 //
 // Weights reach a lane through a ring in shared memory that the lane fills by cp.async for itself (16 bytes of a row: K indices 16 j .. 16 j + 15
-// of each half of the item, in both operands alike), so no warp waits for another.  mma.sync and not tcgen05: with at most eight rows the weights'
+// of each half of the item, in both operands alike), the scales beside them, so no warp waits for another.  mma.sync and not tcgen05: with at most eight rows the weights'
 // bytes bound the layer.
 #include <type_traits>
 
@@ -39,13 +42,14 @@ namespace eq {
 constexpr int kW8Threads = 256;
 constexpr int kW8Warps = kW8Threads / 32;
 // A warp's items are MW x 16 rows x 128 elements, in a ring of w8_depth(MW).
-// With one CTA of either launch on an SM (few) it is deeper: half of what a warp reads is asked for at once.
+// With one CTA of either launch on an SM (few) it is deeper, half of what a warp reads asked for at once: a token of 128 experts of 2048 x 768 21.2 us with
+// three, 17.8 with five.  (Four and six: the two no longer fit one SM, 21.3.)
 constexpr int w8_depth(int mw, bool few) { return few ? 5 : mw == 1 ? 3 : 2; }
 constexpr int w8_ring(int mw, bool few) { return w8_depth(mw, few) * mw * 2048; }
 // Their scales come with them: of sixteen rows eight pairs (rows g, g + 8), of a 128 x 128 block's rows all alike.
 constexpr int w8_scales(int mw, bool block) { return 64 * (block ? 1 : mw); }
 constexpr int w8_stage(int mw, bool few, bool block) { return w8_depth(mw, few) * w8_scales(mw, block); }
-constexpr int kW8SelfTokens = 32;       // tokens up to which the CTAs route and group themselves (one bit each of a word)
+constexpr int kW8SelfTokens = 32;       // tokens up to which the CTAs group the picks themselves (one bit each of a word)
 constexpr int kW8SelfExperts = 256;
 constexpr int kW8MaxTopK = 16;
 constexpr int kW8SelfPicks = kW8SelfTokens * kW8MaxTopK;

@@ -312,11 +312,11 @@ int eq_moe_status(const void* workspace, int64_t T, int64_t E, int64_t topk, int
  * of the router (softmax, ties to the lowest id, renormalised: eq_moe_route).  Weights as the checkpoint stores them, expert-major:
  * gate_up e4m3 [E, 2I, H] (gate rows, then up rows), down e4m3 [E, H, I]; scales are multipliers, f32: block_scales = 0 per output channel,
  * [E, 2I] and [E, H]; 1 per 128 x 128 block (`weight_scale_inv`), [E, 2I/128, H/128] and [E, H/128, I/128].  Activations keep their 16 bits
- * (act_dtype EQ_F16 or EQ_BF16), sums are f32, silu(gate) * up is kept in 16 to 22 bits of fraction, y is rounded once: the weights' values of the
- * reference's FP8 experts (emmy/compiler/loader/quant.py:147-170) in the layer of eq_moe_w4a16.  In f16, |silu(gate) * up| has to stay below 65504.
- * A token whose logits hold a NaN has a result of NaN.
- * Every expert that is picked is read once per eight rows; up to 32 tokens and 256 experts the layer is two launches.  It takes any T, but is
- * built for decode batches: from about sixteen rows an expert on it is bound by its warp-level MMAs.
+ * (act_dtype EQ_F16 or EQ_BF16), sums are f32, silu(gate) * up keeps 22 bits of fraction, y is rounded once: the weights' values of the
+ * reference's FP8 experts (emmy/compiler/loader/quant.py:147-170) in the layer of eq_moe_w4a16.
+ * A token whose logits hold a NaN has a result of NaN.  (Its experts' other tokens are as they are without it.)
+ * A picked expert is read once for every eight rows (sixteen where experts have more than ten on average).  It takes any T, but is built for
+ * decode batches: from about eight rows an expert on it is bound by its warp-level MMAs and what feeds them.
  * E <= 1024, topk <= 16, H and I multiples of 128; gate_up, down, x and y 16-byte aligned; y may be x.  The workspace is 256-byte aligned
  * and written before it is read. */
 size_t eq_moe_w8a16_workspace_bytes(int64_t T, int64_t E, int64_t topk, int64_t H, int64_t I);
