@@ -362,6 +362,8 @@ class QuantMoE(nn.Module):
         want = ((e, n2 // 128, h // 128), (e, h // 128, n2 // 256)) if block else ((e, n2), (e, h))
         if (tuple(gate_up_scale.shape), tuple(down_scale.shape)) != want:
             raise ValueError(f"scales {tuple(gate_up_scale.shape)} and {tuple(down_scale.shape)} are neither per channel nor per 128 x 128 block")
+        if not {w_gate_up.dtype, w_down.dtype} <= {torch.uint8, torch.float8_e4m3fn}:
+            raise ValueError(f"expert weights are e4m3 (or its bits in uint8), got {w_gate_up.dtype} and {w_down.dtype}")
         bits = lambda t: t.view(torch.uint8).contiguous()
         self.packed_gate_up, self.packed_down = bits(w_gate_up), bits(w_down)
         self.gate_up_scale, self.down_scale = gate_up_scale.float().contiguous(), down_scale.float().contiguous()

@@ -465,7 +465,7 @@ def read_adapter(adapter_dir) -> dict[str, tuple[torch.Tensor, torch.Tensor, flo
     cfg = json.loads((Path(adapter_dir) / "adapter_config.json").read_text())
     if cfg.get("peft_type", "LORA") != "LORA":
         raise ValueError(f"adapter of type {cfg['peft_type']!r}, not LORA")
-    for key, plain in (("bias", (None, "none")), ("use_dora", (None, False)), ("fan_in_fan_out", (None, False)), ("modules_to_save", (None, []))):
+    for key, plain in (("bias", (None, "none")), ("use_dora", (None, False)), ("fan_in_fan_out", (None, False)), ("modules_to_save", (None, [])), ("layer_replication", (None, []))):
         if cfg.get(key) not in plain:
             raise ValueError(f"unsupported adapter: {key}={cfg[key]!r}")
     index = CheckpointIndex(adapter_dir)

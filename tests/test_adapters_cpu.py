@@ -71,7 +71,8 @@ def test_scales_stay_f32_when_the_module_changes_type():
 def test_fp8_experts_refuse_what_does_not_fit():
     z = torch.zeros(2, 256, 128, dtype=torch.uint8)
     d, s = z[:, :128].contiguous(), (torch.ones(2, 256), torch.ones(2, 128))
-    for bad in ((z, s[0], z, s[1]), (z[:, :192], s[0], d, s[1]), (z, s[1], d, s[1]), (z, torch.ones(2, 2, 1), d, s[1]), (z, torch.ones(2, 1, 1), d, torch.ones(2, 1, 1))):
+    for bad in ((z, s[0], z, s[1]), (z[:, :192], s[0], d, s[1]), (z, s[1], d, s[1]), (z, torch.ones(2, 2, 1), d, s[1]), (z, torch.ones(2, 1, 1), d, torch.ones(2, 1, 1)),
+                (z.view(torch.float8_e5m2), s[0], d, s[1]), (z, s[0], d.view(torch.int8), s[1])):
         with pytest.raises(ValueError):
             linear.QuantMoE(1).load_fp8_experts(*bad)
     linear.QuantMoE(1).load_fp8_experts(z, torch.ones(2, 2, 1), d, torch.ones(2, 1, 1))
@@ -101,7 +102,7 @@ def test_adapter_directories(tmp_path):
 
 def test_adapter_directories_that_are_refused(tmp_path):
     t = pair("m.q_proj", 4, 16, 24, 1)
-    for i, bad in enumerate((dict(bias="all"), dict(use_dora=True), dict(fan_in_fan_out=True), dict(modules_to_save=["lm_head"]), dict(peft_type="IA3"))):
+    for i, bad in enumerate((dict(bias="all"), dict(use_dora=True), dict(fan_in_fan_out=True), dict(modules_to_save=["lm_head"]), dict(layer_replication=[[0, 2]]), dict(peft_type="IA3"))):
         write_adapter(tmp_path / f"c{i}", t, **bad)
         with pytest.raises(ValueError):
             loader.read_adapter(tmp_path / f"c{i}")

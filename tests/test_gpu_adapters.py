@@ -207,3 +207,29 @@ def test_graphs_of_one_pool_replayed_in_turn():
             y.zero_()
             graph.replay()
             assert torch.equal(y, want)
+
+
+def test_calls_on_two_streams_at_once():
+    """Every form of both operators beside another call of itself: nothing is shared between calls."""
+    from emmy_b200 import ops_moe
+
+    jobs = []
+    for t, k, n, r, ids in ((7, 512, 384, 16, None), (300, 512, 384, 16, None), (4000, 1024, 4096, 64, [0] * 1500 + [1] * 2500)):
+        args = tl.make(t, k, [n], r, 3, BF16, seed=t, ids=ids)
+        jobs.append(lambda args=args: tl.call(args, None))
+    for t, e, h, i in ((1, 8, 256, 128), (20, 16, 512, 256), (60, 16, 512, 256)):
+        weights, _ = tm.experts(e, h, i, True, t)
+        x, logits = tm.inputs(t, e, h, BF16, t)
+        jobs.append(lambda x=x, logits=logits, weights=weights: ops_moe.moe_w8a16(x, logits, *weights, 2))
+    want = [job() for job in jobs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for turn in range(30):
+        for n, job in enumerate(jobs):
+            for shift, stream in enumerate(streams):
+                with torch.cuda.stream(stream):
+                    got.append(((n + 3 * shift) % len(jobs), jobs[(n + 3 * shift) % len(jobs)]()))
+    torch.cuda.synchronize()
+    for n, y in got:
+        assert torch.equal(y, want[n]), n
