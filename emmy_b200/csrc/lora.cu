@@ -90,50 +90,60 @@ __device__ __forceinline__ int lora_adapter(const LoraParams& p, int t) {
     return id >= 0 && id < p.L ? id : -1;
 }
 
-// A_l x of the block's rows, this warp's slice of K, all warps' sums added: part[r][n] is this CTA's share.  Ends behind a barrier of the CTA.
-template <typename T, int kUnroll>
+// A_l x of the block's rows, this warp's slice of K, all warps' sums added: part[r][n] is this CTA's share.  TILES x 8 ranks a pass, STEPS x 32 elements of K asked
+// for at once.  Ends behind a barrier of the CTA.
+template <typename T, int TILES, int STEPS>
 __device__ __forceinline__ void lora_shrink(const LoraParams& p, int adapter, int count, const int32_t* rows_s, float* part, float* red, int slice, int slices) {
-    constexpr int kRows = 16;
+    constexpr int kRows = 16, kPass = 8 * TILES;
+    static_assert(kPass <= kLoraPass, "the warps' sums");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, j = lane & 3;
     const int ranks = p.S * p.R;
     const T* x = static_cast<const T*>(p.x);
     const T* a = static_cast<const T*>(p.a) + static_cast<size_t>(adapter) * ranks * p.K;
     const int chunks = (p.K + 31) / 32;
-    const int c0 = static_cast<int>(static_cast<int64_t>(chunks) * slice / slices), c1 = static_cast<int>(static_cast<int64_t>(chunks) * (slice + 1) / slices);
+    const int c0 = chunks * slice / slices, c1 = chunks * (slice + 1) / slices;  // (2^23 x 64 at most)
     const T* x0 = g < count ? x + static_cast<size_t>(rows_s[g]) * p.K : nullptr;
     const T* x1 = g + 8 < count ? x + static_cast<size_t>(rows_s[g + 8]) * p.K : nullptr;
-    for (int col = 0; col < ranks; col += kLoraPass) {
-        float acc[4][4];
+    for (int col = 0; col < ranks; col += kPass) {
+        float acc[TILES][4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < TILES; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-#pragma unroll kUnroll
-        for (int c = c0; c < c1; ++c) {
-            const int k = 32 * c + 8 * j;
-            const bool in = k < p.K;  // K is a multiple of 8
+        for (int c = c0; c < c1; c += STEPS) {
             const uint4 zero = make_uint4(0, 0, 0, 0);
-            uint4 wv[4];
+            uint4 wv[STEPS][TILES], top[STEPS], bottom[STEPS];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) wv[n] = in && col + 8 * n < ranks ? __ldg(reinterpret_cast<const uint4*>(a + static_cast<size_t>(col + 8 * n + g) * p.K + k)) : zero;
-            const uint4 top = in && x0 ? __ldg(reinterpret_cast<const uint4*>(x0 + k)) : zero, bottom = in && x1 ? __ldg(reinterpret_cast<const uint4*>(x1 + k)) : zero;
+            for (int u = 0; u < STEPS; ++u) {
+                const int k = 32 * (c + u) + 8 * j;
+                const bool in = c + u < c1 && k < p.K;  // K is a multiple of 8
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                mma_16816<T>(acc[n], top.x, bottom.x, top.y, bottom.y, wv[n].x, wv[n].y);
-                mma_16816<T>(acc[n], top.z, bottom.z, top.w, bottom.w, wv[n].z, wv[n].w);
+                for (int n = 0; n < TILES; ++n)
+                    wv[u][n] = in && col + 8 * n < ranks ? __ldg(reinterpret_cast<const uint4*>(a + static_cast<size_t>(col + 8 * n + g) * p.K + k)) : zero;
+                top[u] = in && x0 ? __ldg(reinterpret_cast<const uint4*>(x0 + k)) : zero;
+                bottom[u] = in && x1 ? __ldg(reinterpret_cast<const uint4*>(x1 + k)) : zero;
+            }
+#pragma unroll
+            for (int u = 0; u < STEPS; ++u) {
+                if (c + u >= c1) break;
+#pragma unroll
+                for (int n = 0; n < TILES; ++n) {
+                    mma_16816<T>(acc[n], top[u].x, bottom[u].x, top[u].y, bottom[u].y, wv[u][n].x, wv[u][n].y);
+                    mma_16816<T>(acc[n], top[u].z, bottom[u].z, top[u].w, bottom[u].w, wv[u][n].z, wv[u][n].w);
+                }
             }
         }
         constexpr int kPitch = kLoraPass + 8;  // rows a quarter of the banks apart
         float* mine = red + warp * kRows * kPitch;
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < TILES; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) *reinterpret_cast<float2*>(mine + (8 * h + g) * kPitch + 8 * n + 2 * j) = make_float2(acc[n][2 * h], acc[n][2 * h + 1]);
         __syncthreads();
-        const int width = min(kLoraPass, ranks - col);
-        for (int i = tid; i < count * kLoraPass; i += kLoraThreads) {
-            const int r = i / kLoraPass, n = i % kLoraPass;
+        const int width = min(kPass, ranks - col);
+        for (int i = tid; i < count * kPass; i += kLoraThreads) {
+            const int r = i / kPass, n = i % kPass;
             if (n >= width) continue;
             float s = 0.f;
 #pragma unroll
@@ -188,26 +198,37 @@ __device__ __forceinline__ float lora_join(const float* part, int ranks, uint32_
     return down;
 }
 
+// Two neighbouring values plus v0 mul and v1 mul.
+template <typename T>
+__device__ __forceinline__ uint32_t lora_add2(uint32_t y, float v0, float v1, float mul) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&y));
+        const __half2 h = __floats2half2_rn(fmaf(v0, mul, f.x), fmaf(v1, mul, f.y));
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(fmaf(v0, mul, __uint_as_float(y << 16)), fmaf(v1, mul, __uint_as_float(y & 0xFFFF0000u)));
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
 // y + delta of eight neighbouring columns of a row: acc's columns as the four tiles of a group hold them (first of the lane's two rows, or second).
 template <typename T>
 __device__ __forceinline__ uint4 lora_add8(uint4 v, const float (&acc)[4][4], int second, float mul) {
-    T* e = reinterpret_cast<T*>(&v);
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) e[2 * t + i] = from_float<T>(fmaf(second ? acc[t][2 + i] : acc[t][i], mul, to_float(e[2 * t + i])));
-    return v;
+    const int at = 2 * second;
+    return make_uint4(lora_add2<T>(v.x, acc[0][at], acc[0][at + 1], mul), lora_add2<T>(v.y, acc[1][at], acc[1][at + 1], mul),
+                      lora_add2<T>(v.z, acc[2][at], acc[2][at + 1], mul), lora_add2<T>(v.w, acc[3][at], acc[3][at + 1], mul));
 }
 
 // ------------------------------------------------------------------------------------------------ blocks of 16 rows
 // Bound by latency for few bytes: one row of K=N=4096, rank 16, takes 6.0 us a launch beside 0.04 us of bytes, 17 rows of K=14336 N=4096, rank 32, 8.9 us (0.8), and
 // by how soon A's and B's bytes are asked for: 256 rows of 64 adapters, K=5120 N=34816, rank 64, 91 us for 396 MB, 4.4 TB/s.
+// kSmall: no more than sixteen ranks in all, half the fragments, so more of them are asked for at once.
 // kChunks: of 32 ranks, what a lane asks for at a time; one where there are no more (K=14336 N=4096, rank 32, 17 rows 8.8 us against 10.2; three CTAs an
 // SM then, of 80 registers, 10.5).
-template <typename T, int kChunks>
+template <typename T, int kChunks, bool kSmall>
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid_constant__ LoraParams p) {
     constexpr int kRows = 16;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    static_assert(!kSmall || kChunks == 1, "");
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int32_t rows_s[kRows];
     __shared__ __align__(16) int32_t ids_s[kLoraSelfPlan];
@@ -274,28 +295,33 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid
     const float scaling = __ldg(p.scaling + adapter);
     float* part = reinterpret_cast<float*>(smem);  // [kRows][ranks]: this CTA's share of K
     float* red = part + kRows * ranks;             // [warps][kRows][kLoraPass + 8]; the split h lies here afterwards
-    lora_shrink<T, kChunks + 1>(p, adapter, count, rows_s, part, red, cta * kLoraWarps + warp, ctas * kLoraWarps);
+    lora_shrink<T, kSmall ? 2 : 4, kSmall ? 5 : kChunks + 1>(p, adapter, count, rows_s, part, red, cta * kLoraWarps + warp, ctas * kLoraWarps);
     lora_cluster_arrive();
 
     // ---- expand: this warp's groups of 32 columns, each in steps of 64 ranks; a step's B and its group's y are asked for one step ahead
     const T* b = static_cast<const T*>(p.b) + static_cast<size_t>(adapter) * p.N * p.R;
     const int groups = p.group_ends[p.S - 1];
-    const int g0 = static_cast<int>(static_cast<int64_t>(groups) * cta / ctas), g1 = static_cast<int>(static_cast<int64_t>(groups) * (cta + 1) / ctas);
+    const int g0 = groups * static_cast<int>(cta) / static_cast<int>(ctas), g1 = groups * static_cast<int>(cta + 1) / static_cast<int>(ctas);
     const bool has0 = g < count, has1 = g + 8 < count;
     const size_t y0 = static_cast<size_t>(rows_s[has0 ? g : 0]) * p.N, y1 = static_cast<size_t>(rows_s[has1 ? g + 8 : 0]) * p.N;
     struct Group {
         int section, first, end;  // columns
     };
-    auto group = [&](int gi) {
-        Group v;
-        v.section = 0;
-        while (gi >= p.group_ends[v.section]) ++v.section;
-        const int s = v.section;
-        v.first = (s ? p.ends[s - 1] : 0) + 32 * (gi - (s ? p.group_ends[s - 1] : 0));
-        v.end = p.ends[s];
-        return v;
+    int section = 0, groups_before = 0, columns_before = 0, group_end = p.group_ends[0], column_end = p.ends[0];
+    auto group = [&](int gi) {  // they ascend
+        while (gi >= group_end) {
+            groups_before = group_end;
+            columns_before = column_end;
+            ++section;
+            group_end = p.group_ends[section];
+            column_end = p.ends[section];
+        }
+        return Group{section, columns_before + 32 * (gi - groups_before), column_end};
     };
-    uint4 next_w[4][kChunks], next_y[2];
+    // (with sixteen ranks a lane has four of them, eight bytes of B, and three groups are on their way)
+    constexpr int kAhead = kSmall ? 3 : 1;
+    uint4 next_w[4][kChunks], next_y[kAhead][2];
+    uint2 next_s[kAhead][4] = {};  // (lanes without ranks keep the zeros; columns and rows that nobody stores keep what is there)
     auto ask_w = [&](const Group& v, int k0) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -307,17 +333,34 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid
             }
         }
     };
-    auto ask_y = [&](const Group& v) {
+    const int n_s = 8 * (g >> 1) + (g & 1);
+    const T* b_s = b + n_s * p.R + 4 * j;
+    auto ask_s = [&](const Group& v, uint2 (&to)[4]) {
+        const T* at = b_s + static_cast<size_t>(v.first) * p.R;
+        const int left = 4 * j < p.R ? v.end - v.first - n_s : 0;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            if (2 * t < left) to[t] = __ldg(reinterpret_cast<const uint2*>(at + 2 * t * p.R));
+    };
+    auto ask_y = [&](const Group& v, uint4 (&to)[2]) {
         const int n = v.first + 8 * j;
-        next_y[0] = has0 && n < v.end ? *reinterpret_cast<const uint4*>(yin + y0 + n) : make_uint4(0, 0, 0, 0);
-        next_y[1] = has1 && n < v.end ? *reinterpret_cast<const uint4*>(yin + y1 + n) : make_uint4(0, 0, 0, 0);
+        if (has0 && n < v.end) to[0] = *reinterpret_cast<const uint4*>(yin + y0 + n);
+        if (has1 && n < v.end) to[1] = *reinterpret_cast<const uint4*>(yin + y1 + n);
     };
     int gi = g0 + warp;
-    Group now = {}, ahead = {};
-    if (gi < g1) {
-        ahead = group(gi);
-        ask_w(ahead, 0);
-        ask_y(ahead);
+    Group ahead[kAhead] = {};
+    if constexpr (kSmall) {
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d)
+            if (gi + d * kLoraWarps < g1) {
+                ahead[d] = group(gi + d * kLoraWarps);
+                ask_s(ahead[d], next_s[d]);
+                ask_y(ahead[d], next_y[d]);
+            }
+    } else if (gi < g1) {
+        ahead[0] = group(gi);
+        ask_w(ahead[0], 0);
+        ask_y(ahead[0], next_y[0]);
     }
 
     // ---- h of the whole K, scaled and split; a warp takes a row
@@ -330,7 +373,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid
             lo_s[r * p.h_stride + n] = lo;
         };
         float mul;
-        if (ranks <= 128) mul = lora_join<T, 128>(part + r * ranks, ranks, ctas, scaling, put);
+        if (kSmall) mul = lora_join<T, 32>(part + r * ranks, ranks, ctas, scaling, put);
+        else if (ranks <= 128) mul = lora_join<T, 128>(part + r * ranks, ranks, ctas, scaling, put);
         else mul = lora_join<T, kChunks == 1 ? 32 * kLoraMaxSections : kLoraMaxRanks>(part + r * ranks, ranks, ctas, scaling, put);
         if (lane == 0) mul_s[r] = mul;
     }
@@ -339,8 +383,53 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid
 
     const float mul0 = mul_s[has0 ? g : 0], mul1 = mul_s[has1 ? g + 8 : 0];
     const int lo_at = kRows * p.h_stride;
+    auto put = [&](const Group& v, const uint4 (&yv)[2], const float (&acc)[4][4]) {
+        const int n = v.first + 8 * j;
+        if (n < v.end) {
+            if (has0) *reinterpret_cast<uint4*>(out + y0 + n) = lora_add8<T>(yv[0], acc, 0, mul0);
+            if (has1) *reinterpret_cast<uint4*>(out + y1 + n) = lora_add8<T>(yv[1], acc, 1, mul1);
+        }
+    };
+    if constexpr (kSmall) {
+        uint2 h[2][2] = {};  // value and remainder, rows g and g + 8, of a section
+        int has = -1;
+        for (; gi < g1; gi += kAhead * kLoraWarps) {
+#pragma unroll
+            for (int d = 0; d < kAhead; ++d) {
+                if (gi + d * kLoraWarps >= g1) break;
+                if (ahead[d].section != has) {
+                    has = ahead[d].section;
+                    const T* h_row = hi_s + g * p.h_stride + has * p.R + 4 * j;
+                    if (4 * j < p.R) {
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            h[half][0] = *reinterpret_cast<const uint2*>(h_row + half * lo_at);
+                            h[half][1] = *reinterpret_cast<const uint2*>(h_row + half * lo_at + 8 * p.h_stride);
+                        }
+                    }
+                }
+                float acc[4][4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) mma_16816<T>(acc[t], h[half][0].x, h[half][1].x, h[half][0].y, h[half][1].y, next_s[d][t].x, next_s[d][t].y);
+                put(ahead[d], next_y[d], acc);
+                if (gi + (d + kAhead) * kLoraWarps < g1) {
+                    ahead[d] = group(gi + (d + kAhead) * kLoraWarps);
+                    ask_s(ahead[d], next_s[d]);
+                    ask_y(ahead[d], next_y[d]);
+                }
+            }
+        }
+        lora_cluster_wait();  // no CTA leaves while another may read its sums
+        return;
+    }
     for (; gi < g1; gi += kLoraWarps) {
-        now = ahead;
+        const Group now = ahead[0];
         float acc[4][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t)
@@ -355,15 +444,15 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid
 #pragma unroll
                 for (int c = 0; c < kChunks; ++c) wv[t][c] = next_w[t][c];
             if (k0 == 0) {
-                yv[0] = next_y[0];
-                yv[1] = next_y[1];
+                yv[0] = next_y[0][0];
+                yv[1] = next_y[0][1];
             }
             if (k0 + 32 * kChunks < p.R) {
                 ask_w(now, k0 + 32 * kChunks);
             } else if (gi + kLoraWarps < g1) {
-                ahead = group(gi + kLoraWarps);
-                ask_w(ahead, 0);
-                ask_y(ahead);
+                ahead[0] = group(gi + kLoraWarps);
+                ask_w(ahead[0], 0);
+                ask_y(ahead[0], next_y[0]);
             }
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
@@ -373,8 +462,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     uint4 top = make_uint4(0, 0, 0, 0), bottom = make_uint4(0, 0, 0, 0);
-                    if (in && has0) top = *reinterpret_cast<const uint4*>(h_row + k + half * lo_at);
-                    if (in && has1) bottom = *reinterpret_cast<const uint4*>(h_row + k + half * lo_at + 8 * p.h_stride);
+                    if (in) top = *reinterpret_cast<const uint4*>(h_row + k + half * lo_at);
+                    if (in) bottom = *reinterpret_cast<const uint4*>(h_row + k + half * lo_at + 8 * p.h_stride);
 #pragma unroll
                     for (int t = 0; t < 4; ++t) {
                         mma_16816<T>(acc[t], top.x, bottom.x, top.y, bottom.y, wv[t][c].x, wv[t][c].y);
@@ -383,11 +472,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid
                 }
             }
         }
-        const int n = now.first + 8 * j;
-        if (n < now.end) {
-            if (has0) *reinterpret_cast<uint4*>(out + y0 + n) = lora_add8<T>(yv[0], acc, 0, mul0);
-            if (has1) *reinterpret_cast<uint4*>(out + y1 + n) = lora_add8<T>(yv[1], acc, 1, mul1);
-        }
+        put(now, yv, acc);
     }
     lora_cluster_wait();  // no CTA leaves while another may read its sums
 }
@@ -844,9 +929,9 @@ __global__ void __launch_bounds__(kLoraExpandThreads, 1)
                         tc::tmem_ld_wait();
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
-                            T* e = reinterpret_cast<T*>(&y[4 * h + c]);
+                            uint32_t* e = reinterpret_cast<uint32_t*>(&y[4 * h + c]);
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) e[i] = from_float<T>(fmaf(__uint_as_float(v[8 * c + i]), mul, to_float(e[i])));
+                            for (int i = 0; i < 4; ++i) e[i] = lora_add2<T>(e[i], __uint_as_float(v[8 * c + 2 * i]), __uint_as_float(v[8 * c + 2 * i + 1]), mul);
                         }
                     }
                 }
@@ -960,7 +1045,7 @@ static int lora_forward(LoraParams p, int64_t T_, int64_t L, unsigned char* base
         p.h_stride = (ranks + 63) / 64 * 64 + 32;  // rows 64 bytes apart modulo 128: the 16-byte reads of two rows meet every bank once
         const size_t red = static_cast<size_t>(kLoraWarps) * 16 * (kLoraPass + 8) * sizeof(float), split = 2 * static_cast<size_t>(16) * p.h_stride * 2;
         const int ctas = lora_cluster(units, 4);
-        return lora_launch(p.R <= 32 ? lora_rows_kernel<T, 1> : lora_rows_kernel<T, 2>, p, units * ctas, ctas, static_cast<size_t>(16) * ranks * sizeof(float) + (red > split ? red : split), stream);
+        return lora_launch(ranks <= 16 ? lora_rows_kernel<T, 1, true> : p.R <= 32 ? lora_rows_kernel<T, 1, false> : lora_rows_kernel<T, 2, false>, p, units * ctas, ctas, static_cast<size_t>(16) * ranks * sizeof(float) + (red > split ? red : split), stream);
     }
     // Steps ahead: six where two CTAs an SM have room for them.  24 adapters of rank 16, prompts, us a call with three and with six: 8192 rows of K=N=5120
     // 82 and 73, 4096 of K=14336 N=5120 75 and 64.

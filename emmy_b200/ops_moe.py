@@ -118,29 +118,32 @@ def moe_w8a16(x, router_logits, gate_up, gate_up_scale, down, down_scale, topk: 
     gate_up e4m3 bits [E, 2I, H] (uint8; gate rows, then up rows), down [E, H, I]; scales f32, per output channel ([E, 2I] and [E, H]) or
     per 128 x 128 block ([E, 2I / 128, H / 128] and [E, H / 128, I / 128])."""
     _need_here(x, router_logits, gate_up, gate_up_scale, down, down_scale, workspace, out)
-    t, h = x.shape
-    e, n2, k = gate_up.shape
-    i = down.shape[2]
-    if k != h or n2 != 2 * i or tuple(down.shape) != (e, h, i) or tuple(router_logits.shape) != (t, e):
+    (t, h), (e, n2, k), i = x.shape, gate_up.shape, down.shape[2]
+    if k != h or n2 != 2 * i or down.shape != (e, h, i) or router_logits.shape != (t, e):
         raise ValueError(f"moe_w8a16: x {tuple(x.shape)}, router_logits {tuple(router_logits.shape)}, gate_up {tuple(gate_up.shape)}, down {tuple(down.shape)} do not fit")
     block = gate_up_scale.dim() == 3
-    want = ((e, n2 // 128, h // 128), (e, h // 128, i // 128)) if block else ((e, n2), (e, h))
-    if (tuple(gate_up_scale.shape), tuple(down_scale.shape)) != want:
+    if block:
+        fits = gate_up_scale.shape == (e, n2 // 128, h // 128) and down_scale.shape == (e, h // 128, i // 128)
+    else:
+        fits = gate_up_scale.shape == (e, n2) and down_scale.shape == (e, h)
+    if not fits:
         raise ValueError(f"moe_w8a16: scales {tuple(gate_up_scale.shape)} and {tuple(down_scale.shape)} do not fit the weights")
-    if gate_up.dtype != torch.uint8 or down.dtype != torch.uint8 or any(v.dtype != torch.float32 for v in (router_logits, gate_up_scale, down_scale)):
+    f32, bits, dtype = torch.float32, torch.uint8, x.dtype
+    if not (gate_up.dtype is down.dtype is bits and router_logits.dtype is gate_up_scale.dtype is down_scale.dtype is f32):
         raise ValueError("moe_w8a16: weights are e4m3 bits in uint8, scales and router logits f32")
-    if x.dtype not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"moe_w8a16: activations are f16 or bf16, got {x.dtype}")
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise ValueError(f"moe_w8a16: activations are f16 or bf16, got {dtype}")
     if out is None:
         out = torch.empty_like(x)
-    elif out.shape != x.shape or out.dtype != x.dtype:
-        raise ValueError(f"moe_w8a16: out {tuple(out.shape)} {out.dtype} does not fit x {tuple(x.shape)} {x.dtype}")
+    elif out.shape != x.shape or out.dtype is not dtype:
+        raise ValueError(f"moe_w8a16: out {tuple(out.shape)} {out.dtype} does not fit x {tuple(x.shape)} {dtype}")
     lib = L.load()
-    ws = workspace if workspace is not None else _scratch(lib.eq_moe_w8a16_workspace_bytes(t, e, topk, h, i), x.device)
-    L.check(
-        lib.eq_moe_w8a16(
-            gate_up.data_ptr(), gate_up_scale.data_ptr(), down.data_ptr(), down_scale.data_ptr(), int(block), e, topk, h, i, x.data_ptr(),
-            router_logits.data_ptr(), t, _DTYPE[x.dtype], out.data_ptr(), ws.data_ptr(), ws.numel(), _stream(),
-        )
+    if workspace is None:
+        workspace = _scratch(lib.eq_moe_w8a16_workspace_bytes(t, e, topk, h, i), x.device)
+    status = lib.eq_moe_w8a16(
+        gate_up.data_ptr(), gate_up_scale.data_ptr(), down.data_ptr(), down_scale.data_ptr(), block, e, topk, h, i, x.data_ptr(),
+        router_logits.data_ptr(), t, _DTYPE[dtype], out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream(),
     )
+    if status:
+        L.check(status)
     return out
