@@ -219,8 +219,9 @@ __device__ __forceinline__ uint4 lora_add8(uint4 v, const float (&acc)[4][4], in
 }
 
 // ------------------------------------------------------------------------------------------------ blocks of 16 rows
-// Bound by latency for few bytes: one row of K=N=4096, rank 16, takes 6.0 us a launch beside 0.04 us of bytes, 17 rows of K=14336 N=4096, rank 32, 8.9 us (0.8), and
-// by how soon A's and B's bytes are asked for: 256 rows of 64 adapters, K=5120 N=34816, rank 64, 91 us for 396 MB, 4.4 TB/s.
+// Bound by latency for few bytes: one row of K=N=4096, rank 16, takes 4.9 us a launch beside 0.04 us of bytes, 17 rows of K=14336 N=4096, rank 32, 7.9 us (0.8), and
+// by how soon A's and B's bytes are asked for: 256 rows of 64 adapters, K=5120 N=34816, rank 64, 88 us for 396 MB, 4.5 TB/s.  With four warps a scheduler the
+// instructions between two loads are part of that latency: 64-bit divisions of the shares and zeros for what nobody stores were a fifth of either time.
 // kSmall: no more than sixteen ranks in all, half the fragments, so more of them are asked for at once.
 // kChunks: of 32 ranks, what a lane asks for at a time; one where there are no more (K=14336 N=4096, rank 32, 17 rows 8.8 us against 10.2; three CTAs an
 // SM then, of 80 registers, 10.5).
@@ -973,14 +974,16 @@ static size_t lora_align(size_t v) { return (v + 255) / 256 * 256; }
 static bool lora_wide(int64_t S, int64_t R) { return R <= kLoraWideRank && S <= kLoraMaxSections && S * R <= kLoraWideRanks; }
 
 // Rows of a block.  Above kLoraSelfPlan rows, 16 (lora_rows_kernel reads a block's A and B from L2 again for every 16 rows, and has one launch behind the list) up to
-// T (K + 2 N) max(R, 32) = 10^9, 128 from there on.  Both forced, 16 : 128, us, prompts of 3 adapters | with 100 rows that decode, of 16 adapters:
-//   K=N=4096, rank 16         600 rows 20 : 25 | 20 : 34, 1200 25 : 26 | 27 : 34, 2400 43 : 34 | 44 : 42, 4800 73 : 48 | 73 : 52
-//   K=4096 N=28672, rank 16   300 rows 29 : 30 | 30 : 73, 600 53 : 38 | 53 : 82, 1200 88 : 50 | 88 : 87, 4800 307 : 121 | 303 : 161
-//   K=14336 N=4096, rank 16   600 rows 25 : 35 | 26 : 45, 1200 40 : 37 | 41 : 46, 2400 67 : 46 | 67 : 64
-//   K=N=4096, rank 64         300 rows 19 : 24 | 19 : 31, 600 30 : 26 | 31 : 36, 1200 39 : 27 | 46 : 36; rank 128  300 rows 27 : 27 | 28 : 35, 600 45 : 29 | 47 : 41
+// T (K + 2 N) max(R, 32) = 2 10^9 for sixteen ranks in all, 7 10^8 for more; 128 from there on.  Both forced, 16 : 128, us, prompts of 3 adapters | with 100 rows
+// that decode, of 16 adapters:
+//   K=N=4096, rank 16         1200 rows (0.47 10^9) 21 : 25 | 21 : 34, 2400 (0.94) 32 : 32 | 33 : 42, 4800 (1.9) 53 : 50 | 53 : 49
+//   K=4096 N=28672, rank 16   300 rows (0.59) 22 : 30 | 24 : 72, 600 (1.2) 38 : 37 | 40 : 73, 1200 (2.4) 63 : 48 | 67 : 89, 2400 (4.7) 105 : 71 | 112 : 113
+//   K=14336 N=4096, rank 16   600 rows (0.43) 21 : 32 | 21 : 43, 1200 (0.87) 30 : 36 | 32 : 46, 2400 (1.7) 47 : 44 | 48 : 63
+//   K=N=4096, rank 32         600 rows (0.24) 19 : 22 | 19 : 32, 1200 (0.47) 25 : 25 | 26 : 34, 2400 (0.94) 42 : 33 | 42 : 38
+//   K=N=4096, rank 64         300 rows (0.24) 18 : 21 | 18 : 30, 600 (0.47) 29 : 23 | 29 : 33, 1200 (0.94) 37 : 26 | 41 : 36
 static int lora_block_rows(int64_t T, int64_t K, int64_t N, int64_t S, int64_t R) {
     if (T <= kLoraSelfPlan || !lora_wide(S, R)) return 16;
-    return static_cast<double>(T) * (K + 2 * N) * (R < 32 ? 32 : R) < 1e9 ? 16 : kLoraRows;
+    return static_cast<double>(T) * (K + 2 * N) * (R < 32 ? 32 : R) < (S * R <= 16 ? 2e9 : 7e8) ? 16 : kLoraRows;
 }
 static int64_t lora_units(int64_t T, int64_t L, int block_rows) { return group_max_blocks(T, L, block_rows, block_rows == kLoraRows); }
 

@@ -87,6 +87,8 @@ def call(args, sections, **kw):
         (900, 640, [4096, 136], 128, 3),
         (513, 4096, [2048], 40, 1),
         (3000, 128, [1000, 24, 5000], 64, 2),
+        (5000, 2048, [6000], 16, 3),
+        (4500, 1024, [3000, 4096], 8, 2),
     ],
 )
 def test_matches_the_formula(t, k, sections, r, adapters, dtype):
@@ -155,13 +157,13 @@ def test_scaling_of_zero_and_below():
     close(call(args, [64]), *args, [64])
 
 
-@pytest.mark.parametrize("r", [8, 64, 72, 128])
+@pytest.mark.parametrize("t,n,r", [(1111, 4104, 8), (1111, 4104, 64), (1111, 4104, 72), (1111, 4104, 128), (1500, 24584, 16), (1500, 24584, 64)])
 @pytest.mark.parametrize("order", ["prompts", "decode and prompts", "interleaved", "reversed"])
-def test_where_the_rows_of_a_block_lie(order, r):
+def test_where_the_rows_of_a_block_lie(order, t, n, r):
     """Neighbouring rows, few and many rows apart, ragged last quarters, blocks without an adapter; in place and not; the waits' word stays clear."""
     from emmy_b200 import lib as L
 
-    t, adapters, n = 1111, 7, 4104
+    adapters = 7
     i = torch.arange(t)
     ids = {
         "prompts": i * 5 // t - 1,
