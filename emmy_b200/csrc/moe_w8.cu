@@ -12,7 +12,7 @@
 //
 // What bounds it: the bytes of the picked experts, as long as few rows share one.  5 tokens of 8 experts of 4096 x 14336 stream them at 5.5 TB/s (194 us),
 // 16 tokens as above at 4.5 beside routing, the seam of the two products and their ends; one token (38 MB, 17.6 us, 5.8 at the rate of HBM) is a chain of latencies,
-// of which routing takes 2.8 us, the seam with the split of silu * up 2 and each product 4.  With more rows the MMAs' operands: 200 tokens 199 us for 93 of bytes.
+// of which routing takes 2.8 us, the seam with the split of silu * up 2 and each product 4.  With more rows the MMAs' operands: 200 tokens 189 us for 93 of bytes.
 //
 // Up to 32 tokens and 256 experts:
 //   gate_up  Every CTA groups the picks by expert itself: a block is at most eight rows (picks) of one expert, so
@@ -460,21 +460,32 @@ __device__ __forceinline__ void w8_read_scales(const W8Ring& r, int stage, float
     }
 }
 
-// What a lane reads beside the weights, an item (half an item, with two groups of columns) ahead: its columns at its K indices.
+// What a lane reads beside the weights, an item (half an item, with two groups of columns) ahead: its columns at its K indices.  Where a block has no such row they are
+// the first one's: nobody stores what comes of them, and nothing has to be filled with zeros.
+template <int P, int RB>
+using W8Columns = uint4[RB][P][4 / RB];
+template <int P, int RB>
+__device__ __forceinline__ void w8_copy_columns(W8Columns<P, RB>& to, const W8Columns<P, RB>& from) {
+#pragma unroll
+    for (int c = 0; c < RB; ++c)
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int i = 0; i < 4 / RB; ++i) to[c][p][i] = from[c][p][i];
+}
 template <int P, int RB>
 struct W8Ahead {
-    uint4 b[RB][P][4 / RB];
-    const void* col[RB];      // null: none
-    int k;                    // 128-element block
+    const void* col[RB];
+    int k;  // 128-element block
 
     // RAW: the column is f32, 32 of its values to b, for halves().  Else it is f16, `stride` elements between the parts.
     template <bool RAW>
-    __device__ __forceinline__ void fetch(int stride, int half) {
+    __device__ __forceinline__ void fetch(W8Columns<P, RB>& b, int stride, int half) const {
         if constexpr (RAW) {
             static_assert(P == 2 && RB == 1, "32 values of f32 are two parts of f16");
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                b[0][i >> 2][i & 3] = col[0] ? __ldcg(reinterpret_cast<const uint4*>(static_cast<const float*>(col[0]) + k * 128 + (i >> 2) * 64 + (i & 3) * 4)) : make_uint4(0, 0, 0, 0);
+                b[0][i >> 2][i & 3] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const float*>(col[0]) + k * 128 + (i >> 2) * 64 + (i & 3) * 4));
         } else {
 #pragma unroll
             for (int c = 0; c < RB; ++c)
@@ -482,8 +493,7 @@ struct W8Ahead {
                 for (int p = 0; p < P; ++p)
 #pragma unroll
                     for (int i = 0; i < 4 / RB; ++i)
-                        b[c][p][i] = col[c] ? *reinterpret_cast<const uint4*>(static_cast<const __half*>(col[c]) + p * stride + k * 128 + (half + (i >> 1)) * 64 + (i & 1) * 8)
-                                            : make_uint4(0, 0, 0, 0);
+                        b[c][p][i] = *reinterpret_cast<const uint4*>(static_cast<const __half*>(col[c]) + p * stride + k * 128 + (half + (i >> 1)) * 64 + (i & 1) * 8);
         }
     }
 };
@@ -610,6 +620,7 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     }
     W8Ahead<P, RB> next;
+    W8Columns<P, RB> b0, b1;  // the next ones, and those in hand (the second half's)
     int at = first;  // the tile that `next` is of
     next.k = skip;
     auto enter = [&]() {
@@ -617,19 +628,16 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
         const W8Block blk = w8_block<SELF>(p, plan, t.block);
 #pragma unroll
         for (int c = 0; c < RB; ++c) {
-            const int r = g + 8 * c;
-            next.col[c] = nullptr;
-            if (r < blk.count) {
-                if (DOWN) {
-                    next.col[c] = p.h16 + static_cast<size_t>(blk.row0 + r) * P * K + 16 * j;
-                } else {
-                    const int token = SELF ? plan.token[blk.row0 + r] : p.rows[blk.row0 + r] / p.topk;
-                    next.col[c] = (OWN ? own + static_cast<size_t>(token) * own_stride : p.x16 + static_cast<size_t>(token) * K) + 16 * j;
-                }
+            const int row = blk.row0 + (g + 8 * c < blk.count ? g + 8 * c : 0);
+            if (DOWN) {
+                next.col[c] = p.h16 + static_cast<size_t>(row) * P * K + 16 * j;
+            } else {
+                const int token = SELF ? plan.token[row] : p.rows[row] / p.topk;
+                next.col[c] = (OWN ? own + static_cast<size_t>(token) * own_stride : p.x16 + static_cast<size_t>(token) * K) + 16 * j;
             }
         }
     };
-    auto fetch = [&](int half) { next.template fetch<false>(K, half); };
+    auto fetch = [&](W8Columns<P, RB>& b, int half) { next.template fetch<false>(b, K, half); };
     // the finished sums of a tile (lane: channels g and g + 8, or gate and up of channel g; rows 2 j, 2 j + 1)
     auto finish = [&](int rel, const float (&sum)[RB][MW][4]) {
         const Tile t = tile_of(rel);
@@ -670,7 +678,7 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
 
     if (n > 0) {
         enter();
-        fetch(0);
+        fetch(b0, 0);
     }
     int stage = 0;
     int rel = first, it = skip;
@@ -683,22 +691,26 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_tiles_kernel(const __gri
             float s0[MW], s1[MW];
             w8_read_scales<BLOCK, MW>(ring, stage, s0, s1);
             const uint32_t slot = ring.base + stage * MW * 2048;
-            W8Ahead<P, RB> now = next;
-            if constexpr (RB == 2) {
-                fetch(1);
-                w8_item<P, MW, RB>(slot, now.b, s0, s1, sum);
-#pragma unroll
-                for (int q = 0; q < 2 * P * 2; ++q) now.b[q & 1][(q >> 1) & (P - 1)][q / (2 * P)] = next.b[q & 1][(q >> 1) & (P - 1)][q / (2 * P)];
-            }
-            if (i + c + 1 < n) {
-                if (++next.k == items) {
-                    next.k = 0;
-                    ++at;
-                    enter();
+            auto advance = [&](W8Columns<P, RB>& to) {
+                if (i + c + 1 < n) {
+                    if (++next.k == items) {
+                        next.k = 0;
+                        ++at;
+                        enter();
+                    }
+                    fetch(to, 0);
                 }
-                fetch(0);
+            };
+            if constexpr (RB == 2) {  // the halves of an item
+                fetch(b1, 1);
+                w8_item<P, MW, RB>(slot, b0, s0, s1, sum);
+                advance(b0);
+                w8_item<P, MW, RB>(slot + 1024, b1, s0, s1, sum);
+            } else {
+                w8_copy_columns<P, RB>(b1, b0);
+                advance(b0);
+                w8_item<P, MW, RB>(slot, b1, s0, s1, sum);
             }
-            w8_item<P, MW, RB>(slot + (RB - 1) * 1024, now.b, s0, s1, sum);
             __syncwarp();
             w8_issue<BLOCK, MW>(ring, stage, items, open);
             stage = stage + 1 == kDepth ? 0 : stage + 1;
@@ -771,7 +783,7 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
     __syncthreads();
     const int items = p.I / 128, chan = static_cast<int>(blockIdx.x / ctas) * kChan, own_stride = p.I + 8;
     const int total = plan.n_blocks * items, shares = kW8Warps * ctas, mine = rank * kW8Warps + warp;
-    const int q0 = static_cast<int>(static_cast<int64_t>(total) * mine / shares), n = static_cast<int>(static_cast<int64_t>(total) * (mine + 1) / shares) - q0;
+    const int q0 = total * mine / shares, n = total * (mine + 1) / shares - q0;  // (512 blocks of 512 items, 64 shares at most)
     const int first = q0 / items, skip = q0 - first * items;
     W8Ring ring;
     ring.base = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * kRing + lane * 16;
@@ -807,25 +819,24 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
         __syncthreads();
     }
     W8Ahead<P, 1> next;
+    W8Columns<P, 1> b0, b1;  // the next ones, and those in hand
     int at = first;
     next.k = skip;
     float up = 1.f;  // what brings this lane's row of h to f16
     auto enter = [&]() {
         const int row0 = plan.row0[at];
-        next.col[0] = nullptr;
-        if (g < plan.count[at]) {
-            if (OWN) {
-                next.col[0] = own + static_cast<size_t>(row0 + g) * P * own_stride + 16 * j;
-            } else {
-                next.col[0] = p.h + static_cast<size_t>(row0 + g) * p.I + 16 * j;
-                up = w8_up(__uint_as_float(__ldcg(p.h_max + row0 + g)));
-            }
+        const int row = row0 + (g < plan.count[at] ? g : 0);
+        if (OWN) {
+            next.col[0] = own + static_cast<size_t>(row) * P * own_stride + 16 * j;
+        } else {
+            next.col[0] = p.h + static_cast<size_t>(row) * p.I + 16 * j;
+            up = w8_up(__uint_as_float(__ldcg(p.h_max + row)));
         }
     };
-    auto fetch = [&]() { next.template fetch<kRaw>(own_stride, 0); };
+    auto fetch = [&](W8Columns<P, 1>& b) { next.template fetch<kRaw>(b, own_stride, 0); };
     if (n > 0) {
         enter();
-        fetch();
+        fetch(b0);
     }
     float* my_sums = sums + warp * p.T * kChan;
     int stage = 0;
@@ -845,7 +856,7 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
             __syncwarp();
             float s0[MW], s1[MW];
             w8_read_scales<BLOCK, MW>(ring, stage, s0, s1);
-            W8Ahead<P, 1> now = next;
+            w8_copy_columns<P, 1>(b1, b0);
             const float now_up = up;
             if (i + c + 1 < n) {
                 if (++next.k == items) {
@@ -853,10 +864,10 @@ __global__ void __launch_bounds__(kW8Threads, 2) moe_w8_down_kernel(const __grid
                     ++at;
                     enter();
                 }
-                fetch();
+                fetch(b0);
             }
-            if constexpr (kRaw) w8_halves(now.b[0], now_up);
-            w8_item<P, MW, 1>(ring.base + stage * MW * 2048, now.b, s0, s1, sum);
+            if constexpr (kRaw) w8_halves(b1[0], now_up);
+            w8_item<P, MW, 1>(ring.base + stage * MW * 2048, b1, s0, s1, sum);
             __syncwarp();
             w8_issue<BLOCK, MW>(ring, stage, items, open);
             stage = stage + 1 == kDepth ? 0 : stage + 1;
@@ -1005,8 +1016,9 @@ static int w8_forward(W8Params p, const uint8_t* gate_up, const float* gate_up_s
     // Thirty-two rows a warp where there are enough of them: half as many reads of the activations, which lie in L1 and L2, for the same weights.
     const bool wide = R * (p.I / 16) >= 8 * most, own = self && !wide && own_x + own_h <= kW8Own;
     // Sixteen rows a block where experts have that many: the weights of an expert with nine to sixteen rows are read and expanded once and not twice, but half as
-    // far ahead.  128 experts of 2048 x 768, top 8, us a layer with 8 and 16: 128 tokens 175 and 187, 160 194 and 192, 200 236 and 203, 256 296 and 248.
-    const int rb = R > 10 * static_cast<int64_t>(p.E) ? 2 : 1;
+    // far ahead.  128 experts of 2048 x 768, top 8, us a layer with 8 and 16: 96 tokens 149 and 171, 128 174 and 176, 144 180 and 180, 160 193 and 180, 200 236 and
+    // 189, 256 298 and 230; 64 experts, top 6: 96 tokens 161 and 165, 128 193 and 182.
+    const int rb = R > 9 * static_cast<int64_t>(p.E) ? 2 : 1;
     int st = EQ_OK;
     p.h_max = self && !own ? w.h_max : nullptr;
     p.h16 = w.h16;

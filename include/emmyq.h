@@ -315,7 +315,7 @@ int eq_moe_status(const void* workspace, int64_t T, int64_t E, int64_t topk, int
  * (act_dtype EQ_F16 or EQ_BF16), sums are f32, silu(gate) * up keeps 22 bits of fraction, y is rounded once: the weights' values of the
  * reference's FP8 experts (emmy/compiler/loader/quant.py:147-170) in the layer of eq_moe_w4a16.
  * A token whose logits hold a NaN has a result of NaN.  (Its experts' other tokens are as they are without it.)
- * A picked expert is read once for every eight rows (sixteen where experts have more than ten on average).  It takes any T, but is built for
+ * A picked expert is read once for every eight rows (sixteen where experts have more than nine on average).  It takes any T, but is built for
  * decode batches: from about eight rows an expert on it is bound by its warp-level MMAs and what feeds them.
  * E <= 1024, topk <= 16, H and I multiples of 128; gate_up, down, x and y 16-byte aligned; y may be x.  The workspace is 256-byte aligned
  * and written before it is read. */
