@@ -4,8 +4,8 @@
 // A_l[s], B_l is [N, R] over all of them.
 //
 // Up to 256 rows one launch, lora_rows_kernel.  A unit is a block of at most 16 rows of one adapter; a cluster of CTAs works on it:
-//   rows     which rows share an adapter is worked out by every CTA from the ids alone (a row's rank among the rows of its adapter; the rows
-//            whose rank is a multiple of 16 open a block).
+//   rows     which rows share an adapter is worked out by every CTA from the ids alone (a row's rank among the rows of its adapter, by a match in its
+//            warp and a table of the warps' counts; the rows whose rank is a multiple of 16 open a block).
 //   shrink   h = A_l x by mma.sync m16n8k16 (rows as M, ranks as N), K cut over all warps of the cluster: every byte of x and A_l is
 //            read by one warp, straight into the fragment's registers (16 bytes a lane: a lane's eight K values are the K indices
 //            {2j, 2j+1, 2j+8, 2j+9} of two steps, in both operands alike).  The warps' sums meet in shared memory in warp order, the
@@ -91,8 +91,8 @@ __device__ __forceinline__ int lora_adapter(const LoraParams& p, int t) {
 }
 
 // A_l x of the block's rows, this warp's slice of K, all warps' sums added: part[r][n] is this CTA's share.  TILES x 8 ranks a pass, STEPS x 32 elements of K asked
-// for at once.  Ends behind a barrier of the CTA.
-template <typename T, int TILES, int STEPS>
+// for at once; PASSES: there are several passes, the next one's first are asked for while the sums of one meet.  Ends behind a barrier of the CTA.
+template <typename T, int TILES, int STEPS, bool PASSES>
 __device__ __forceinline__ void lora_shrink(const LoraParams& p, int adapter, int count, const int32_t* rows_s, float* part, float* red, int slice, int slices) {
     constexpr int kRows = 16, kPass = 8 * TILES;
     static_assert(kPass <= kLoraPass, "the warps' sums");
@@ -105,6 +105,21 @@ __device__ __forceinline__ void lora_shrink(const LoraParams& p, int adapter, in
     const int c0 = chunks * slice / slices, c1 = chunks * (slice + 1) / slices;  // (2^23 x 64 at most)
     const T* x0 = g < count ? x + static_cast<size_t>(rows_s[g]) * p.K : nullptr;
     const T* x1 = g + 8 < count ? x + static_cast<size_t>(rows_s[g + 8]) * p.K : nullptr;
+    uint4 wv[STEPS][TILES], top[STEPS], bottom[STEPS];
+    auto load = [&](int col, int c) {
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int u = 0; u < STEPS; ++u) {
+            const int k = 32 * (c + u) + 8 * j;
+            const bool in = c + u < c1 && k < p.K;  // K is a multiple of 8
+#pragma unroll
+            for (int n = 0; n < TILES; ++n)
+                wv[u][n] = in && col + 8 * n < ranks ? __ldg(reinterpret_cast<const uint4*>(a + static_cast<size_t>(col + 8 * n + g) * p.K + k)) : zero;
+            top[u] = in && x0 ? __ldg(reinterpret_cast<const uint4*>(x0 + k)) : zero;
+            bottom[u] = in && x1 ? __ldg(reinterpret_cast<const uint4*>(x1 + k)) : zero;
+        }
+    };
+    if (PASSES) load(0, c0);
     for (int col = 0; col < ranks; col += kPass) {
         float acc[TILES][4];
 #pragma unroll
@@ -112,18 +127,7 @@ __device__ __forceinline__ void lora_shrink(const LoraParams& p, int adapter, in
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
         for (int c = c0; c < c1; c += STEPS) {
-            const uint4 zero = make_uint4(0, 0, 0, 0);
-            uint4 wv[STEPS][TILES], top[STEPS], bottom[STEPS];
-#pragma unroll
-            for (int u = 0; u < STEPS; ++u) {
-                const int k = 32 * (c + u) + 8 * j;
-                const bool in = c + u < c1 && k < p.K;  // K is a multiple of 8
-#pragma unroll
-                for (int n = 0; n < TILES; ++n)
-                    wv[u][n] = in && col + 8 * n < ranks ? __ldg(reinterpret_cast<const uint4*>(a + static_cast<size_t>(col + 8 * n + g) * p.K + k)) : zero;
-                top[u] = in && x0 ? __ldg(reinterpret_cast<const uint4*>(x0 + k)) : zero;
-                bottom[u] = in && x1 ? __ldg(reinterpret_cast<const uint4*>(x1 + k)) : zero;
-            }
+            if (!PASSES) load(col, c);
 #pragma unroll
             for (int u = 0; u < STEPS; ++u) {
                 if (c + u >= c1) break;
@@ -133,7 +137,9 @@ __device__ __forceinline__ void lora_shrink(const LoraParams& p, int adapter, in
                     mma_16816<T>(acc[n], top[u].z, bottom[u].z, top[u].w, bottom[u].w, wv[u][n].z, wv[u][n].w);
                 }
             }
+            if (PASSES && c + STEPS < c1) load(col, c + STEPS);
         }
+        if (PASSES && col + kPass < ranks) load(col + kPass, c0);
         constexpr int kPitch = kLoraPass + 8;  // rows a quarter of the banks apart
         float* mine = red + warp * kRows * kPitch;
 #pragma unroll
@@ -219,8 +225,8 @@ __device__ __forceinline__ uint4 lora_add8(uint4 v, const float (&acc)[4][4], in
 }
 
 // ------------------------------------------------------------------------------------------------ blocks of 16 rows
-// Bound by latency for few bytes: one row of K=N=4096, rank 16, takes 4.9 us a launch beside 0.04 us of bytes, 17 rows of K=14336 N=4096, rank 32, 7.9 us (0.8), and
-// by how soon A's and B's bytes are asked for: 256 rows of 64 adapters, K=5120 N=34816, rank 64, 88 us for 396 MB, 4.5 TB/s.  With four warps a scheduler the
+// Bound by latency for few bytes: one row of K=N=4096, rank 16, takes 5.0 us a launch beside 0.04 us of bytes, 17 rows of K=14336 N=4096, rank 32, 7.9 us (0.8), and
+// by how soon A's and B's bytes are asked for: 256 rows of 64 adapters, K=5120 N=34816, rank 64, 83 us for 396 MB, 4.8 TB/s.  With four warps a scheduler the
 // instructions between two loads are part of that latency: 64-bit divisions of the shares and zeros for what nobody stores were a fifth of either time.
 // kSmall: no more than sixteen ranks in all, half the fragments, so more of them are asked for at once.
 // kChunks: of 32 ranks, what a lane asks for at a time; one where there are no more (K=14336 N=4096, rank 32, 17 rows 8.8 us against 10.2; three CTAs an
@@ -232,7 +238,6 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid
     static_assert(!kSmall || kChunks == 1, "");
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int32_t rows_s[kRows];
-    __shared__ __align__(16) int32_t ids_s[kLoraSelfPlan];
     __shared__ int32_t lead_s[kLoraWarps];
     __shared__ int32_t block_s[3];
     __shared__ float mul_s[kRows];
@@ -246,16 +251,22 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid
     // ---- the unit's adapter and rows (the same for all CTAs of the cluster)
     int adapter = -1, count = 0;
     if (!p.blocks) {
-        int mine = -2, rank = 0;
-        if (tid < p.T) mine = lora_adapter(p, tid);
-        ids_s[tid] = mine;
+        // a row's rank: the rows of its kind ahead of it in its warp, and those that the warps before counted, a byte a warp
+        const int mine = tid < p.T ? lora_adapter(p, tid) : -2;
+        const uint32_t same = __match_any_sync(0xFFFFFFFFu, mine);
+        int rank = __popc(same & ((1u << lane) - 1));
         if (tid == 0) block_s[0] = -2;
-        __syncthreads();
-        for (int i = 0; i < (p.T & ~3); i += 4) {
-            const int4 v = *reinterpret_cast<const int4*>(ids_s + i);
-            rank += (v.x == mine && i < tid) + (v.y == mine && i + 1 < tid) + (v.z == mine && i + 2 < tid) + (v.w == mine && i + 3 < tid);
+        if (p.T > 32) {
+            uint2* counts = reinterpret_cast<uint2*>(smem);  // [L + 1]
+            const int kind = mine >= 0 ? mine : p.L;
+            for (int i = tid; i <= p.L; i += kLoraThreads) counts[i] = make_uint2(0, 0);
+            __syncthreads();
+            if (tid < p.T && rank == 0) reinterpret_cast<uint8_t*>(counts + kind)[warp] = static_cast<uint8_t>(__popc(same));
+            __syncthreads();
+            const uint2 others = counts[kind];
+            const uint64_t ahead_of = ((static_cast<uint64_t>(others.y) << 32) | others.x) & ((uint64_t(1) << (8 * warp)) - 1);
+            rank = static_cast<int>(__dp4a(static_cast<uint32_t>(ahead_of), 0x01010101u, __dp4a(static_cast<uint32_t>(ahead_of >> 32), 0x01010101u, static_cast<uint32_t>(rank))));
         }
-        for (int i = p.T & ~3; i < p.T; ++i) rank += ids_s[i] == mine && i < tid;
         const bool leads = tid < p.T && rank % kRows == 0 && !(mine < 0 && p.in_place);
         const uint32_t leaders = __ballot_sync(0xFFFFFFFFu, leads);
         if (lane == 0) lead_s[warp] = __popc(leaders);
@@ -296,7 +307,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid
     const float scaling = __ldg(p.scaling + adapter);
     float* part = reinterpret_cast<float*>(smem);  // [kRows][ranks]: this CTA's share of K
     float* red = part + kRows * ranks;             // [warps][kRows][kLoraPass + 8]; the split h lies here afterwards
-    lora_shrink<T, kSmall ? 2 : 4, kSmall ? 5 : kChunks + 1>(p, adapter, count, rows_s, part, red, cta * kLoraWarps + warp, ctas * kLoraWarps);
+    lora_shrink<T, kSmall ? 2 : 4, kSmall ? 5 : kChunks + 1, kChunks == 2>(p, adapter, count, rows_s, part, red, cta * kLoraWarps + warp, ctas * kLoraWarps);
     lora_cluster_arrive();
 
     // ---- expand: this warp's groups of 32 columns, each in steps of 64 ranks; a step's B and its group's y are asked for one step ahead
@@ -1048,7 +1059,8 @@ static int lora_forward(LoraParams p, int64_t T_, int64_t L, unsigned char* base
         p.h_stride = (ranks + 63) / 64 * 64 + 32;  // rows 64 bytes apart modulo 128: the 16-byte reads of two rows meet every bank once
         const size_t red = static_cast<size_t>(kLoraWarps) * 16 * (kLoraPass + 8) * sizeof(float), split = 2 * static_cast<size_t>(16) * p.h_stride * 2;
         const int ctas = lora_cluster(units, 4);
-        return lora_launch(ranks <= 16 ? lora_rows_kernel<T, 1, true> : p.R <= 32 ? lora_rows_kernel<T, 1, false> : lora_rows_kernel<T, 2, false>, p, units * ctas, ctas, static_cast<size_t>(16) * ranks * sizeof(float) + (red > split ? red : split), stream);
+        const size_t counts = p.blocks || p.T <= 32 ? 0 : (static_cast<size_t>(L) + 1) * sizeof(uint2), work = static_cast<size_t>(16) * ranks * sizeof(float) + (red > split ? red : split);
+        return lora_launch(ranks <= 16 ? lora_rows_kernel<T, 1, true> : p.R <= 32 ? lora_rows_kernel<T, 1, false> : lora_rows_kernel<T, 2, false>, p, units * ctas, ctas, work > counts ? work : counts, stream);
     }
     // Steps ahead: six where two CTAs an SM have room for them.  24 adapters of rank 16, prompts, us a call with three and with six: 8192 rows of K=N=5120
     // 82 and 73, 4096 of K=14336 N=5120 75 and 64.
