@@ -42,11 +42,12 @@ def _need_here(*tensors):
     here = None
     for t in tensors:
         if t is not None:
-            if not t.is_cuda or not t.is_contiguous():
-                _need_cuda(t)
             if here is None:
+                if not t.is_cuda:
+                    _need_cuda(t)
                 here = torch._C._cuda_getDevice()
-            if t.get_device() != here:
+            if t.get_device() != here or not t.is_contiguous():  # (-1: not on a GPU)
+                _need_cuda(t)
                 raise ValueError(f"a tensor is on cuda:{t.get_device()}, the current device is cuda:{here}: call under torch.cuda.device()")
 
 
