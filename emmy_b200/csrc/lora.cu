@@ -3,7 +3,7 @@
 // A projection that holds several linears side by side (q, k and v; gate and up) has one A per linear: section s of the columns reads
 // A_l[s], B_l is [N, R] over all of them.
 //
-// Up to 256 rows one launch, lora_rows_kernel.  A unit is a block of at most 16 rows of one adapter; a cluster of CTAs works on it:
+// Up to 256 rows, and up to 2048 where blocks have 16 rows (lora_block_rows), one launch, lora_rows_kernel.  A unit is a block of at most 16 rows of one adapter; a cluster of CTAs works on it:
 //   rows     which rows share an adapter is worked out by every CTA from the ids alone (a row's rank among the rows of its adapter, by a match in its
 //            warp and a table of the warps' counts; the rows whose rank is a multiple of 16 open a block).
 //   shrink   h = A_l x by mma.sync m16n8k16 (rows as M, ranks as N), K cut over all warps of the cluster: every byte of x and A_l is
@@ -13,7 +13,7 @@
 //   expand   every CTA takes a share of the columns in groups of 32: rows as M, columns as N, R as K.  The columns of a group are dealt
 //            to the four MMA tiles so that a lane ends with eight neighbouring ones: y is read and written 16 bytes at a time.  The
 //            next group's B and y are on their way while a group is multiplied, the first one's before the CTAs have met.
-// Above, two, the first of them group.cu's list of the blocks; for larger calls (lora_block_rows) three: blocks of at most 128 rows, lora_shrink_kernel
+// Above, two, the first of them group.cu's list of the blocks (1999 rows of K=N=5120, rank 16: 26 us, 23 with the list made by every CTA); for larger calls three: blocks of at most 128 rows, lora_shrink_kernel
 // writes h, lora_expand_kernel adds B h to y in tiles of 128 rows x 128 columns.  Both products run on tcgen05.  The shrink's threads gather the rows of a
 // block, which lie anywhere, by cp.async into the swizzled tile that the MMA reads, three to six steps ahead; the expand's tiles come and go by TMA.
 // h is kept in f32 and enters the second product as two 16-bit numbers, value and remainder (bf16: 16 bits of fraction, f16: 22, after
@@ -28,7 +28,8 @@ namespace eq {
 
 constexpr int kLoraThreads = 256;
 constexpr int kLoraWarps = kLoraThreads / 32;
-constexpr int kLoraSelfPlan = kLoraThreads;  // rows up to which a CTA works out the blocks itself, one row a thread
+constexpr int kLoraSelfPlan = kLoraThreads;  // rows up to which a CTA works out the blocks itself, one row a thread, and needs no workspace
+constexpr int kLoraSelfRows = 8 * kLoraThreads;  // and up to which it does so for blocks of 16 rows, eight rows a thread
 constexpr int kLoraMaxSections = 8;
 constexpr int kLoraMaxRanks = 1024;          // S * R
 constexpr int kLoraWideRanks = 256;          // S * R, and
@@ -48,7 +49,7 @@ struct LoraParams {
     const float* scaling; // [L]
     const int32_t* ids;   // [T]
     void* out;            // [T][N], may be y
-    GroupBlock* blocks;        // above kLoraSelfPlan rows
+    GroupBlock* blocks;        // null: the CTAs work them out
     const int32_t* n_blocks;
     const int32_t* rows;
     void* hi;             // [T][S x R rounded up to 16] h of the rows in their order of `rows`, value and remainder
@@ -250,7 +251,81 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_rows_kernel(const __grid
     asm volatile("griddepcontrol.wait;" ::: "memory");  // everything read below may come from the kernel before
     // ---- the unit's adapter and rows (the same for all CTAs of the cluster)
     int adapter = -1, count = 0;
-    if (!p.blocks) {
+    if (!p.blocks && p.T > kLoraSelfPlan) {
+        // Every warp has a run of neighbouring rows and counts the kinds in it; the blocks lie in the order of their kinds, rows without an adapter last.
+        if (blockIdx.x == 0 && tid == 0) *p.status = 0;
+        uint4* counts = reinterpret_cast<uint4*>(smem);  // [L + 1] rows of each warp, 16 bits
+        if (tid == 0) block_s[0] = -2;
+        for (int i = tid; i <= p.L; i += kLoraThreads) counts[i] = make_uint4(0, 0, 0, 0);
+        constexpr int kMine = kLoraSelfRows / kLoraThreads;
+        const int steps = (p.T + kLoraThreads - 1) / kLoraThreads, t0 = 32 * steps * warp + lane;
+        int kind[kMine], rank[kMine];
+#pragma unroll
+        for (int c = 0; c < kMine; ++c) {
+            kind[c] = -1;
+            if (c < steps && t0 + 32 * c < p.T) {
+                const int id = lora_adapter(p, t0 + 32 * c);
+                kind[c] = id >= 0 ? id : p.L;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < kMine; ++c) {
+            if (c >= steps) break;
+            const uint32_t same = __match_any_sync(0xFFFFFFFFu, kind[c]);
+            uint16_t* mine = reinterpret_cast<uint16_t*>(counts + max(kind[c], 0)) + warp;
+            const int before = kind[c] >= 0 ? *mine : 0;
+            rank[c] = before + __popc(same & ((1u << lane) - 1));
+            __syncwarp();
+            if (kind[c] >= 0 && __ffs(same) - 1 == lane) *mine = static_cast<uint16_t>(before + __popc(same));
+            __syncwarp();
+        }
+        __syncthreads();
+        // rows of kind i in the first `warps` warps' runs
+        auto rows_of = [&](int i, int warps) {
+            const uint4 v = counts[i];
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            uint32_t sum = 0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) sum += (2 * q < warps ? w[q] & 0xFFFFu : 0u) + (2 * q + 1 < warps ? w[q] >> 16 : 0u);
+            return static_cast<int>(sum);
+        };
+        const int kinds = p.in_place ? p.L : p.L + 1, per = (kinds + kLoraThreads - 1) / kLoraThreads, from_kind = min(tid * per, kinds), to_kind = min(from_kind + per, kinds);
+        int blocks = 0;
+        for (int i = from_kind; i < to_kind; ++i) blocks += (rows_of(i, kLoraWarps) + kRows - 1) / kRows;
+        int at = blocks;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int up = __shfl_up_sync(0xFFFFFFFFu, at, d);
+            if (lane >= d) at += up;
+        }
+        if (lane == 31) lead_s[warp] = at;
+        __syncthreads();
+        at -= blocks;
+        for (int w = 0; w < warp; ++w) at += lead_s[w];
+        if (at <= unit && unit < at + blocks) {
+            for (int i = from_kind; i < to_kind; ++i) {
+                const int n = rows_of(i, kLoraWarps), its = (n + kRows - 1) / kRows;
+                if (unit < at + its) {
+                    block_s[0] = i;
+                    block_s[1] = kRows * (unit - at);
+                    block_s[2] = min(kRows, n - block_s[1]);
+                    break;
+                }
+                at += its;
+            }
+        }
+        __syncthreads();
+        const int target = block_s[0];
+        if (target == -2) return;  // the whole cluster: fewer blocks than the launch allowed for
+        const int first = block_s[1] - rows_of(target, warp);
+#pragma unroll
+        for (int c = 0; c < kMine; ++c)
+            if (c < steps && kind[c] == target && rank[c] >= first && rank[c] < first + kRows) rows_s[rank[c] - first] = t0 + 32 * c;
+        adapter = target < p.L ? target : -1;
+        count = block_s[2];
+        __syncthreads();
+    } else if (!p.blocks) {
         // a row's rank: the rows of its kind ahead of it in its warp, and those that the warps before counted, a byte a warp
         const int mine = tid < p.T ? lora_adapter(p, tid) : -2;
         const uint32_t same = __match_any_sync(0xFFFFFFFFu, mine);
@@ -985,7 +1060,7 @@ static size_t lora_align(size_t v) { return (v + 255) / 256 * 256; }
 static bool lora_wide(int64_t S, int64_t R) { return R <= kLoraWideRank && S <= kLoraMaxSections && S * R <= kLoraWideRanks; }
 
 // Rows of a block.  Above kLoraSelfPlan rows, 16 (lora_rows_kernel reads a block's A and B from L2 again for every 16 rows, and has one launch behind the list) up to
-// T (K + 2 N) max(R, 32) = 2 10^9 for sixteen ranks in all, 7 10^8 for more; 128 from there on.  Both forced, 16 : 128, us, prompts of 3 adapters | with 100 rows
+// T (K + 2 N) max(R, 32) = 2 10^9 for sixteen ranks in all, 7 10^8 for more; 128 from there on.  Both forced (16 with a list, 3 us more), 16 : 128, us, prompts of 3 adapters | with 100 rows
 // that decode, of 16 adapters:
 //   K=N=4096, rank 16         1200 rows (0.47 10^9) 21 : 25 | 21 : 34, 2400 (0.94) 32 : 32 | 33 : 42, 4800 (1.9) 53 : 50 | 53 : 49
 //   K=4096 N=28672, rank 16   300 rows (0.59) 22 : 30 | 24 : 72, 600 (1.2) 38 : 37 | 40 : 73, 1200 (2.4) 63 : 48 | 67 : 89, 2400 (4.7) 105 : 71 | 112 : 113
@@ -1033,14 +1108,15 @@ static int lora_forward(LoraParams p, int64_t T_, int64_t L, unsigned char* base
     const int ranks = p.S * p.R, section_ranks = (p.R + 15) & ~15;
     const int block_rows = lora_block_rows(p.T, p.K, p.N, p.S, p.R);
     const int64_t units = lora_units(T_, L, block_rows);
-    if (p.T > kLoraSelfPlan) {
+    const bool self = block_rows == 16 && p.T <= kLoraSelfRows;
+    p.status = p.T > kLoraSelfPlan ? reinterpret_cast<int*>(base) : nullptr;
+    if (!self) {
         size_t o = 256;
         auto take = [&](size_t bytes) {
             void* at = base + o;
             o += lora_align(bytes);
             return at;
         };
-        p.status = reinterpret_cast<int*>(base);
         int32_t* n_blocks = reinterpret_cast<int32_t*>(base) + 1;
         GroupBlock* blocks = static_cast<GroupBlock*>(take(static_cast<size_t>(units) * sizeof(GroupBlock)));
         int32_t* rows = static_cast<int32_t*>(take(static_cast<size_t>(T_) * 4));
@@ -1059,7 +1135,7 @@ static int lora_forward(LoraParams p, int64_t T_, int64_t L, unsigned char* base
         p.h_stride = (ranks + 63) / 64 * 64 + 32;  // rows 64 bytes apart modulo 128: the 16-byte reads of two rows meet every bank once
         const size_t red = static_cast<size_t>(kLoraWarps) * 16 * (kLoraPass + 8) * sizeof(float), split = 2 * static_cast<size_t>(16) * p.h_stride * 2;
         const int ctas = lora_cluster(units, 4);
-        const size_t counts = p.blocks || p.T <= 32 ? 0 : (static_cast<size_t>(L) + 1) * sizeof(uint2), work = static_cast<size_t>(16) * ranks * sizeof(float) + (red > split ? red : split);
+        const size_t counts = p.blocks || p.T <= 32 ? 0 : (static_cast<size_t>(L) + 1) * (p.T > kLoraSelfPlan ? sizeof(uint4) : sizeof(uint2)), work = static_cast<size_t>(16) * ranks * sizeof(float) + (red > split ? red : split);
         return lora_launch(ranks <= 16 ? lora_rows_kernel<T, 1, true> : p.R <= 32 ? lora_rows_kernel<T, 1, false> : lora_rows_kernel<T, 2, false>, p, units * ctas, ctas, work > counts ? work : counts, stream);
     }
     // Steps ahead: six where two CTAs an SM have room for them.  24 adapters of rank 16, prompts, us a call with three and with six: 8192 rows of K=N=5120

@@ -87,6 +87,8 @@ def call(args, sections, **kw):
         (900, 640, [4096, 136], 128, 3),
         (513, 4096, [2048], 40, 1),
         (3000, 128, [1000, 24, 5000], 64, 2),
+        (2048, 128, [136], 16, 40),  # every CTA's own list of blocks, and one row more than it takes
+        (2049, 128, [136], 16, 40),
         (5000, 2048, [6000], 16, 3),
         (4500, 1024, [3000, 4096], 8, 2),
     ],
