@@ -403,6 +403,9 @@ class LoRALinear(nn.Module):
         self.sections = tuple(sections) if sections is not None else (base.out_features,)
         if slots < 1 or rank < 1 or sum(self.sections) != base.out_features:
             raise ValueError(f"{slots} slots of rank {rank}, sections {self.sections} of {base.out_features} outputs")
+        if slots > 4096 or len(self.sections) > 8 or len(self.sections) * self.rank > 1024 or any(v <= 0 or v % 8 for v in (self.in_features, *self.sections)):
+            raise ValueError(f"the kernels take up to 4096 slots, 8 sections, sections x rank up to 1024 and widths in eights; got {slots}, "
+                             f"{self.in_features} -> {self.sections}, rank {rank}")
         device = next((t.device for t in (*base.parameters(), *base.buffers())), None)
         make = lambda *shape, of=dtype: torch.zeros(shape, dtype=of, device=device)
         self.register_buffer("lora_a", make(slots, len(self.sections), self.rank, self.in_features), persistent=False)

@@ -52,7 +52,8 @@ def test_slots_refuse_what_does_not_fit():
                 dict(a=[torch.zeros(3, 8), None]), dict(b=[torch.zeros(16, 3), None]), dict(b=[torch.zeros(8, 4), None])):
         with pytest.raises(ValueError):
             m.check_adapter(**{**ok, **bad})
-    for bad in (dict(slots=0), dict(rank=0), dict(sections=(8, 8)), dict(dtype=torch.float32)):
+    for bad in (dict(slots=0), dict(rank=0), dict(sections=(8, 8)), dict(dtype=torch.float32), dict(slots=4097), dict(rank=1025), dict(rank=505, sections=(8, 8, 8)), dict(k=12),
+                dict(n=20), dict(sections=(12, 12)), dict(n=72, sections=(8,) * 9), dict(sections=(24, 8, -8))):
         with pytest.raises(ValueError):
             lora(**bad)
 
