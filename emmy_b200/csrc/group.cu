@@ -41,21 +41,26 @@ __global__ void __launch_bounds__(32 * kGroupWarps) group_rows_kernel(const int3
     const int t0 = min(static_cast<int64_t>(run) * warp, static_cast<int64_t>(T)), t1 = min(t0 + run, T);
     int32_t* mine = counts + warp * kinds;
     int32_t *kind_rows = counts + warps * kinds, *kind_first = kind_rows + kinds, *kind_head = kind_first + kinds, *kind_block = kind_head + kinds;
-    constexpr int kAhead = 4;  // ids in flight
-    auto kind_of = [&](int t) {
-        if (t >= t1) return -1;
-        const int id = ids[t];
-        return id >= 0 && id < keys ? id : keep_rest ? keys : -1;
+    constexpr int kAhead = 8;  // ids in flight; where a warp has no more, they are read and matched once
+    int kind[kAhead];
+    uint32_t same[kAhead];  // the lanes of the same kind
+    auto kinds_of = [&](int t) {
+        int id[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) id[a] = t + 32 * a + lane < t1 ? ids[t + 32 * a + lane] : -1;
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+            kind[a] = id[a] >= 0 && id[a] < keys ? id[a] : keep_rest && t + 32 * a + lane < t1 ? keys : -1;
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+            if (t + 32 * a < t1) same[a] = __match_any_sync(0xFFFFFFFFu, kind[a]);
     };
     for (int t = t0; t < t1; t += 32 * kAhead) {
-        int kind[kAhead];
-#pragma unroll
-        for (int a = 0; a < kAhead; ++a) kind[a] = kind_of(t + 32 * a + lane);
+        kinds_of(t);
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
             if (t + 32 * a >= t1) break;
-            const uint32_t same = __match_any_sync(0xFFFFFFFFu, kind[a]);
-            if (kind[a] >= 0 && __ffs(same) - 1 == lane) mine[kind[a]] += __popc(same);
+            if (kind[a] >= 0 && __ffs(same[a]) - 1 == lane) mine[kind[a]] += __popc(same[a]);
             __syncwarp();
         }
     }
@@ -83,16 +88,13 @@ __global__ void __launch_bounds__(32 * kGroupWarps) group_rows_kernel(const int3
     }
     __syncthreads();
     for (int t = t0; t < t1; t += 32 * kAhead) {
-        int kind[kAhead];
-#pragma unroll
-        for (int a = 0; a < kAhead; ++a) kind[a] = kind_of(t + 32 * a + lane);
+        if (run > 32 * kAhead) kinds_of(t);
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
             if (t + 32 * a >= t1) break;
-            const uint32_t same = __match_any_sync(0xFFFFFFFFu, kind[a]);
-            if (kind[a] >= 0) rows[mine[kind[a]] + __popc(same & ((1u << lane) - 1))] = t + 32 * a + lane;
+            if (kind[a] >= 0) rows[mine[kind[a]] + __popc(same[a] & ((1u << lane) - 1))] = t + 32 * a + lane;
             __syncwarp();
-            if (kind[a] >= 0 && __ffs(same) - 1 == lane) mine[kind[a]] += __popc(same);
+            if (kind[a] >= 0 && __ffs(same[a]) - 1 == lane) mine[kind[a]] += __popc(same[a]);
             __syncwarp();
         }
     }
