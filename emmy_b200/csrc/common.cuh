@@ -37,6 +37,10 @@ int fail(int status, const char* fmt, ...);
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Dynamic shared memory up to which a launch need not raise its kernel's limit: the 48 KB that every kernel has hold its static arrays too, which are
+// far below 16 KB in the kernels whose dynamic size varies.
+constexpr size_t kSmemUnasked = 32 * 1024;
+
 // Number of SMs of the current device (cached per device id).
 int sm_count();
 

@@ -986,7 +986,7 @@ static W8Workspace w8_carve(void* base, int64_t T, int64_t E, int64_t topk, int6
 
 template <typename... P, typename... A>
 static int w8_launch(void (*kernel)(P...), int64_t grid, int cluster, size_t smem, cudaStream_t stream, A... args) {
-    if (smem > 48 * 1024) EQ_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+    if (smem > kSmemUnasked) EQ_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(grid));
     cfg.blockDim = dim3(kW8Threads);
