@@ -180,14 +180,15 @@ __device__ __forceinline__ float lora_join(const float* part, int ranks, uint32_
 #pragma unroll
             for (int c = 0; c < 8; ++c) h[i] += v[c];
             h[i] = n < ranks ? h[i] * scaling : 0.f;
-            big = fmaxf(big, fabsf(h[i]));
+            const float size = fabsf(h[i]);
+            big = size < INFINITY ? fmaxf(big, size) : big;  // (an infinity in one section's sums is no reason to leave another's out of range)
         }
     }
-    float up = 1.f, down = 1.f;  // powers of two that bring the row's largest value to [2^13, 2^14) in f16, and back
+    float up = 1.f, down = 1.f;  // powers of two that bring the row's largest finite value to [2^13, 2^14) in f16, and back
     if (std::is_same<T, __half>::value) {
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, off));
-        if (big > 0.f && big < INFINITY) {
+        if (big > 0.f) {
             const int e = min(13 + 127 - static_cast<int>(__float_as_uint(big) >> 23), 120);
             up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
             down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
