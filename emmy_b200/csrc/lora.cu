@@ -1222,6 +1222,13 @@ extern "C" int eq_lora_add(const void* y, const void* x, const void* a, const vo
     const size_t need = eq_lora_workspace_bytes(T, L, S, R);
     EQ_REQUIRE(need == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= need), EQ_ERR_WORKSPACE,
                "eq_lora_add: workspace of %zu bytes (256-byte aligned) needed, %zu given", need, workspace_bytes);
+    // CTAs write rows of out while others read x, A, B and their rows of y
+    const uintptr_t out0 = reinterpret_cast<uintptr_t>(out), out1 = out0 + static_cast<size_t>(T) * N * 2;
+    auto apart = [&](const void* from, size_t bytes) { return reinterpret_cast<uintptr_t>(from) >= out1 || reinterpret_cast<uintptr_t>(from) + bytes <= out0; };
+    EQ_REQUIRE((out == y || apart(y, static_cast<size_t>(T) * N * 2)) && apart(x, static_cast<size_t>(T) * K * 2) && apart(a, static_cast<size_t>(L) * S * R * K * 2) &&
+                   apart(b, static_cast<size_t>(L) * N * R * 2) && apart(scaling, static_cast<size_t>(L) * 4) && apart(adapter_ids, static_cast<size_t>(T) * 4) &&
+                   (need == 0 || apart(workspace, need)),
+               EQ_ERR_BAD_ARG, "eq_lora_add: out may be y and overlaps no other argument");
     p.x = x;
     p.y = y;
     p.a = a;

@@ -26,7 +26,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     """out[t] = y[t] + scaling[l] * b[l] @ (a[l] @ x[t]) with l = adapter_ids[t]; rows whose id lies outside [0, L) keep y[t].
 
     y [T, N] is a linear's output for x [T, K]; a [L, R, K] (or [L, S, R, K] for a projection of S linears side by side whose widths are
-    `sections`), b [L, N, R], scaling f32 [L], adapter_ids int32 [T].  `out` may be y."""
+    `sections`), b [L, N, R], scaling f32 [L], adapter_ids int32 [T].  `out` may be y (and is refused where it overlaps
+    anything else: x, with y = x too)."""
     _need_here(y, x, a, b, scaling, adapter_ids, out, workspace)
     (t, k), n = x.shape, y.shape[1]
     if a.dim() == 4:

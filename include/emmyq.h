@@ -335,9 +335,9 @@ int eq_moe_w8a16(const uint8_t* gate_up, const float* gate_up_scale, const uint8
  *   NULL where S is 1) are their columns: columns of linear s read A_l[s].
  *   Adapters of a smaller rank than R are stored with zeros behind it (zero rows of A, zero columns of B).
  * Products and sums in f32 (A x enters the second product as two 16-bit numbers that hold 16 to 22 bits of it); one rounding, of the
- * result.  out may be y, and overlaps nothing else.  K, N, R and the widths are multiples of 8, S * R <= 1024, S <= 8, L <= 4096;
- * y, x, a, b and out 16-byte aligned.  The workspace is needed above 256 rows only (256-byte aligned, written before it is read); nothing
- * is kept between calls. */
+ * result.  out may be y; one that overlaps anything else is refused (EQ_ERR_BAD_ARG; y may be x where out is neither).  K, N, R and the
+ * widths are multiples of 8, S * R <= 1024, S <= 8, L <= 4096; y, x, a, b and out 16-byte aligned.  The workspace is needed above 256 rows
+ * only (256-byte aligned, written before it is read); nothing is kept between calls. */
 size_t eq_lora_workspace_bytes(int64_t T, int64_t L, int64_t S, int64_t R);
 int eq_lora_add(const void* y, const void* x, const void* a, const void* b, const float* scaling, const int32_t* adapter_ids, int64_t T, int64_t K, int64_t N,
                 int64_t R, int64_t L, int64_t S, const int64_t* section_widths, int act_dtype, void* out, void* workspace, size_t workspace_bytes,

@@ -36,3 +36,27 @@ print("compared")
 def test_shared_memory_around_the_limit_that_every_kernel_has(case, dtype):
     run = subprocess.run([sys.executable, "-c", FIRST_CALL.format(case=case, dtype=dtype)], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and run.stdout.strip() == "compared", run.stderr[-2000:]
+
+
+def test_an_output_beside_what_is_read():
+    """Outputs that touch x or y on either side are other memory; one that is x is refused (y being x or not), one that is y is not."""
+    import torch
+
+    from emmy_b200.lib import EmmyqError
+    from tests import test_gpu_lora as tl
+
+    for t in (5, 300):
+        args = tl.make(t, 64, [64], 8, 3, torch.bfloat16, seed=t)
+        want = tl.call(args, [64])
+        rows = torch.empty(5 * t, 64, dtype=torch.bfloat16, device="cuda")
+        y, x = rows[t : 2 * t], rows[3 * t : 4 * t]
+        for first in (0, 2 * t, 4 * t, t):  # before, between and behind them; y itself
+            y.copy_(args[0]), x.copy_(args[1])
+            out = rows[first : first + t]
+            assert tl.call([y, x, *args[2:]], [64], out=out) is out and torch.equal(out, want)
+            assert torch.equal(x, args[1]) and (first == t or torch.equal(y, args[0]))
+        for args_, out in (((y, x), x), ((x, x), x), ((y, x), rows[2 * t + 1 : 3 * t + 1]), ((y, x), rows[t + 1 : 2 * t + 1])):
+            with pytest.raises(EmmyqError, match="EQ_ERR_BAD_ARG"):
+                tl.call([*args_, *args[2:]], [64], out=out)
+        both = tl.call([x, x, *args[2:]], [64])  # y is x, the result is new
+        tl.close(both, x, x, *args[2:], [64])
