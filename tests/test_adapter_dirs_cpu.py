@@ -28,3 +28,17 @@ def test_adapters_that_changed_their_base_are_refused(tmp_path, how):
 def test_adapters_that_left_their_base_alone_are_read(tmp_path, how):
     write_adapter(tmp_path, tensors(), init_lora_weights=how)
     assert loader.read_adapter(tmp_path)[MODULE][2] == 2.0
+
+
+@pytest.mark.parametrize("config", [dict(alora_invocation_tokens=[5, 7]), dict(use_qalora=True), dict(lora_bias=True)], ids=str)
+def test_adapters_that_are_no_plain_product_are_refused(tmp_path, config):
+    """Active behind certain tokens only; A on group averages of x; a bias beside B."""
+    write_adapter(tmp_path, tensors(), **config)
+    with pytest.raises(ValueError, match=next(iter(config))):
+        loader.read_adapter(tmp_path)
+
+
+def test_the_same_keys_at_rest(tmp_path):
+    write_adapter(tmp_path, tensors(), alora_invocation_tokens=None, use_qalora=False, lora_bias=False)
+    a, b, scaling = loader.read_adapter(tmp_path)[MODULE]
+    assert scaling == 2.0 and torch.equal(a, tensors()[f"base_model.model.{MODULE}.lora_A.weight"])
