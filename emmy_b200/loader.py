@@ -463,7 +463,8 @@ _ADAPTER_RE = re.compile(r"^(?:base_model\.model\.)?(?P<module>.+)\.lora_(?P<ab>
 
 def read_adapter(adapter_dir) -> dict[str, tuple[torch.Tensor, torch.Tensor, float]]:
     """module path -> (A [r, K], B [N, r], scaling) of a low-rank adapter directory, on the host.  scaling = alpha / r, or alpha / sqrt(r)
-    with `use_rslora`, alpha by `alpha_pattern` where an entry names the module (path or dotted suffix).  What is not such a product
+    with `use_rslora`, alpha by `alpha_pattern` where an entry names the module (path or dotted suffix), 8 where the
+    configuration names none.  What is not such a product
     (trained biases, embeddings or saved modules, a magnitude vector, transposed weights, inputs averaged by groups, rows that are adapted
     behind certain tokens only) raises, and so does an adapter whose making
     changed its base (`init_lora_weights` of pissa, olora, corda, loftq and the like): beside the checkpoint's own base it is another one."""
@@ -487,7 +488,7 @@ def read_adapter(adapter_dir) -> dict[str, tuple[torch.Tensor, torch.Tensor, flo
         a, b = ab["A"], ab["B"]
         if a.dim() != 2 or b.dim() != 2 or a.shape[0] != b.shape[1] or a.shape[0] == 0:
             raise ValueError(f"adapter of {module!r}: A {tuple(a.shape)} and B {tuple(b.shape)} do not chain")
-        alpha = cfg.get("lora_alpha", a.shape[0])
+        alpha = cfg.get("lora_alpha", 8)  # the format's own default
         for pattern, value in (cfg.get("alpha_pattern") or {}).items():
             if re.match(rf"(.*\.)?({pattern})$", module):
                 alpha = value

@@ -42,3 +42,11 @@ def test_the_same_keys_at_rest(tmp_path):
     write_adapter(tmp_path, tensors(), alora_invocation_tokens=None, use_qalora=False, lora_bias=False)
     a, b, scaling = loader.read_adapter(tmp_path)[MODULE]
     assert scaling == 2.0 and torch.equal(a, tensors()[f"base_model.model.{MODULE}.lora_A.weight"])
+
+
+@pytest.mark.parametrize("r", [2, 4, 16])
+def test_a_missing_alpha_is_the_formats_default(tmp_path, r):
+    write_adapter(tmp_path, tensors(r))
+    config = tmp_path / "adapter_config.json"
+    config.write_text(config.read_text().replace('"lora_alpha": 8, ', ""))
+    assert "lora_alpha" not in config.read_text() and loader.read_adapter(tmp_path)[MODULE][2] == 8 / r
