@@ -481,6 +481,8 @@ def read_adapter(adapter_dir) -> dict[str, tuple[torch.Tensor, torch.Tensor, flo
         if not m:
             raise ValueError(f"unsupported adapter tensor {key!r}")
         pairs.setdefault(m["module"], {})[m["ab"]] = index.tensor(key)
+    if not pairs:
+        raise ValueError(f"{adapter_dir} holds no adapter tensors in safetensors")
     out = {}
     for module, ab in pairs.items():
         if set(ab) != {"A", "B"}:

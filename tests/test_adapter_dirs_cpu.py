@@ -50,3 +50,15 @@ def test_a_missing_alpha_is_the_formats_default(tmp_path, r):
     config = tmp_path / "adapter_config.json"
     config.write_text(config.read_text().replace('"lora_alpha": 8, ', ""))
     assert "lora_alpha" not in config.read_text() and loader.read_adapter(tmp_path)[MODULE][2] == 8 / r
+
+
+def test_a_directory_without_tensors_is_refused(tmp_path):
+    """As of an adapter that was saved in another format: its slot would be cleared and the base served in its place."""
+    write_adapter(tmp_path, tensors())
+    m = lora()
+    loader.load_adapter(tmp_path, {MODULE: m}, 0)
+    held = m.lora_a.clone()
+    (tmp_path / "adapter_model.safetensors").rename(tmp_path / "adapter_model.bin")
+    with pytest.raises(ValueError, match="no adapter tensors"):
+        loader.load_adapter(tmp_path, {MODULE: m}, 0)
+    assert held.any() and torch.equal(m.lora_a, held)
