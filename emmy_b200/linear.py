@@ -431,6 +431,7 @@ class LoRALinear(nn.Module):
                                    or ai.shape[0] > self.rank):
                 raise ValueError(f"adapter {tuple(ai.shape)} / {tuple(bi.shape)} does not fit {self.in_features} -> {width} at rank {self.rank}")
 
+    @torch.no_grad()
     def load_adapter(self, slot: int, a, b, scaling: float) -> "LoRALinear":
         """a [r, K] and b [N, r], or one of each per section (None for a section that the adapter leaves alone); r <= rank."""
         a, b = (list(t) if isinstance(t, (list, tuple)) else [t] for t in (a, b))
@@ -446,6 +447,7 @@ class LoRALinear(nn.Module):
         self.scaling[slot] = scaling
         return self
 
+    @torch.no_grad()
     def clear_adapter(self, slot: int) -> "LoRALinear":
         if not 0 <= slot < self.slots:
             raise ValueError(f"slot {slot} of {self.slots}")
