@@ -186,6 +186,13 @@ def _flat(x):
     return (x, x.shape[:-1]) if x.dim() == 2 else (x.reshape(-1, x.shape[-1]), x.shape[:-1])
 
 
+def _moved_f32(before, after):
+    """An f32 buffer that moves with its module (`after`: what the module's conversion made of it) and keeps type and values."""
+    if before is None:
+        return None
+    return after.float() if before.is_meta else before.to(after.device)  # (a meta tensor has no values to keep)
+
+
 class W4A16Linear(nn.Module):
     """AWQ (`fmt="awq"`), GPTQ (`fmt="gptq"`, optional act-order `g_idx`) or compressed-tensors (`fmt="ct"`: its three
     tensors already transposed into GPTQ's orientation) int4 linear.
@@ -340,8 +347,7 @@ class QuantMoE(nn.Module):
     def _apply(self, fn, *args, **kwargs):
         scales = self.gate_up_scale, self.down_scale
         super()._apply(fn, *args, **kwargs)
-        if scales[0] is not None:  # they move with the module and stay f32
-            self.gate_up_scale, self.down_scale = (s.to(t.device) for s, t in zip(scales, (self.gate_up_scale, self.down_scale)))
+        self.gate_up_scale, self.down_scale = map(_moved_f32, scales, (self.gate_up_scale, self.down_scale))
         return self
 
     def load_experts(self, w_gate_up, w_down, group_size: int = 128, fmt: str = "awq") -> "QuantMoE":
@@ -415,7 +421,10 @@ class LoRALinear(nn.Module):
     def _apply(self, fn, *args, **kwargs):
         scaling = self.scaling
         super()._apply(fn, *args, **kwargs)
-        self.scaling = scaling.to(self.scaling.device)  # moves with the module and stays f32
+        self.scaling = _moved_f32(scaling, self.scaling)
+        if scaling.is_meta and not self.scaling.is_meta:  # built without storage: the slots are empty, as they are from the start
+            for t in (self.lora_a, self.lora_b, self.scaling):
+                t.zero_()
         return self
 
     def check_adapter(self, slot: int, a, b) -> None:
