@@ -142,6 +142,17 @@ def _(y, x, a, b, scaling, adapter_ids, sections):
     return torch.empty_like(y, memory_format=torch.contiguous_format)
 
 
+@torch.library.custom_op("emmyq::lora_add_in", mutates_args=("workspace",), device_types="cuda")
+def _lora_add_in_op(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor, adapter_ids: torch.Tensor,
+                    sections: list[int], workspace: torch.Tensor) -> torch.Tensor:
+    return ops_lora.lora_add(y.contiguous(), x.contiguous(), a, b, scaling, adapter_ids.contiguous(), sections=sections, workspace=workspace)
+
+
+@_lora_add_in_op.register_fake
+def _(y, x, a, b, scaling, adapter_ids, sections, workspace):
+    return torch.empty_like(y, memory_format=torch.contiguous_format)
+
+
 # An eager call on plain CUDA tensors needs nothing of the dispatcher: going through the custom op's Python layers costs about 20 us,
 # four times the kernel at one token (with the lighter calls of ops.py a 4096 x 4096 W4A16Linear of one row 49 -> 19 us a call,
 # FP8Linear of 32 rows 43 -> 27, NVFP4Linear of 40 rows 47 -> 28, QuantMoE of one token 56 -> 35).  "Plain" is decided on each call,
@@ -464,15 +475,22 @@ class LoRALinear(nn.Module):
             t[slot].zero_()
         return self
 
-    def forward(self, x: torch.Tensor, adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
-        """adapter_ids: int32, one per row of x (x.shape[:-1]); None: the base alone."""
+    def workspace(self, rows: int) -> torch.Tensor:
+        """Scratch of the caller's own for calls of up to `rows` rows, which ops_lora.lora_status asks about."""
+        return ops_lora.lora_workspace(rows, self.slots, len(self.sections), self.rank, self.lora_a.device)
+
+    def forward(self, x: torch.Tensor, adapter_ids: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+        """adapter_ids: int32, one per row of x (x.shape[:-1]); None: the base alone.  workspace: of `workspace()`, for a caller that will ask
+        ops_lora.lora_status whether the waits of a call of more than 256 rows ended in time; without one the call takes scratch that nobody can ask."""
         y = self.base(x)
         if adapter_ids is None:
             return y
         x2, lead = _flat(x)
         y2, ids = y.reshape(-1, self.out_features), adapter_ids.reshape(-1)
         if _direct(x2, y2, ids, self.lora_a, self.lora_b):
-            out = ops_lora.lora_add(y2.contiguous(), x2.contiguous(), self.lora_a, self.lora_b, self.scaling, ids.contiguous(), sections=self.sections)
-        else:
+            out = ops_lora.lora_add(y2.contiguous(), x2.contiguous(), self.lora_a, self.lora_b, self.scaling, ids.contiguous(), sections=self.sections, workspace=workspace)
+        elif workspace is None:
             out = _lora_add_op(y2, x2, self.lora_a, self.lora_b, self.scaling, ids, list(self.sections))
+        else:
+            out = _lora_add_in_op(y2, x2, self.lora_a, self.lora_b, self.scaling, ids, list(self.sections), workspace)
         return out.reshape(*lead, self.out_features)

@@ -21,13 +21,25 @@ def _section_array(sections, n):
     return array
 
 
+def lora_workspace(t: int, adapters: int, sections: int, rank: int, device) -> torch.Tensor:
+    """Zeroed scratch for calls of up to t rows over `adapters` slots of `sections` x `rank`."""
+    return torch.zeros(max(L.load().eq_lora_workspace_bytes(t, adapters, sections, rank), 256), dtype=torch.uint8, device=device)
+
+
+def lora_status(workspace: torch.Tensor) -> None:
+    """Synchronizes the stream; raises EmmyqError(EQ_ERR_TIMEOUT) if a bounded wait of the last call of more than 256 rows on this workspace ran out."""
+    _need_here(workspace)
+    L.check(L.load().eq_lora_status(workspace.data_ptr(), _stream()))
+
+
 def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor, adapter_ids: torch.Tensor, sections=None,
              workspace: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """out[t] = y[t] + scaling[l] * b[l] @ (a[l] @ x[t]) with l = adapter_ids[t]; rows whose id lies outside [0, L) keep y[t].
 
     y [T, N] is a linear's output for x [T, K]; a [L, R, K] (or [L, S, R, K] for a projection of S linears side by side whose widths are
     `sections`), b [L, N, R], scaling f32 [L], adapter_ids int32 [T].  `out` may be y (and is refused where it overlaps
-    anything else: x, with y = x too)."""
+    anything else: x, with y = x too).  Above 256 rows the kernels wait for one another, with a limit: `out` holds the result only if
+    lora_status(workspace) raises nothing (a loop asks once for many calls, with a workspace of its own for each that it asks about)."""
     _need_here(y, x, a, b, scaling, adapter_ids, out, workspace)
     (t, k), n = x.shape, y.shape[1]
     if a.dim() == 4:
