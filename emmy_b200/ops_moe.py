@@ -112,11 +112,19 @@ def moe_status(workspace, t: int, w: MoEWeights, topk: int) -> None:
     L.check(L.load().eq_moe_status(_ptr(workspace), t, w.experts, topk, w.hidden, w.inter, _stream()))
 
 
+# Tokens of a call of the kernels where the scratch is this module's: above 32 tokens it takes topk (8 I + 4 H) bytes for each, and more tokens at once
+# are no faster.  Whole and in pieces of 1024, 2048, 4096, us: 8192 tokens of 128 experts of 2048 x 768, top 8, 6651 and 5759, 5693, 6137 (975 MB and 244 with
+# 2048), of 8 experts of 4096 x 14336, top 2, 49324 and 46155, 43931, 47010 (2215 MB and 554); 4096 of the former 3110 and 2863, 2707.  (2048 in pieces of
+# 1024 1458 and 1445, 8590 and 11000.)
+_W8_PIECE = 2048
+
+
 def moe_w8a16(x, router_logits, gate_up, gate_up_scale, down, down_scale, topk: int, workspace=None, out=None):
     """One routed MoE layer of a few tokens on FP8 experts: y[T, H] from x[T, H] and f32 router logits [T, E].
 
     gate_up e4m3 bits [E, 2I, H] (uint8; gate rows, then up rows), down [E, H, I]; scales f32, per output channel ([E, 2I] and [E, H]) or
-    per 128 x 128 block ([E, 2I / 128, H / 128] and [E, H / 128, I / 128])."""
+    per 128 x 128 block ([E, 2I / 128, H / 128] and [E, H / 128, I / 128]).  `out` may be x.  It takes any T, in pieces of 2048 tokens with scratch for
+    one of them; with a workspace of the caller's (eq_moe_w8a16_workspace_bytes of all T) in one call."""
     _need_here(x, router_logits, gate_up, gate_up_scale, down, down_scale, workspace, out)
     (t, h), (e, n2, k), i = x.shape, gate_up.shape, down.shape[2]
     if k != h or n2 != 2 * i or down.shape != (e, h, i) or router_logits.shape != (t, e):
@@ -138,12 +146,15 @@ def moe_w8a16(x, router_logits, gate_up, gate_up_scale, down, down_scale, topk: 
     elif out.shape != x.shape or out.dtype is not dtype:
         raise ValueError(f"moe_w8a16: out {tuple(out.shape)} {out.dtype} does not fit x {tuple(x.shape)} {dtype}")
     lib = L.load()
+    piece = t
     if workspace is None:
-        workspace = _scratch(lib.eq_moe_w8a16_workspace_bytes(t, e, topk, h, i), x.device)
-    status = lib.eq_moe_w8a16(
-        gate_up.data_ptr(), gate_up_scale.data_ptr(), down.data_ptr(), down_scale.data_ptr(), block, e, topk, h, i, x.data_ptr(),
-        router_logits.data_ptr(), t, _DTYPE[dtype], out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream(),
-    )
-    if status:
-        L.check(status)
+        piece = min(t, _W8_PIECE)
+        workspace = _scratch(lib.eq_moe_w8a16_workspace_bytes(piece, e, topk, h, i), x.device)
+    for t0 in range(0, t, piece) if t else (0,):
+        status = lib.eq_moe_w8a16(
+            gate_up.data_ptr(), gate_up_scale.data_ptr(), down.data_ptr(), down_scale.data_ptr(), block, e, topk, h, i, x.data_ptr() + 2 * t0 * h,
+            router_logits.data_ptr() + 4 * t0 * e, min(piece, t - t0), _DTYPE[dtype], out.data_ptr() + 2 * t0 * h, workspace.data_ptr(), workspace.numel(), _stream(),
+        )
+        if status:
+            L.check(status)
     return out

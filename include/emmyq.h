@@ -318,7 +318,8 @@ int eq_moe_status(const void* workspace, int64_t T, int64_t E, int64_t topk, int
  * A picked expert is read once for every eight rows (sixteen where experts have more than nine on average).  It takes any T, but is built for
  * decode batches: from about eight rows an expert on it is bound by its warp-level MMAs and what feeds them.
  * E <= 1024, topk <= 16, H and I multiples of 128; gate_up, down, x and y 16-byte aligned; y may be x.  The workspace is 256-byte aligned
- * and written before it is read. */
+ * and written before it is read; above 32 tokens it is about topk (8 I + 4 H) bytes a token, so that a prompt is better given in pieces of
+ * some thousand tokens (they do not depend on one another). */
 size_t eq_moe_w8a16_workspace_bytes(int64_t T, int64_t E, int64_t topk, int64_t H, int64_t I);
 int eq_moe_w8a16(const uint8_t* gate_up, const float* gate_up_scale, const uint8_t* down, const float* down_scale, int block_scales, int64_t E, int64_t topk,
                  int64_t H, int64_t I, const void* x, const float* router_logits, int64_t T, int act_dtype, void* y, void* workspace,
