@@ -1072,6 +1072,7 @@ static int lora_block_rows(int64_t T, int64_t K, int64_t N, int64_t S, int64_t R
     if (T <= kLoraSelfPlan || !lora_wide(S, R)) return 16;
     return static_cast<double>(T) * (K + 2 * N) * (R < 32 ? 32 : R) < (S * R <= 16 ? 2e9 : 7e8) ? 16 : kLoraRows;
 }
+static bool lora_self(int64_t T, int block_rows) { return block_rows == 16 && T <= kLoraSelfRows; }
 static int64_t lora_units(int64_t T, int64_t L, int block_rows) { return group_max_blocks(T, L, block_rows, block_rows == kLoraRows); }
 
 // CTAs of a cluster: the largest of 8, 4, 2, 1 whose grid stays within `most` CTAs an SM.  (The grid is sized for the most blocks that the rows can
@@ -1109,7 +1110,7 @@ static int lora_forward(LoraParams p, int64_t T_, int64_t L, unsigned char* base
     const int ranks = p.S * p.R, section_ranks = (p.R + 15) & ~15;
     const int block_rows = lora_block_rows(p.T, p.K, p.N, p.S, p.R);
     const int64_t units = lora_units(T_, L, block_rows);
-    const bool self = block_rows == 16 && p.T <= kLoraSelfRows;
+    const bool self = lora_self(p.T, block_rows);
     p.status = p.T > kLoraSelfPlan ? reinterpret_cast<int*>(base) : nullptr;
     if (!self) {
         size_t o = 256;
@@ -1185,6 +1186,11 @@ extern "C" size_t eq_lora_workspace_bytes(int64_t T, int64_t L, int64_t S, int64
     const int64_t few = lora_units(T, L, 16), many = lora_units(T, L, kLoraRows);
     const size_t lists = 256 + lora_align(static_cast<size_t>(few > many ? few : many) * sizeof(GroupBlock)) + lora_align(static_cast<size_t>(T) * 4);
     return !lora_wide(S, R) ? lists : lists + lora_align(static_cast<size_t>(T) * 4) + 2 * lora_align(static_cast<size_t>(T) * S * ((R + 15) / 16 * 16) * 2);
+}
+
+extern "C" const char* eq_lora_kernel(int64_t T, int64_t K, int64_t N, int64_t R, int64_t S) {
+    const int block_rows = lora_block_rows(T, K, N, S, R);
+    return block_rows == kLoraRows ? "lora_expand_kernel" : lora_self(T, block_rows) ? "lora_rows_kernel" : "group_rows_kernel + lora_rows_kernel";
 }
 
 extern "C" int eq_lora_add(const void* y, const void* x, const void* a, const void* b, const float* scaling, const int32_t* adapter_ids, int64_t T, int64_t K,

@@ -340,6 +340,9 @@ int eq_moe_w8a16(const uint8_t* gate_up, const float* gate_up_scale, const uint8
  * widths are multiples of 8, S * R <= 1024, S <= 8, L <= 4096; y, x, a, b and out 16-byte aligned.  The workspace is needed above 256 rows
  * only (256-byte aligned, written before it is read); nothing is kept between calls. */
 size_t eq_lora_workspace_bytes(int64_t T, int64_t L, int64_t S, int64_t R);
+/* The kernels that a call of this extent takes, for tests and profiles: "lora_rows_kernel", "group_rows_kernel + lora_rows_kernel" (blocks
+ * of 16 rows) or "lora_expand_kernel" (blocks of 128 rows: group_rows_kernel, lora_shrink_kernel and it). */
+const char* eq_lora_kernel(int64_t T, int64_t K, int64_t N, int64_t R, int64_t S);
 int eq_lora_add(const void* y, const void* x, const void* a, const void* b, const float* scaling, const int32_t* adapter_ids, int64_t T, int64_t K, int64_t N,
                 int64_t R, int64_t L, int64_t S, const int64_t* section_widths, int act_dtype, void* out, void* workspace, size_t workspace_bytes,
                 void* stream);
