@@ -1004,21 +1004,39 @@ static int w8_launch(void (*kernel)(P...), int64_t grid, int cluster, size_t sme
     return EQ_OK;
 }
 
+// Which kernels a call takes.
+struct W8Form {
+    bool self;  // the CTAs group the picks, two products and nothing else
+    bool own;   // and route and bring x and silu * up to f16 as well
+    bool wide;  // thirty-two rows a warp
+    int rb;     // groups of eight rows of a block, general form
+};
+static int64_t w8_own_x(int64_t T, int64_t H, bool f16) { return f16 ? 0 : T * (H + 8) * 2; }
+static int64_t w8_own_h(int64_t R, int64_t I) { return R * kW8PartsH * (I + 8) * 2; }
+static W8Form w8_form(int64_t T, int64_t E, int64_t topk, int64_t H, int64_t I, bool f16) {
+    W8Form f;
+    const int64_t R = T * topk;
+    f.self = w8_self(T, E, H, I);
+    // Thirty-two rows a warp where there are enough of them: half as many reads of the activations, which lie in L1 and L2, for the same weights.
+    f.wide = R * (I / 16) >= 16 * static_cast<int64_t>(sm_count());
+    f.own = f.self && !f.wide && w8_own_x(T, H, f16) + w8_own_h(R, I) <= kW8Own;
+    // Sixteen rows a block where experts have that many: the weights of an expert with nine to sixteen rows are read and expanded once and not twice, but half as
+    // far ahead.  128 experts of 2048 x 768, top 8, us a layer with 8 and 16: 96 tokens 149 and 171, 128 174 and 176, 144 180 and 180, 160 193 and 180, 200 236 and
+    // 189, 256 298 and 230; 64 experts, top 6: 96 tokens 161 and 165, 128 193 and 182.
+    f.rb = R > 9 * E ? 2 : 1;
+    return f;
+}
+
 template <typename T, bool BLOCK>
 static int w8_forward(W8Params p, const uint8_t* gate_up, const float* gate_up_scale, const uint8_t* down, const float* down_scale, const W8Workspace& w,
                       cudaStream_t stream) {
     const size_t plan = (sizeof(W8Plan) + 15) / 16 * 16;
     const int64_t R = static_cast<int64_t>(p.T) * p.topk;
-    const bool self = w8_self(p.T, p.E, p.H, p.I);
     constexpr bool f16 = std::is_same<T, __half>::value;  // x is read as it is
-    const int64_t own_x = f16 ? 0 : static_cast<int64_t>(p.T) * (p.H + 8) * 2, own_h = R * kW8PartsH * (p.I + 8) * 2;
-    const int64_t sms = sm_count(), most = 2 * sms;
-    // Thirty-two rows a warp where there are enough of them: half as many reads of the activations, which lie in L1 and L2, for the same weights.
-    const bool wide = R * (p.I / 16) >= 8 * most, own = self && !wide && own_x + own_h <= kW8Own;
-    // Sixteen rows a block where experts have that many: the weights of an expert with nine to sixteen rows are read and expanded once and not twice, but half as
-    // far ahead.  128 experts of 2048 x 768, top 8, us a layer with 8 and 16: 96 tokens 149 and 171, 128 174 and 176, 144 180 and 180, 160 193 and 180, 200 236 and
-    // 189, 256 298 and 230; 64 experts, top 6: 96 tokens 161 and 165, 128 193 and 182.
-    const int rb = R > 9 * static_cast<int64_t>(p.E) ? 2 : 1;
+    const W8Form form = w8_form(p.T, p.E, p.topk, p.H, p.I, f16);
+    const bool self = form.self, wide = form.wide, own = form.own;
+    const int rb = form.rb;
+    const int64_t own_x = w8_own_x(p.T, p.H, f16), own_h = w8_own_h(R, p.I), sms = sm_count(), most = 2 * sms;
     int st = EQ_OK;
     p.h_max = self && !own ? w.h_max : nullptr;
     p.h16 = w.h16;
@@ -1077,6 +1095,12 @@ using namespace eq;
 extern "C" size_t eq_moe_w8a16_workspace_bytes(int64_t T, int64_t E, int64_t topk, int64_t H, int64_t I) {
     if (T <= 0 || E <= 0 || topk <= 0 || H <= 0 || I <= 0) return 0;
     return w8_carve(nullptr, T, E, topk, H, I).bytes;
+}
+
+extern "C" const char* eq_moe_w8a16_kernel(int64_t T, int64_t E, int64_t topk, int64_t H, int64_t I, int act_dtype) {
+    const W8Form f = w8_form(T, E, topk, H, I, act_dtype == EQ_F16);
+    if (f.self) return f.own ? "moe_w8_down_kernel, own" : f.wide ? "moe_w8_down_kernel, wide" : "moe_w8_down_kernel";
+    return f.rb == 2 ? "moe_w8_tiles_kernel, sixteen rows" : "moe_w8_tiles_kernel, eight rows";
 }
 
 extern "C" int eq_moe_w8a16(const uint8_t* gate_up, const float* gate_up_scale, const uint8_t* down, const float* down_scale, int block_scales, int64_t E,

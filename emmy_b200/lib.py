@@ -130,6 +130,7 @@ def load() -> C.CDLL:
         "eq_moe_w4a16": (i, [p, p, i, i64, i64, i64, i64, i64, p, p, i64, i, p, p, sz, p]),
         "eq_moe_status": (i, [p, i64, i64, i64, i64, i64, p]),
         "eq_moe_w8a16_workspace_bytes": (sz, [i64, i64, i64, i64, i64]),
+        "eq_moe_w8a16_kernel": (C.c_char_p, [i64, i64, i64, i64, i64, i]),
         "eq_moe_w8a16": (i, [p, p, p, p, i, i64, i64, i64, i64, p, p, i64, i, p, p, sz, p]),
         "eq_lora_workspace_bytes": (sz, [i64, i64, i64, i64]),
         "eq_lora_kernel": (C.c_char_p, [i64, i64, i64, i64, i64]),

@@ -321,6 +321,10 @@ int eq_moe_status(const void* workspace, int64_t T, int64_t E, int64_t topk, int
  * and written before it is read; above 32 tokens it is about topk (8 I + 4 H) bytes a token, so that a prompt is better given in pieces of
  * some thousand tokens (they do not depend on one another). */
 size_t eq_moe_w8a16_workspace_bytes(int64_t T, int64_t E, int64_t topk, int64_t H, int64_t I);
+/* The form that a call of this extent takes, for tests and profiles, by the kernel of its down product: "moe_w8_down_kernel" (up to 32
+ * tokens; with ", own" two launches in all, with ", wide" thirty-two weight rows a warp) or "moe_w8_tiles_kernel" with ", eight rows" or
+ * ", sixteen rows" of an expert in a block. */
+const char* eq_moe_w8a16_kernel(int64_t T, int64_t E, int64_t topk, int64_t H, int64_t I, int act_dtype);
 int eq_moe_w8a16(const uint8_t* gate_up, const float* gate_up_scale, const uint8_t* down, const float* down_scale, int block_scales, int64_t E, int64_t topk,
                  int64_t H, int64_t I, const void* x, const float* router_logits, int64_t T, int act_dtype, void* y, void* workspace,
                  size_t workspace_bytes, void* stream);

@@ -1,0 +1,30 @@
+"""Which kernels a call of the FP8 expert layer takes (on 148 SMs, what a machine without a GPU assumes), and that the GPU tests of each form take it."""
+
+import pytest
+
+from emmy_b200 import lib as L
+from tests import test_gpu_moe_w8_forms as forms
+
+
+@pytest.fixture(scope="module")
+def kernel():
+    from emmy_b200.build import build
+
+    build()
+    return lambda t, e, topk, h, i, f16=False: L.load().eq_moe_w8a16_kernel(t, e, topk, h, i, L.EQ_F16 if f16 else L.EQ_BF16).decode()
+
+
+def test_the_lines_between_the_forms(kernel):
+    assert kernel(1, 128, 8, 2048, 768) == forms.OWN and kernel(2, 128, 8, 2048, 768) == kernel(2, 128, 8, 2048, 768, True) == forms.DOWN
+    # 36 KB of f16 activations: 4112 of x and 32128 or 33152 of silu * up
+    assert kernel(1, 64, 8, 2048, 996) == forms.OWN and kernel(1, 64, 8, 2048, 1028) == forms.DOWN and kernel(1, 64, 8, 2048, 1028, True) == forms.OWN
+    # picks x I / 16 from sixteen rows an SM on
+    assert kernel(16, 128, 4, 512, 576) == forms.DOWN and kernel(16, 128, 4, 512, 592) == forms.WIDE
+    assert kernel(32, 256, 1, 512, 256) == forms.DOWN and kernel(33, 256, 1, 512, 256) == kernel(1, 257, 1, 512, 256) == kernel(1, 8, 1, 512, 65664) == forms.EIGHT
+    assert kernel(144, 128, 8, 2048, 768) == forms.EIGHT and kernel(145, 128, 8, 2048, 768) == forms.SIXTEEN
+
+
+@pytest.mark.parametrize("form", list(forms.CASES))
+def test_every_case_takes_its_form(kernel, form):
+    t, e, topk, h, i = forms.CASES[form]
+    assert {kernel(t, e, topk, h, i, f16) for f16 in (False, True)} == {forms.FORM_OF[form]}
