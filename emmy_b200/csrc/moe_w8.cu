@@ -22,7 +22,7 @@
 //            memory in warp order.
 //   down     A cluster of CTAs has sixteen output channels of ALL the blocks: the picks of a token meet inside it (f32, a fixed order), y is written
 //            once, and nothing is combined in memory.  It has grouped the picks and asked for its first weights before the launch ahead of it ends.
-// Where the activations are small (kW8Own: a token or two) these two launches are the layer, one CTA an SM each, so that the second one is resident, has routed
+// Where a CTA of either launch fits an SM with f16 activations of its own (w8_form) these two launches are the layer, one CTA an SM each, so that the second one is resident, has routed
 // too and asked for its first weights while the first one runs.  Else w8_prep_kernel routes the tokens and brings x (of bf16) to f16 ahead of them.
 // Then no launch has to come between the two: the rows' largest values are found as they are written, and the second one splits what it reads of them.
 // Above, w8_prep_kernel and group.cu list the blocks, w8_parts_kernel splits the rows of silu * up (there are so many CTAs for each row that they would do it
@@ -55,7 +55,6 @@ constexpr int kW8MaxTopK = 16;
 constexpr int kW8SelfPicks = kW8SelfTokens * kW8MaxTopK;
 constexpr int kW8BlockRows = 8;
 constexpr int kW8PartsH = 2;            // value and remainder of silu(gate) * up
-constexpr int kW8Own = 36 * 1024;       // bytes of f16 activations that the two launches of a few tokens make for themselves, a CTA of either on an SM
 
 struct W8Params {
     const uint8_t* w;         // this phase's weights: gate_up [E][2I][H] or down [E][H][I]
@@ -1011,15 +1010,29 @@ struct W8Form {
     bool wide;  // thirty-two rows a warp
     int rb;     // groups of eight rows of a block, general form
 };
-static int64_t w8_own_x(int64_t T, int64_t H, bool f16) { return f16 ? 0 : T * (H + 8) * 2; }
-static int64_t w8_own_h(int64_t R, int64_t I) { return R * kW8PartsH * (I + 8) * 2; }
+constexpr size_t kW8Plan = (sizeof(W8Plan) + 15) / 16 * 16;
+// Dynamic shared memory of a CTA; with few the activations come on top.
+static size_t w8_tiles_smem(int mw, int rb, bool few, bool block) { return static_cast<size_t>(kW8Warps) * (w8_ring(mw, few) + w8_stage(mw, few, block) + 2 * mw * rb * 32 * sizeof(float4)); }
+static size_t w8_down_smem(int64_t T, int mw, bool few, bool block) {
+    return static_cast<size_t>(kW8Warps) * (w8_ring(mw, few) + w8_stage(mw, few, block) + static_cast<size_t>(T) * 16 * mw * sizeof(float)) + kW8Plan;
+}
+static size_t w8_own_x(int64_t T, int64_t H, bool f16) { return f16 ? 0 : static_cast<size_t>(T) * (H + 8) * 2; }
+static size_t w8_own_h(int64_t R, int64_t I) { return static_cast<size_t>(R) * kW8PartsH * (I + 8) * 2; }
+
 static W8Form w8_form(int64_t T, int64_t E, int64_t topk, int64_t H, int64_t I, bool f16) {
     W8Form f;
-    const int64_t R = T * topk;
+    const int64_t R = T * topk, sms = sm_count();
     f.self = w8_self(T, E, H, I);
     // Thirty-two rows a warp where there are enough of them: half as many reads of the activations, which lie in L1 and L2, for the same weights.
-    f.wide = R * (I / 16) >= 16 * static_cast<int64_t>(sm_count());
-    f.own = f.self && !f.wide && w8_own_x(T, H, f16) + w8_own_h(R, I) <= kW8Own;
+    f.wide = R * (I / 16) >= 16 * sms;
+    // CTAs that route and convert for themselves, no launch ahead of them: where one of either product, with its activations, fits an SM beside the other
+    // (228 KB; 1 KB of each is the system's, up to 256 bytes are static), and the down product's slabs of sixteen channels are no more than SMs.  Without
+    // and with, us: 128 experts of 2048 x 768, a token, top 8 18.7 : 17.7, two, top 4 20.7 : 18.9; 64 of 2048 x 1024, three of f16, top 2 19.4 : 16.4, four (too large
+    // by 1 KB) 22.3 : 23.4; 8 of 2048 x 2048, two of f16 19.8 : 17.3; 32 of 1024 x 512, top 4, three 15.9 : 15.7, four (too large) 16.4 : 18.4; more slabs than
+    // SMs: 8 of 4096 x 4096, one, top 1 20.9 : 22.8, 32 of 5120 x 768, one of f16, top 8 32.3 : 45.3.
+    constexpr size_t kSm = 228 * 1024, kBeside = 1024 + 256;
+    f.own = f.self && !f.wide && H / 16 <= sms &&
+            w8_tiles_smem(1, 1, true, true) + kW8Plan + w8_own_x(T, H, f16) + w8_down_smem(T, 1, true, true) + w8_own_h(R, I) + 2 * kBeside <= kSm;
     // Sixteen rows a block where experts have that many: the weights of an expert with nine to sixteen rows are read and expanded once and not twice, but half as
     // far ahead.  128 experts of 2048 x 768, top 8, us a layer with 8 and 16: 96 tokens 149 and 171, 128 174 and 176, 144 180 and 180, 160 193 and 180, 200 236 and
     // 189, 256 298 and 230; 64 experts, top 6: 96 tokens 161 and 165, 128 193 and 182.
@@ -1030,13 +1043,14 @@ static W8Form w8_form(int64_t T, int64_t E, int64_t topk, int64_t H, int64_t I, 
 template <typename T, bool BLOCK>
 static int w8_forward(W8Params p, const uint8_t* gate_up, const float* gate_up_scale, const uint8_t* down, const float* down_scale, const W8Workspace& w,
                       cudaStream_t stream) {
-    const size_t plan = (sizeof(W8Plan) + 15) / 16 * 16;
+    const size_t plan = kW8Plan;
     const int64_t R = static_cast<int64_t>(p.T) * p.topk;
     constexpr bool f16 = std::is_same<T, __half>::value;  // x is read as it is
     const W8Form form = w8_form(p.T, p.E, p.topk, p.H, p.I, f16);
     const bool self = form.self, wide = form.wide, own = form.own;
     const int rb = form.rb;
-    const int64_t own_x = w8_own_x(p.T, p.H, f16), own_h = w8_own_h(R, p.I), sms = sm_count(), most = 2 * sms;
+    const size_t own_x = w8_own_x(p.T, p.H, f16), own_h = w8_own_h(R, p.I);
+    const int64_t sms = sm_count(), most = 2 * sms;
     int st = EQ_OK;
     p.h_max = self && !own ? w.h_max : nullptr;
     p.h16 = w.h16;
@@ -1055,7 +1069,7 @@ static int w8_forward(W8Params p, const uint8_t* gate_up, const float* gate_up_s
     if (st != EQ_OK) return st;
     p.w = gate_up;
     p.scale = gate_up_scale;
-    auto smem = [&](int mw, int rb = 1, bool few = false) { return static_cast<size_t>(kW8Warps) * (w8_ring(mw, few) + w8_stage(mw, few, BLOCK) + 2 * mw * rb * 32 * sizeof(float4)); };
+    auto smem = [](int mw, int rb = 1, bool few = false) { return w8_tiles_smem(mw, rb, few, BLOCK); };
     if (self) {
         const int64_t tiles = R * (p.I / (wide ? 16 : 8)), at_once = own ? sms : most, grid = tiles < at_once ? tiles : at_once;
         if (own) st = w8_launch(moe_w8_tiles_kernel<T, BLOCK, true, false, true, 1, 1>, grid, 1, smem(1, 1, true) + plan + own_x, stream, p);
@@ -1073,7 +1087,7 @@ static int w8_forward(W8Params p, const uint8_t* gate_up, const float* gate_up_s
         const int64_t slabs = p.H / (16 * mw);
         int cluster = 8;  // two CTAs an SM at most, one beside the launch ahead
         while (cluster > 1 && slabs * cluster > (own ? sms : most)) cluster /= 2;
-        const size_t bytes = static_cast<size_t>(kW8Warps) * (w8_ring(mw, own) + w8_stage(mw, own, BLOCK) + static_cast<size_t>(p.T) * 16 * mw * sizeof(float)) + plan;
+        const size_t bytes = w8_down_smem(p.T, mw, own, BLOCK);
         if (wide) return w8_launch(moe_w8_down_kernel<T, BLOCK, false, 2>, slabs * cluster, cluster, bytes, stream, p);
         return own ? w8_launch(moe_w8_down_kernel<T, BLOCK, true, 1>, slabs * cluster, cluster, bytes + own_h, stream, p)
                      : w8_launch(moe_w8_down_kernel<T, BLOCK, false, 1>, slabs * cluster, cluster, bytes, stream, p);
