@@ -1023,8 +1023,12 @@ static W8Form w8_form(int64_t T, int64_t E, int64_t topk, int64_t H, int64_t I, 
     W8Form f;
     const int64_t R = T * topk, sms = sm_count();
     f.self = w8_self(T, E, H, I);
-    // Thirty-two rows a warp where there are enough of them: half as many reads of the activations, which lie in L1 and L2, for the same weights.
-    f.wide = R * (I / 16) >= 16 * sms;
+    // Thirty-two rows a warp where there are enough of them: half as many reads of the activations, which lie in L1 and L2, for the same weights.  us a layer with
+    // sixteen and thirty-two, by R I / 16.  H from 1280 on: 16 experts of 2048 x 2816, top 4, 1408 40.1 : 36.6, 5632 67 : 62, 22528 110 : 93; 128 of 2048 x 768,
+    // top 8, 768 28.4 : 27.5, 2304 55 : 50, 12288 135 : 119; 128 of 1280 x 768, 768 24.6 : 23.2, 2304 47 : 41; below, nothing in it (32 of 2048 x 512, top 4, 384
+    // 18.9 : 18.9; 8 of 2048 x 256, top 2, 256 14.6 : 15.7).  Narrower layers have few slabs of thirty-two channels, in clusters of eight: 32 of 1024 x 512, 384
+    // 16.0 : 20.7, 768 18.6 : 24.1, 1536 23.2 : 23.4; 128 of 1024 x 768, 2304 35.5 : 32.9, 7680 68 : 59, 12288 (32 tokens) 80 : 90; of 640 x 768, 3072 35 : 31.
+    f.wide = R * (I / 16) >= (H >= 1280 ? 4 : 16) * sms;
     // CTAs that route and convert for themselves, no launch ahead of them: where one of either product, with its activations, fits an SM beside the other
     // (228 KB; 1 KB of each is the system's, up to 256 bytes are static), and the down product's slabs of sixteen channels are no more than SMs.  Without
     // and with, us: 128 experts of 2048 x 768, a token, top 8 18.7 : 17.7, two, top 4 20.7 : 18.9; 64 of 2048 x 1024, three of f16, top 2 19.4 : 16.4, four (too large
