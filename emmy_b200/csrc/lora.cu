@@ -1075,12 +1075,22 @@ static int lora_block_rows(int64_t T, int64_t K, int64_t N, int64_t S, int64_t R
 static bool lora_self(int64_t T, int block_rows) { return block_rows == 16 && T <= kLoraSelfRows; }
 static int64_t lora_units(int64_t T, int64_t L, int block_rows) { return group_max_blocks(T, L, block_rows, block_rows == kLoraRows); }
 
-// CTAs of a cluster: the largest of 8, 4, 2, 1 whose grid stays within `most` CTAs an SM.  (The grid is sized for the most blocks that the rows can
-// make: usually there are fewer.)
-static int lora_cluster(int64_t units, int most) {
+// CTAs of a cluster: the largest of 8, 4, 2, 1 with which so many blocks stay within `most` CTAs an SM, and two within `pairs`.
+static int lora_cluster(int64_t blocks, int64_t most, int64_t pairs) {
     int ctas = 8;
-    while (ctas > 1 && units * ctas > most * sm_count()) ctas /= 2;
+    while (ctas > 1 && blocks * ctas > (ctas > 2 ? most : pairs) * sm_count()) ctas /= 2;
     return ctas;
+}
+// Blocks of 16 rows that a call is likely to have.  (The most that it can have are T / 16 and one for each kind of rows, but not every adapter is met.)  Within two
+// CTAs an SM, which run at once; two a block within four an SM, as wide projections gain more from them than narrow ones lose.  us with clusters of 1, 2, 4, 8,
+// the one that is taken in brackets:
+//   K=N=4096, rank 16             64 rows of 64 adapters 15.7 11.3 [8.5] 12.3, 256 of 8 16.7 11.3 8.5 [7.9], 256 of 64 18.4 12.3 [9.9] 15.7, 256 of 400 23.6 [26.3] 26.6 41.3
+//     prompts of three            500 rows 17.1 12.6 9.9 [10.2], 700 19.5 13.7 [10.9] 16.0, 1200 23.9 [17.7] 20.5 25.3, 2000 26.3 [19.8] 24.9 39.9, 3200 33.1 [37.9] 37.5 56.0
+//   K=14336 N=4096, rank 16       64 of 64 31.1 19.1 [13.0] 16.7, 200 of 200 37.9 [24.2] 27.6 37.9, 256 of 400 39.9 [43.0] 40.3 54.3
+//   K=4096 N=28672, rank 64       64 of 64 163 103 [64] 68, 128 of 128 196 [116] 112 100, 256 of 64 178 108 [71] 78, 256 of 400 225 [209] 179 193
+static int64_t lora_likely_blocks(int64_t T, int64_t L) {
+    const int64_t kinds = L + 1 < T ? L + 1 : T;
+    return T / 16 + kinds * 3 / 4;
 }
 
 static int lora_launch(void (*kernel)(const LoraParams), const LoraParams& p, int64_t grid, int cluster, size_t smem, cudaStream_t stream) {
@@ -1136,7 +1146,7 @@ static int lora_forward(LoraParams p, int64_t T_, int64_t L, unsigned char* base
     if (block_rows == 16) {
         p.h_stride = (ranks + 63) / 64 * 64 + 32;  // rows 64 bytes apart modulo 128: the 16-byte reads of two rows meet every bank once
         const size_t red = static_cast<size_t>(kLoraWarps) * 16 * (kLoraPass + 8) * sizeof(float), split = 2 * static_cast<size_t>(16) * p.h_stride * 2;
-        const int ctas = lora_cluster(units, 4);
+        const int ctas = lora_cluster(lora_likely_blocks(T_, L), 2, 4);
         const size_t counts = p.blocks || p.T <= 32 ? 0 : (static_cast<size_t>(L) + 1) * (p.T > kLoraSelfPlan ? sizeof(uint4) : sizeof(uint2)), work = static_cast<size_t>(16) * ranks * sizeof(float) + (red > split ? red : split);
         return lora_launch(ranks <= 16 ? lora_rows_kernel<T, 1, true> : p.R <= 32 ? lora_rows_kernel<T, 1, false> : lora_rows_kernel<T, 2, false>, p, units * ctas, ctas, work > counts ? work : counts, stream);
     }
@@ -1144,7 +1154,9 @@ static int lora_forward(LoraParams p, int64_t T_, int64_t L, unsigned char* base
     // 82 and 73, 4096 of K=14336 N=5120 75 and 64.
     p.stages = kLoraStages * (kLoraSub + lora_stage_rows(ranks)) <= 110 * 1024 ? kLoraStages : 3;
     const size_t stages = p.stages * (kLoraSub + lora_stage_rows(ranks)), sums = static_cast<size_t>(kLoraRows) * (ranks + 4) * sizeof(float);
-    const int ctas = lora_cluster(units, 3);
+    // (a shrink of blocks of 128 rows, three CTAs an SM: with at most 1, 2, 3, 4, 8, us a call, 8192 rows of two adapters, K=4096 N=28672, rank 64, 220 208 208 216 216; of
+    // 24, rank 16, 4096 rows of K=14336 N=5120 156 95 65 65 62, 8192 of K=N=5120 108 87 87 90 89)
+    const int ctas = lora_cluster(units, 3, 3);
     const int st = lora_launch(lora_shrink_kernel<T>, p, units * ctas, ctas, 1024 + (stages > sums ? stages : sums), stream);
     if (st != EQ_OK) return st;
     const CUtensorMapDataType elem = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
