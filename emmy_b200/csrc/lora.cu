@@ -1061,16 +1061,21 @@ static size_t lora_align(size_t v) { return (v + 255) / 256 * 256; }
 static bool lora_wide(int64_t S, int64_t R) { return R <= kLoraWideRank && S <= kLoraMaxSections && S * R <= kLoraWideRanks; }
 
 // Rows of a block.  Above kLoraSelfPlan rows, 16 (lora_rows_kernel reads a block's A and B from L2 again for every 16 rows, and has one launch behind the list) up to
-// T (K + 2 N) max(R, 32) = 2 10^9 for sixteen ranks in all, 7 10^8 for more; 128 from there on.  Both forced (16 with a list, 3 us more), 16 : 128, us, prompts of 3 adapters | with 100 rows
-// that decode, of 16 adapters:
-//   K=N=4096, rank 16         1200 rows (0.47 10^9) 21 : 25 | 21 : 34, 2400 (0.94) 32 : 32 | 33 : 42, 4800 (1.9) 53 : 50 | 53 : 49
-//   K=4096 N=28672, rank 16   300 rows (0.59) 22 : 30 | 24 : 72, 600 (1.2) 38 : 37 | 40 : 73, 1200 (2.4) 63 : 48 | 67 : 89, 2400 (4.7) 105 : 71 | 112 : 113
-//   K=14336 N=4096, rank 16   600 rows (0.43) 21 : 32 | 21 : 43, 1200 (0.87) 30 : 36 | 32 : 46, 2400 (1.7) 47 : 44 | 48 : 63
-//   K=N=4096, rank 32         600 rows (0.24) 19 : 22 | 19 : 32, 1200 (0.47) 25 : 25 | 26 : 34, 2400 (0.94) 42 : 33 | 42 : 38
-//   K=N=4096, rank 64         300 rows (0.24) 18 : 21 | 18 : 30, 600 (0.47) 29 : 23 | 29 : 33, 1200 (0.94) 37 : 26 | 41 : 36
+// T (K + 2 N) max(R, 32) = 2 10^9 for sixteen ranks in all, 8 10^8 for more; 128 from there on.  The line is where prompts cross.  Requests that decode fill few rows of a
+// block of 128, and with many adapters blocks of 16 would be faster far beyond it; but how the rows lie is not known on the host.  Both forced, 16 : 128, us, prompts of 3
+// adapters | 100 rows that decode, of 16 adapters, and prompts | rows that decode in any order, of 16 | of 64; in brackets the expression in 10^9:
+//   K=N=4096, rank 16         600 rows (0.2) 11 : 23 | 11 : 33 | 12 : 31 | 17 : 61, 2400 (0.9) 35 : 34 | 34 : 42 | 33 : 59 | 36 : 88, 4800 (1.9) 54 : 50 | 53 : 50 | 53 : 83 | 56 : 87,
+//                             6000 (2.4) 59 : 54 | 59 : 58 | 61 : 88 | 64 : 94
+//   K=4096 N=28672, rank 16   300 rows (0.6) 20 : 31 | 21 : 72 | 25 : 84 | 42 : 186, 900 (1.8) 35 : 44 | 39 : 84 | 48 : 85 | 73 : 244, 1200 (2.4) 56 : 49 | 60 : 89 | 74 : 95 | 77 : 275,
+//                             2400 (4.7) 105 : 71 | 109 : 114 | 121 : 177 | 126 : 300
+//   K=14336 N=4096, rank 16   1200 rows (0.9) 27 : 37 | 28 : 46 | 27 : 49 | 30 : 117, 2400 (1.7) 52 : 45 | 52 : 64 | 39 : 70 | 55 : 128, 3600 (2.6) 59 : 53 | 59 : 69 | 60 : 85 | 63 : 121
+//   K=N=4096, rank 32         1200 rows (0.5) 22 : 27 | 22 : 35 | 23 : 38 | 25 : 78, 1800 (0.7) 23 : 29 | 24 : 37 | 25 : 42 | 27 : 87, 2400 (0.9) 43 : 34 | 43 : 38 | 35 : 60 | 46 : 89
+//   K=N=4096, rank 64         600 rows (0.5) 21 : 23 | 22 : 35 | 22 : 33 | 34 : 65, 900 (0.7) 22 : 25 | 24 : 38 | 24 : 36 | 35 : 74, 1200 (0.9) 34 : 27 | 35 : 37 | 33 : 40 | 38 : 81
+//   K=4096 N=28672, rank 64   300 rows (1.2) 40 : 33 | 40 : 75 | 41 : 85 | 68 : 193, 600 (2.4) 68 : 38 | 69 : 77 | 70 : 90 | 118 : 219
+//   K=N=5120, rank 128        300 rows (0.6) 26 : 26 | 27 : 41 | 27 : 43 | 41 : 84, 1200 (2.4) 66 : 34 | 67 : 45 | 62 : 55 | 72 : 107
 static int lora_block_rows(int64_t T, int64_t K, int64_t N, int64_t S, int64_t R) {
     if (T <= kLoraSelfPlan || !lora_wide(S, R)) return 16;
-    return static_cast<double>(T) * (K + 2 * N) * (R < 32 ? 32 : R) < (S * R <= 16 ? 2e9 : 7e8) ? 16 : kLoraRows;
+    return static_cast<double>(T) * (K + 2 * N) * (R < 32 ? 32 : R) < (S * R <= 16 ? 2e9 : 8e8) ? 16 : kLoraRows;
 }
 static bool lora_self(int64_t T, int block_rows) { return block_rows == 16 && T <= kLoraSelfRows; }
 static int64_t lora_units(int64_t T, int64_t L, int block_rows) { return group_max_blocks(T, L, block_rows, block_rows == kLoraRows); }

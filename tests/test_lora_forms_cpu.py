@@ -18,10 +18,10 @@ def test_the_lines_between_the_forms(kernel):
     assert kernel(1, 4096, 4096, 16) == kernel(256, 5120, 34816, 64, 2) == "lora_rows_kernel"
     # 257 to 2048 rows in blocks of 16: every CTA lists the blocks itself
     assert kernel(257, 1024, 520, 16) == kernel(2048, 128, 136, 16) == "lora_rows_kernel" and kernel(2049, 128, 136, 16) == forms.LIST
-    # T (K + 2 N) max(R, 32) = 2e9 with sixteen ranks in all, 7e8 with more
+    # T (K + 2 N) max(R, 32) = 2e9 with sixteen ranks in all, 8e8 with more
     assert kernel(2048, 1024, 14746, 16) == "lora_rows_kernel" and kernel(2048, 1024, 14748, 16) == forms.TILES
-    assert kernel(1000, 1000, 10437, 32) == "lora_rows_kernel" and kernel(1000, 1000, 10438, 32) == forms.TILES
-    assert kernel(1000, 1000, 10438, 8, 2) == "lora_rows_kernel" and kernel(1000, 1000, 10438, 8, 3) == forms.TILES
+    assert kernel(1000, 1000, 11999, 32) == "lora_rows_kernel" and kernel(1000, 1000, 12000, 32) == forms.TILES
+    assert kernel(1000, 1000, 12000, 8, 2) == "lora_rows_kernel" and kernel(1000, 1000, 12000, 8, 3) == forms.TILES
     # ranks that the tiles do not hold
     assert kernel(100000, 4096, 4096, 128, 2) == forms.TILES and kernel(100000, 4096, 4096, 136) == kernel(100000, 4096, 4096, 88, 3) == forms.LIST
 
