@@ -20,6 +20,8 @@
 // the row is brought to the top of f16's range by a power of two): the result is rounded once, as it is stored.
 // Up to 16 rows a block, mma.sync and not tcgen05: a decode batch is bound by the bytes of A and B and by latency, and fragments need no trip through
 // shared or tensor memory.
+#include <math.h>
+
 #include "group.cuh"
 #include "mma_sync.cuh"
 #include "tc_common.cuh"
@@ -1086,17 +1088,20 @@ static int lora_cluster(int64_t blocks, int64_t most, int64_t pairs) {
     while (ctas > 1 && blocks * ctas > (ctas > 2 ? most : pairs) * sm_count()) ctas /= 2;
     return ctas;
 }
-// Blocks of 16 rows that a call is likely to have.  (The most that it can have are T / 16 and one for each kind of rows, but not every adapter is met.)  Within two
-// CTAs an SM, which run at once; two a block within four an SM, as wide projections gain more from them than narrow ones lose.  us with clusters of 1, 2, 4, 8,
-// the one that is taken in brackets:
-//   K=N=4096, rank 16             64 rows of 64 adapters 15.7 11.3 [8.5] 12.3, 256 of 8 16.7 11.3 8.5 [7.9], 256 of 64 18.4 12.3 [9.9] 15.7, 256 of 400 23.6 [26.3] 26.6 41.3
-//     prompts of three            500 rows 17.1 12.6 9.9 [10.2], 700 19.5 13.7 [10.9] 16.0, 1200 23.9 [17.7] 20.5 25.3, 2000 26.3 [19.8] 24.9 39.9, 3200 33.1 [37.9] 37.5 56.0
-//   K=14336 N=4096, rank 16       64 of 64 31.1 19.1 [13.0] 16.7, 200 of 200 37.9 [24.2] 27.6 37.9, 256 of 400 39.9 [43.0] 40.3 54.3
-//   K=4096 N=28672, rank 64       64 of 64 163 103 [64] 68, 128 of 128 196 [116] 112 100, 256 of 64 178 108 [71] 78, 256 of 400 225 [209] 179 193
+// Blocks of 16 rows that a call is likely to have: the kinds of rows that T draws out of L + 1 meet, with one block each or half a block more than they fill.
 static int64_t lora_likely_blocks(int64_t T, int64_t L) {
-    const int64_t kinds = L + 1 < T ? L + 1 : T;
-    return T / 16 + kinds * 3 / 4;
+    const double kinds = static_cast<double>(L + 1), met = kinds * (1 - exp(-T / kinds)), filled = T / met / 16 + 0.5;
+    return static_cast<int64_t>(ceil(met * (filled < 1 ? 1 : filled)));
 }
+// Within two CTAs an SM, which run at once; projections of 5120 columns and more keep two a block up to four an SM.  us with clusters of 1, 2, 4, 8, the one that is
+// taken in brackets:
+//   K=N=4096, rank 16             64 rows of 64 adapters 15.7 11.3 [8.5] 12.3, 256 of 8 16.7 11.3 8.5 [7.9], 256 of 64 18.4 12.3 [9.9] 15.7, 256 of 400 [23.6] 26.3 26.6 41.3
+//     prompts of three            500 rows 17.1 12.6 9.9 [10.2], 700 19.5 13.7 [10.9] 16.0, 1200 23.9 [17.7] 20.5 25.3, 2000 26.3 [19.8] 24.9 39.9, 3200 [33.1] 37.9 37.5 56.0
+//   K=14336 N=4096, rank 16       64 of 64 31.1 19.1 [13.0] 16.7, 200 of 200 37.9 [24.2] 27.6 37.9, 256 of 400 [39.9] 43.0 40.3 54.3
+//   K=4096 N=28672, rank 64       64 of 64 163 103 [64] 68, 128 of 128 196 [116] 112 100, 256 of 64 178 108 [71] 78, 256 of 400 225 [209] 179 193
+// and 1 : 2 with more blocks than SMs, 256 rows of 256 and of 400 adapters, 2400 mixed rows of 100, rank 16: K=1024 N=1024 9 : 11, 9 : 13, 16 : 19, N=4096 17 : 17, 18 : 21, 28 : 30,
+// N=5120 26 : 22, 28 : 23, 33 : 37, N=8192 37 : 27, 38 : 30, 43 : 44; K=4096 N=4096 23 : 23, 24 : 26, 32 : 35, N=8192 38 : 31, 39 : 36, 47 : 48.
+static int lora_rows_cluster(int64_t T, int64_t L, int64_t N) { return lora_cluster(lora_likely_blocks(T, L), 2, N >= 5120 ? 4 : 2); }
 
 static int lora_launch(void (*kernel)(const LoraParams), const LoraParams& p, int64_t grid, int cluster, size_t smem, cudaStream_t stream) {
     if (smem > kSmemUnasked) EQ_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024));
@@ -1151,7 +1156,7 @@ static int lora_forward(LoraParams p, int64_t T_, int64_t L, unsigned char* base
     if (block_rows == 16) {
         p.h_stride = (ranks + 63) / 64 * 64 + 32;  // rows 64 bytes apart modulo 128: the 16-byte reads of two rows meet every bank once
         const size_t red = static_cast<size_t>(kLoraWarps) * 16 * (kLoraPass + 8) * sizeof(float), split = 2 * static_cast<size_t>(16) * p.h_stride * 2;
-        const int ctas = lora_cluster(lora_likely_blocks(T_, L), 2, 4);
+        const int ctas = lora_rows_cluster(T_, L, p.N);
         const size_t counts = p.blocks || p.T <= 32 ? 0 : (static_cast<size_t>(L) + 1) * (p.T > kLoraSelfPlan ? sizeof(uint4) : sizeof(uint2)), work = static_cast<size_t>(16) * ranks * sizeof(float) + (red > split ? red : split);
         return lora_launch(ranks <= 16 ? lora_rows_kernel<T, 1, true> : p.R <= 32 ? lora_rows_kernel<T, 1, false> : lora_rows_kernel<T, 2, false>, p, units * ctas, ctas, work > counts ? work : counts, stream);
     }
