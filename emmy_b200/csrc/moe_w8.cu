@@ -1028,7 +1028,10 @@ static W8Form w8_form(int64_t T, int64_t E, int64_t topk, int64_t H, int64_t I, 
     // top 8, 768 28.4 : 27.5, 2304 55 : 50, 12288 135 : 119; 128 of 1280 x 768, 768 24.6 : 23.2, 2304 47 : 41; below, nothing in it (32 of 2048 x 512, top 4, 384
     // 18.9 : 18.9; 8 of 2048 x 256, top 2, 256 14.6 : 15.7).  Narrower layers have few slabs of thirty-two channels, in clusters of eight: 32 of 1024 x 512, 384
     // 16.0 : 20.7, 768 18.6 : 24.1, 1536 23.2 : 23.4; 128 of 1024 x 768, 2304 35.5 : 32.9, 7680 68 : 59, 12288 (32 tokens) 80 : 90; of 640 x 768, 3072 35 : 31.
-    f.wide = R * (I / 16) >= (H >= 1280 ? 4 : 16) * sms;
+    // And clusters of four do not pack into all slots of two CTAs an SM: 256 experts of 2304 x 896, top 8, whose down product has 288, 1344 42.8 : 47.1, 2688
+    // 71.7 : 76.9, 14336 225 : 260 (with 272, of 2176 x 896, 42.1 : 39.1, 69.9 : 62.8; 209 : 237 at 32 tokens).
+    const int64_t fours = 4 * (H / 32);
+    f.wide = R * (I / 16) >= (H >= 1280 ? 4 : 16) * sms && !(fours <= 2 * sms && fours > 2 * sms * 15 / 16);
     // CTAs that route and convert for themselves, no launch ahead of them: where one of either product, with its activations, fits an SM beside the other
     // (228 KB; 1 KB of each is the system's, up to 256 bytes are static), and the down product's slabs of sixteen channels are no more than SMs.  Without
     // and with, us: 128 experts of 2048 x 768, a token, top 8 18.7 : 17.7, two, top 4 20.7 : 18.9; 64 of 2048 x 1024, three of f16, top 2 19.4 : 16.4, four (too large

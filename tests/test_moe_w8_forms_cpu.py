@@ -24,6 +24,8 @@ def test_the_lines_between_the_forms(kernel):
     # picks x I / 16 from sixteen an SM on, from four where the layer is 1280 wide
     assert kernel(16, 128, 4, 1152, 576) == forms.DOWN and kernel(16, 128, 4, 1152, 592) == forms.WIDE
     assert kernel(4, 128, 4, 1280, 576) == forms.DOWN and kernel(4, 128, 4, 1280, 592) == forms.WIDE
+    # and not with 278 to 296 CTAs in clusters of four
+    assert kernel(32, 128, 8, 2176, 768) == kernel(32, 128, 8, 2432, 768) == forms.WIDE and kernel(32, 128, 8, 2304, 768) == forms.DOWN
     assert kernel(32, 256, 1, 512, 256) == forms.DOWN and kernel(33, 256, 1, 512, 256) == kernel(1, 257, 1, 512, 256) == kernel(1, 8, 1, 512, 65664) == forms.EIGHT
     assert kernel(144, 128, 8, 2048, 768) == forms.EIGHT and kernel(145, 128, 8, 2048, 768) == forms.SIXTEEN
 
