@@ -1033,13 +1033,13 @@ static W8Form w8_form(int64_t T, int64_t E, int64_t topk, int64_t H, int64_t I, 
     const int64_t fours = 4 * (H / 32);
     f.wide = R * (I / 16) >= (H >= 1280 ? 4 : 16) * sms && !(fours <= 2 * sms && fours > 2 * sms * 15 / 16);
     // CTAs that route and convert for themselves, no launch ahead of them: where one of either product, with its activations, fits an SM beside the other
-    // (228 KB; 1 KB of each is the system's, up to 256 bytes are static), and the down product's slabs of sixteen channels are no more than SMs.  Without
+    // (228 KB; 1 KB of each is the system's, 192 bytes of both are static), and the down product's slabs of sixteen channels are no more than SMs.  Without
     // and with, us: 128 experts of 2048 x 768, a token, top 8 18.7 : 17.7, two, top 4 20.7 : 18.9; 64 of 2048 x 1024, three of f16, top 2 19.4 : 16.4, four (too large
-    // by 1 KB) 22.3 : 23.4; 8 of 2048 x 2048, two of f16 19.8 : 17.3; 32 of 1024 x 512, top 4, three 15.9 : 15.7, four (too large) 16.4 : 18.4; more slabs than
-    // SMs: 8 of 4096 x 4096, one, top 1 20.9 : 22.8, 32 of 5120 x 768, one of f16, top 8 32.3 : 45.3.
-    constexpr size_t kSm = 228 * 1024, kBeside = 1024 + 256;
+    // by 1 KB) 22.3 : 23.4; 8 of 2048 x 2048, two of f16 19.8 : 17.3; 8 of 2304 x 512, top 8, two of f16 (96 bytes are left) 18.4 : 16.9; 32 of 1024 x 512, top 4,
+    // three 15.9 : 15.7, four (too large) 16.4 : 18.4; more slabs than SMs: 8 of 4096 x 4096, one, top 1 20.9 : 22.8, 32 of 5120 x 768, one of f16, top 8 32.3 : 45.3.
+    constexpr size_t kSm = 228 * 1024, kBeside = 2 * 1024 + 256;
     f.own = f.self && !f.wide && H / 16 <= sms &&
-            w8_tiles_smem(1, 1, true, true) + kW8Plan + w8_own_x(T, H, f16) + w8_down_smem(T, 1, true, true) + w8_own_h(R, I) + 2 * kBeside <= kSm;
+            w8_tiles_smem(1, 1, true, true) + kW8Plan + w8_own_x(T, H, f16) + w8_down_smem(T, 1, true, true) + w8_own_h(R, I) + kBeside <= kSm;
     // Sixteen rows a block where experts have that many: the weights of an expert with nine to sixteen rows are read and expanded once and not twice, but half as
     // far ahead.  128 experts of 2048 x 768, top 8, us a layer with 8 and 16: 96 tokens 149 and 171, 128 174 and 176, 144 180 and 180, 160 193 and 180, 200 236 and
     // 189, 256 298 and 230; 64 experts, top 6: 96 tokens 161 and 165, 128 193 and 182.

@@ -16,9 +16,10 @@ def kernel():
 
 def test_the_lines_between_the_forms(kernel):
     assert kernel(1, 128, 8, 2048, 768) == forms.OWN and kernel(2, 128, 8, 2048, 768) == kernel(2, 128, 8, 2048, 768, True) == forms.WIDE
-    # a CTA of either launch on an SM, f16 activations beside them: 233472 bytes for 199328 and 512 a token
+    # a CTA of either launch on an SM, f16 activations beside them: 233472 bytes for 199072 and 512 a token
     assert kernel(2, 128, 4, 2048, 768) == forms.OWN and kernel(4, 64, 2, 2048, 1024, True) == forms.DOWN and kernel(3, 64, 2, 2048, 1024, True) == forms.OWN
     assert kernel(3, 64, 2, 2048, 1024) == forms.DOWN and kernel(2, 8, 2, 2048, 2048, True) == forms.OWN and kernel(2, 8, 2, 2048, 2048) == forms.DOWN
+    assert kernel(2, 8, 8, 2304, 512, True) == forms.OWN and kernel(2, 8, 8, 2304, 640, True) == forms.DOWN
     # and no more slabs of sixteen channels than SMs
     assert kernel(1, 32, 1, 2304, 512) == forms.OWN and kernel(1, 32, 1, 2432, 512) == kernel(1, 32, 1, 5120, 128, True) == forms.DOWN
     # picks x I / 16 from sixteen an SM on, from four where the layer is 1280 wide
