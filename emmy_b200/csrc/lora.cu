@@ -3,7 +3,8 @@
 // A projection that holds several linears side by side (q, k and v; gate and up) has one A per linear: section s of the columns reads
 // A_l[s], B_l is [N, R] over all of them.
 //
-// Up to 256 rows, and up to 2048 where blocks have 16 rows (lora_block_rows), one launch, lora_rows_kernel.  A unit is a block of at most 16 rows of one adapter; a cluster of CTAs works on it:
+// Up to 256 rows, and up to 2048 where blocks have 16 rows (lora_block_rows), one launch, lora_rows_kernel.  A unit is a block of at most 16 rows of
+// one adapter; a cluster of CTAs works on it:
 //   rows     which rows share an adapter is worked out by every CTA from the ids alone (a row's rank among the rows of its adapter, by a match in its
 //            warp and a table of the warps' counts; the rows whose rank is a multiple of 16 open a block).
 //   shrink   h = A_l x by mma.sync m16n8k16 (rows as M, ranks as N), K cut over all warps of the cluster: every byte of x and A_l is
@@ -13,9 +14,13 @@
 //   expand   every CTA takes a share of the columns in groups of 32: rows as M, columns as N, R as K.  The columns of a group are dealt
 //            to the four MMA tiles so that a lane ends with eight neighbouring ones: y is read and written 16 bytes at a time.  The
 //            next group's B and y are on their way while a group is multiplied, the first one's before the CTAs have met.
-// Above, two, the first of them group.cu's list of the blocks (1999 rows of K=N=5120, rank 16: 26 us, 23 with the list made by every CTA); for larger calls three: blocks of at most 128 rows, lora_shrink_kernel
-// writes h, lora_expand_kernel adds B h to y in tiles of 128 rows x 128 columns.  Both products run on tcgen05.  The shrink's threads gather the rows of a
-// block, which lie anywhere, by cp.async into the swizzled tile that the MMA reads, three to six steps ahead; the expand's tiles come and go by TMA.
+// Above, two, the first of them group.cu's list of the blocks (1999 rows of K=N=5120, rank 16: 26 us, 23 with the list made by every CTA); for larger
+// calls three: blocks of at most 128 rows, lora_shrink_kernel writes h, lora_expand_kernel adds B h to y in tiles of 128 rows x 128 columns.  Both products
+// run on tcgen05.  The shrink's threads gather the rows of a block, which lie anywhere, by cp.async into the swizzled tile that the MMA reads, three to six
+// steps ahead; the expand's tiles come and go by TMA.
+// The tiles hold up to 256 ranks in all and 128 of a section.  More stay in blocks of 16 rows at any size, whose A and B come from L2 again for each: 8192 rows,
+// prompts of 3 adapters, K=4096, us (bytes at the rate of HBM): N = 4096 + 1024 + 1024 of rank 128 400 (43), N=4096 of rank 256 356 (33); 4096 + 1024 of rank
+// 128, on the tiles, 112 (37).
 // h is kept in f32 and enters the second product as two 16-bit numbers, value and remainder (bf16: 16 bits of fraction, f16: 22, after
 // the row is brought to the top of f16's range by a power of two): the result is rounded once, as it is stored.
 // Up to 16 rows a block, mma.sync and not tcgen05: a decode batch is bound by the bytes of A and B and by latency, and fragments need no trip through
@@ -230,7 +235,7 @@ __device__ __forceinline__ uint4 lora_add8(uint4 v, const float (&acc)[4][4], in
 
 // ------------------------------------------------------------------------------------------------ blocks of 16 rows
 // Bound by latency for few bytes: one row of K=N=4096, rank 16, takes 5.0 us a launch beside 0.04 us of bytes, 17 rows of K=14336 N=4096, rank 32, 7.9 us (0.8), and
-// by how soon A's and B's bytes are asked for: 256 rows of 64 adapters, K=5120 N=34816, rank 64, 83 us for 396 MB, 4.8 TB/s.  With four warps a scheduler the
+// by how soon A's and B's bytes are asked for: 256 rows of 64 adapters, K=5120 N=34816, rank 64, 84 us for 396 MB, 4.7 TB/s.  With four warps a scheduler the
 // instructions between two loads are part of that latency: 64-bit divisions of the shares and zeros for what nobody stores were a fifth of either time.
 // kSmall: no more than sixteen ranks in all, half the fragments, so more of them are asked for at once.
 // kChunks: of 32 ranks, what a lane asks for at a time; one where there are no more (K=14336 N=4096, rank 32, 17 rows 8.8 us against 10.2; three CTAs an
@@ -1157,8 +1162,10 @@ static int lora_forward(LoraParams p, int64_t T_, int64_t L, unsigned char* base
         p.h_stride = (ranks + 63) / 64 * 64 + 32;  // rows 64 bytes apart modulo 128: the 16-byte reads of two rows meet every bank once
         const size_t red = static_cast<size_t>(kLoraWarps) * 16 * (kLoraPass + 8) * sizeof(float), split = 2 * static_cast<size_t>(16) * p.h_stride * 2;
         const int ctas = lora_rows_cluster(T_, L, p.N);
-        const size_t counts = p.blocks || p.T <= 32 ? 0 : (static_cast<size_t>(L) + 1) * (p.T > kLoraSelfPlan ? sizeof(uint4) : sizeof(uint2)), work = static_cast<size_t>(16) * ranks * sizeof(float) + (red > split ? red : split);
-        return lora_launch(ranks <= 16 ? lora_rows_kernel<T, 1, true> : p.R <= 32 ? lora_rows_kernel<T, 1, false> : lora_rows_kernel<T, 2, false>, p, units * ctas, ctas, work > counts ? work : counts, stream);
+        const size_t counts = p.blocks || p.T <= 32 ? 0 : (static_cast<size_t>(L) + 1) * (p.T > kLoraSelfPlan ? sizeof(uint4) : sizeof(uint2));
+        const size_t work = static_cast<size_t>(16) * ranks * sizeof(float) + (red > split ? red : split);
+        return lora_launch(ranks <= 16 ? lora_rows_kernel<T, 1, true> : p.R <= 32 ? lora_rows_kernel<T, 1, false> : lora_rows_kernel<T, 2, false>, p, units * ctas, ctas,
+                           work > counts ? work : counts, stream);
     }
     // Steps ahead: six where two CTAs an SM have room for them.  24 adapters of rank 16, prompts, us a call with three and with six: 8192 rows of K=N=5120
     // 82 and 73, 4096 of K=14336 N=5120 75 and 64.

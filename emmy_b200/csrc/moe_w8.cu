@@ -10,7 +10,8 @@
 // instructions per 2 KB of weights beside the 89 cycles that HBM needs for them: 123 us.  m16n8k32 on e4m3 parts of the activations converts both
 // operands inside every MMA: 189 us.)
 //
-// What bounds it: the bytes of the picked experts, as long as few rows share one.  5 tokens of 8 experts of 4096 x 14336 stream them at 5.5 TB/s (194 us),
+// What bounds it: the bytes of the picked experts, as long as few rows share one.  5 tokens of 8 experts of 4096 x 14336 stream them at 5.0 to 5.2 TB/s (five of them
+// picked 176 us, seven 242),
 // 16 tokens as above at 4.5 beside routing, the seam of the two products and their ends; one token (38 MB, 17.6 us, 5.8 at the rate of HBM) is a chain of latencies,
 // of which routing takes 2.8 us, the seam with the split of silu * up 2 and each product 4.  With more rows the MMAs' operands: 200 tokens 189 us for 93 of bytes.
 //
@@ -22,8 +23,8 @@
 //            memory in warp order.
 //   down     A cluster of CTAs has sixteen output channels of ALL the blocks: the picks of a token meet inside it (f32, a fixed order), y is written
 //            once, and nothing is combined in memory.  It has grouped the picks and asked for its first weights before the launch ahead of it ends.
-// Where a CTA of either launch fits an SM with f16 activations of its own (w8_form) these two launches are the layer, one CTA an SM each, so that the second one is resident, has routed
-// too and asked for its first weights while the first one runs.  Else w8_prep_kernel routes the tokens and brings x (of bf16) to f16 ahead of them.
+// Where a CTA of either launch fits an SM with f16 activations of its own (w8_form) these two launches are the layer, one CTA an SM each, so that the second
+// one is resident, has routed too and asked for its first weights while the first one runs.  Else w8_prep_kernel routes the tokens and brings x (of bf16) to f16 ahead of them.
 // Then no launch has to come between the two: the rows' largest values are found as they are written, and the second one splits what it reads of them.
 // Above, w8_prep_kernel and group.cu list the blocks, w8_parts_kernel splits the rows of silu * up (there are so many CTAs for each row that they would do it
 // many times: 64 tokens of 128 experts of 2048 x 768 152 us for 143), and both products run as streams of tiles; the down rows go to memory in f32 and

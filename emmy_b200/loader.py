@@ -456,18 +456,26 @@ def load_experts(index: CheckpointIndex, experts: dict[int, dict[str, LinearSpec
 # ---------------------------------------------------------------------------------------------- low-rank adapters
 
 # what an adapter's configuration may hold; of the ways to initialise A and B those that leave the base as it was
-_ADAPTER_PLAIN = (("bias", (None, "none")), ("lora_bias", (None, False)), ("use_dora", (None, False)), ("use_qalora", (None, False)),
-                  ("alora_invocation_tokens", (None, [])), ("fan_in_fan_out", (None, False)), ("modules_to_save", (None, [])), ("layer_replication", (None, [])), ("init_lora_weights", (None, True, False, "gaussian", "eva", "orthogonal")))
+_ADAPTER_PLAIN = (
+    ("bias", (None, "none")),
+    ("lora_bias", (None, False)),
+    ("use_dora", (None, False)),
+    ("use_qalora", (None, False)),
+    ("alora_invocation_tokens", (None, [])),
+    ("fan_in_fan_out", (None, False)),
+    ("modules_to_save", (None, [])),
+    ("layer_replication", (None, [])),
+    ("init_lora_weights", (None, True, False, "gaussian", "eva", "orthogonal")),
+)
 _ADAPTER_RE = re.compile(r"^(?:base_model\.model\.)?(?P<module>.+)\.lora_(?P<ab>[AB])\.weight$")
 
 
 def read_adapter(adapter_dir) -> dict[str, tuple[torch.Tensor, torch.Tensor, float]]:
     """module path -> (A [r, K], B [N, r], scaling) of a low-rank adapter directory, on the host.  scaling = alpha / r, or alpha / sqrt(r)
-    with `use_rslora`, alpha by `alpha_pattern` where an entry names the module (path or dotted suffix), 8 where the
-    configuration names none.  What is not such a product
-    (trained biases, embeddings or saved modules, a magnitude vector, transposed weights, inputs averaged by groups, rows that are adapted
-    behind certain tokens only) raises, and so does an adapter whose making
-    changed its base (`init_lora_weights` of pissa, olora, corda, loftq and the like): beside the checkpoint's own base it is another one."""
+    with `use_rslora`, alpha by `alpha_pattern` where an entry names the module (path or dotted suffix), 8 where the configuration names none.
+    What is not such a product (trained biases, embeddings or saved modules, a magnitude vector, transposed weights, inputs averaged by groups,
+    rows that are adapted behind certain tokens only) raises, and so does an adapter whose making changed its base (`init_lora_weights` of pissa,
+    olora, corda, loftq and the like): beside the checkpoint's own base it is another one."""
     cfg = json.loads((Path(adapter_dir) / "adapter_config.json").read_text())
     if cfg.get("peft_type", "LORA") != "LORA":
         raise ValueError(f"adapter of type {cfg['peft_type']!r}, not LORA")
