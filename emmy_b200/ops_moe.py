@@ -148,7 +148,9 @@ def moe_w8a16(x, router_logits, gate_up, gate_up_scale, down, down_scale, topk: 
     lib = L.load()
     piece = t
     if workspace is None:
-        piece = min(t, _W8_PIECE)
+        shift = abs(out.data_ptr() - x.data_ptr())
+        if shift == 0 or shift >= 2 * t * h:  # (a piece's result on the rows of a later one: all of them at once, x is read before y is written)
+            piece = min(t, _W8_PIECE)
         workspace = _scratch(lib.eq_moe_w8a16_workspace_bytes(piece, e, topk, h, i), x.device)
     for t0 in range(0, t, piece) if t else (0,):
         status = lib.eq_moe_w8a16(

@@ -64,3 +64,17 @@ def test_a_prompt_in_pieces_captured():
             v.copy_(a)
         graph.replay()
         assert torch.equal(y, ref)
+
+
+def test_a_result_that_overlaps_its_input():
+    """As it was before prompts came in pieces: rows of the result on other rows of x."""
+    e, topk, h, i, t = 8, 2, 256, 256, 5000
+    w, _ = tm.experts(e, h, i, True, seed=3)
+    x, logits = tm.inputs(t, e, h, BF16, seed=3)
+    ws = torch.empty(1 << 30, dtype=torch.uint8, device="cuda")
+    want = tm.call(x, logits, w, topk, workspace=ws)
+    for shift in (-1000, 1000):
+        both = torch.zeros(t + 2000, h, dtype=BF16, device="cuda")
+        held, out = both[1000 : 1000 + t], both[1000 + shift : 1000 + shift + t]
+        held.copy_(x)
+        assert torch.equal(tm.call(held, logits, w, topk, out=out), want)
