@@ -1028,7 +1028,7 @@ static W8Form w8_form(int64_t T, int64_t E, int64_t topk, int64_t H, int64_t I, 
     // sixteen and thirty-two, by R I / 16.  H from 1280 on: 16 experts of 2048 x 2816, top 4, 1408 40.1 : 36.6, 5632 67 : 62, 22528 110 : 93; 128 of 2048 x 768,
     // top 8, 768 28.4 : 27.5, 2304 55 : 50, 12288 135 : 119; 128 of 1280 x 768, 768 24.6 : 23.2, 2304 47 : 41; below, nothing in it (32 of 2048 x 512, top 4, 384
     // 18.9 : 18.9; 8 of 2048 x 256, top 2, 256 14.6 : 15.7).  Narrower layers have few slabs of thirty-two channels, in clusters of eight: 32 of 1024 x 512, 384
-    // 16.0 : 20.7, 768 18.6 : 24.1, 1536 23.2 : 23.4; 128 of 1024 x 768, 2304 35.5 : 32.9, 7680 68 : 59, 12288 (32 tokens) 80 : 90; of 640 x 768, 3072 35 : 31.
+    // 16.0 : 20.7, 768 18.6 : 24.1, 1536 23.2 : 23.4; 128 of 1024 x 768, 2304 35.5 : 32.9, 7680 68 : 59, 12288 (32 tokens) 80 : 90; of 640 x 768, 4608 43 : 38.
     // And clusters of four do not pack into all slots of two CTAs an SM: 256 experts of 2304 x 896, top 8, whose down product has 288, 1344 42.8 : 47.1, 2688
     // 71.7 : 76.9, 14336 225 : 260 (with 272, of 2176 x 896, 42.1 : 39.1, 69.9 : 62.8; 209 : 237 at 32 tokens).
     const int64_t fours = 4 * (H / 32);
